@@ -75,6 +75,19 @@ class bt_attn_args(Structure):
         super().__init__(ctypes.sizeof(type(self)), *args, **kw)    # struct_size first; positional fields follow as before
 
 
+class bt_kv8_cache(Structure):
+    _fields_ = [("struct_size", c_uint32), ("block", c_int32), ("kv_heads", c_int32), ("head_dim", c_int32), ("batch", c_int64),
+                ("n_max", c_int64), ("k_codes", c_void_p), ("v_codes", c_void_p), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("k_tail", c_void_p), ("v_tail", c_void_p)]
+
+    def __init__(self, *args, **kw):
+        super().__init__(ctypes.sizeof(type(self)), *args, **kw)    # struct_size: the library rejects any other value
+
+
+class bt_kv8_rows(Structure):
+    _fields_ = [("p", c_void_p), ("b_stride", c_int64), ("t_stride", c_int64), ("h_stride", c_int64)]
+
+
 _SIGS = {
     "bt_version": (c_int, []),
     "bt_last_error": (c_char_p, []),
@@ -114,6 +127,19 @@ _SIGS = {
                                  c_void_p, c_int64, c_void_p, c_int64, c_void_p]),
     "bt_topk_sample": (c_int, [c_int, c_int64, c_int64, c_void_p, c_int64, c_float, c_int32, c_uint64, c_void_p, c_int64,
                                c_void_p, c_int64, c_void_p]),
+    "bt_quant_rows": (c_int, [c_int, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_float, c_void_p, c_int64, c_void_p,
+                              c_void_p]),
+    "bt_linear_q8_scratch_bytes": (c_int64, [c_int64, c_int64, c_int64]),
+    "bt_linear_q8": (c_int, [c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_void_p, c_void_p,
+                             c_void_p, c_int64, c_void_p, c_int64, c_int, c_void_p, c_int64, c_void_p]),
+    "bt_kv8_append": (c_int, [c_int, POINTER(bt_kv8_cache), c_int32, c_int32, POINTER(bt_kv8_rows), POINTER(bt_kv8_rows),
+                              POINTER(bt_kv8_rows), POINTER(bt_kv8_rows), c_void_p, c_int32, c_void_p, c_int32, c_void_p, c_void_p,
+                              c_int64, c_void_p]),
+    "bt_kv8_read": (c_int, [c_int, POINTER(bt_kv8_cache), c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p]),
+    "bt_attention_kv8_split_count": (c_int32, [c_int64, c_int32, c_int32, c_int32, c_int64]),
+    "bt_attention_kv8_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32, c_int32]),
+    "bt_attention_kv8": (c_int, [c_int, POINTER(bt_kv8_cache), c_int32, c_int32, POINTER(bt_kv8_rows), c_void_p, c_int32, c_void_p,
+                                 c_int64, c_void_p, c_int64, c_int32, c_void_p, c_int64, c_void_p]),
     "bt_decoder_forward": (c_int, [c_int, POINTER(bt_decoder_dims), POINTER(bt_decoder_weights), c_int64, c_int32,
                                    c_void_p, POINTER(bt_attn_args), c_int32, c_void_p, c_void_p, c_int64, c_void_p]),
     "bt_finish_block": (c_int, [c_int64, c_int32, c_int32, c_void_p, c_void_p, c_int64, c_void_p, c_void_p, c_void_p,

@@ -3,7 +3,9 @@
 torch is used for device memory and streams only; no arithmetic runs in ATen here."""
 from __future__ import annotations
 
-from typing import Optional
+import contextlib
+import ctypes
+from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -171,3 +173,227 @@ def rope_tables(max_pos: int, rot: int, base: float, device) -> torch.Tensor:
     inv_freq = 1.0 / (base ** (torch.arange(0, rot, 2, dtype=torch.float32) / rot))
     freqs = torch.outer(torch.arange(max(max_pos, 1), dtype=torch.float32), inv_freq)
     return torch.stack([freqs.cos(), freqs.sin()]).contiguous().to(device)
+
+
+# ---- 8-bit serving ----------------------------------------------------------------------------------------------------------------
+_ON_DEVICE = contextlib.nullcontext()
+
+
+def _on(device, *tensors):
+    """A context in which `device` is the current one; every tensor (None: left out) has to live there."""
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise _lib.BtError(f"all tensors must be on {device}, got one on {t.device}")
+    if device.type != "cuda":
+        raise _lib.BtError("libbt_hip operates on GPU memory only; got a CPU tensor (move the model/inputs to 'cuda')")
+    return _ON_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _expect(t: torch.Tensor, what: str, shape, dtype) -> None:
+    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+        raise _lib.BtError(f"{what} must be contiguous {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
+
+
+def quantize_rows(x: torch.Tensor, ln_w: Optional[torch.Tensor] = None, ln_b: Optional[torch.Tensor] = None, eps: float = 1e-5):
+    """(codes, scales) of the rows of ``x`` [..., K] -- of LayerNorm(x; ln_w, ln_b, eps) if weights are given -- in 8-bit integers with one
+    scale per row: codes int8 [..., round_up(K, 16)] (zero behind column K), scales float32 [...].  Activations and weights alike:
+    ``quantize_rows(weight)`` has one scale per output channel.  A row with an infinity or NaN in it gets scale NaN."""
+    if x.dim() and x.shape[-1] == 0:
+        raise _lib.BtError("rows are empty")
+    x2, ldx = _rows(x)
+    M, K = x2.shape
+    if (ln_w is None) != (ln_b is None):
+        raise _lib.BtError("LayerNorm needs ln_w and ln_b")
+    for w in (ln_w, ln_b):
+        if w is not None:
+            _expect(w, "LayerNorm weight", (K,), x.dtype)
+    Kp = (K + 15) // 16 * 16
+    with _on(x.device, ln_w, ln_b):
+        codes = torch.empty(x.shape[:-1] + (Kp,), dtype=torch.int8, device=x.device)
+        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        check(lib().bt_quant_rows(dtype_code(x.dtype), M, K, ptr(x2), ldx, ptr(ln_w), ptr(ln_b), float(eps), ptr(codes), Kp, ptr(scales),
+                                  current_stream()), "bt_quant_rows")
+    return codes, scales
+
+
+def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight: Tuple[torch.Tensor, torch.Tensor],
+              bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, act: str = "none",
+              out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None, scratch: Optional[torch.Tensor] = None):
+    """out = act(x @ weight.T + bias) + residual in 8-bit integers with scales per token and per output channel.  ``x``: rows in fp32 or
+    bf16 (quantised here) or the (codes, scales) that ``quantize_rows`` made of them; ``weight``: ``quantize_rows`` of the nn.Linear
+    weight [N, K].  The sum over K is exact; ``dtype`` (default: that of x, bias, residual or out, whichever is a float tensor) is the
+    type of bias, residual and result.  ``scratch`` (any dtype, >= bt_linear_q8_scratch_bytes) is allocated when it is needed and not
+    given."""
+    wc, ws = weight
+    if isinstance(x, torch.Tensor):
+        dtype = dtype or x.dtype
+        if x.shape[-1] > wc.shape[-1] or (x.shape[-1] + 15) // 16 * 16 != wc.shape[-1]:
+            raise _lib.BtError(f"x has {x.shape[-1]} columns, the weight's rows of codes {wc.shape[-1]}")
+        x = quantize_rows(x)
+    xc, xs = x
+    if dtype is None:
+        dtype = next((t.dtype for t in (out, residual, bias) if t is not None), None)
+        if dtype is None:
+            raise _lib.BtError("quantised x without bias, residual or out: say which dtype the result has")
+    code = dtype_code(dtype)
+    if xc.dtype != torch.int8 or wc.dtype != torch.int8 or xs.dtype != torch.float32 or ws.dtype != torch.float32:
+        raise _lib.BtError("quantised operands are (int8 codes, float32 scales)")
+    a2, lda = _rows(xc)
+    lda = lda if a2.shape[0] > 1 else a2.shape[1]     # the stride of one row says nothing
+    if wc.dim() != 2 or wc.stride(1) != 1:
+        raise _lib.BtError("weight codes must be [N, K] with unit inner stride")
+    M, K = a2.shape
+    N = wc.shape[0]
+    if wc.shape[1] != K:
+        raise _lib.BtError(f"codes of x have {K} columns, those of the weight {wc.shape[1]}")
+    if xs.numel() != M or ws.numel() != N or not xs.is_contiguous() or not ws.is_contiguous():
+        raise _lib.BtError("one contiguous scale per row of codes is needed")
+    if act not in ("none", "gelu"):
+        raise _lib.BtError(f"unknown activation {act!r}")
+    if bias is not None:
+        _expect(bias, "bias", (N,), dtype)
+    shape = xc.shape[:-1] + (N,)
+    r2, ldr = None, 0
+    if residual is not None:
+        if residual.shape != shape or residual.dtype != dtype:
+            raise _lib.BtError(f"residual must be {dtype} {tuple(shape)}")
+        r2, ldr = _rows(residual)
+    with _on(xc.device, xs, wc, ws, bias, residual, out, scratch):
+        if out is None:
+            out = torch.empty(shape, dtype=dtype, device=xc.device)
+        elif out.shape != shape or out.dtype != dtype:
+            raise _lib.BtError(f"out must be {dtype} {tuple(shape)}")
+        o2, ldo = _rows(out)
+        if scratch is None:
+            need = int(lib().bt_linear_q8_scratch_bytes(M, N, K))
+            if need:
+                scratch = torch.empty(need, dtype=torch.uint8, device=xc.device)
+        check(lib().bt_linear_q8(code, M, N, K, ptr(a2), lda, ptr(xs), ptr(wc), wc.stride(0) if N > 1 else K, ptr(ws), ptr(bias), ptr(r2), ldr, ptr(o2), ldo,
+                                 _lib.BT_ACT_GELU if act == "gelu" else _lib.BT_ACT_NONE, ptr(scratch),
+                                 0 if scratch is None else scratch.numel() * scratch.element_size(), current_stream()), "bt_linear_q8")
+    return out
+
+
+def _kv8(kv: Sequence[torch.Tensor]):
+    """(bt_kv8_cache, dtype code) of one layer of an 8-bit cache: (k_codes, v_codes, k_scale, v_scale, k_tail, v_tail)."""
+    kc, vc, ks, vs, kt, vt = kv
+    if kc.dim() != 4 or kt.dim() != 4:
+        raise _lib.BtError("a layer of an 8-bit cache is (k_codes, v_codes, k_scale, v_scale, k_tail, v_tail), see runtime.KV8Cache")
+    B, H, n_max, d = kc.shape
+    block = kt.shape[2]
+    if block == 0 or n_max % block:
+        raise _lib.BtError(f"{n_max} rows are not a whole number of blocks of {block}")
+    for t, what, shape, dtype in ((kc, "k_codes", (B, H, n_max, d), torch.int8), (vc, "v_codes", (B, H, n_max // block, d, block), torch.int8),
+                                  (ks, "k_scale", (B, H, n_max // block), torch.float32), (vs, "v_scale", ks.shape, torch.float32),
+                                  (kt, "k_tail", (B, H, block, d), kt.dtype), (vt, "v_tail", (B, H, d, block), kt.dtype)):
+        if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
+            _expect(t, what, shape, dtype)
+    return _lib.bt_kv8_cache(block, H, d, B, n_max, ptr(kc), ptr(vc), ptr(ks), ptr(vs), ptr(kt), ptr(vt)), dtype_code(kt.dtype)
+
+
+def _kv8_rows(t: torch.Tensor, what: str, batch: int, q_len: int, d: int, dtype):
+    if t.dim() != 4 or t.shape[0] != batch or t.shape[1] != q_len or t.shape[3] != d or t.dtype != dtype:
+        raise _lib.BtError(f"{what} must be {dtype} [{batch}, {q_len}, heads, {d}], got {t.dtype} {tuple(t.shape)}")
+    if t.stride(3) != 1:
+        raise _lib.BtError(f"{what} must have unit inner stride")
+    return _lib.bt_kv8_rows(ptr(t), *(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))     # the stride of one row says nothing
+
+
+def _pos0(pos0):
+    if isinstance(pos0, torch.Tensor):
+        if pos0.dtype != torch.int32 or pos0.numel() != 1:
+            raise _lib.BtError("a device-side pos0 is one int32")
+        return ptr(pos0), 0
+    return None, int(pos0)
+
+
+def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.Tensor, v: torch.Tensor, pos0,
+               rope: Optional[torch.Tensor] = None, pos_table: Optional[torch.Tensor] = None, q_out: Optional[torch.Tensor] = None):
+    """Append rows ``k``, ``v`` [B, q_len, kv_heads, d] (any outer strides: views of a fused projection) at row ``pos0`` (an int, or one
+    int32 on the device) of one layer of an 8-bit cache (``runtime.KV8Cache``), rotating ``k`` and ``q`` [B, q_len, heads, d] by ``rope``
+    (``rope_tables``) at positions pos0 + t or ``pos_table[pos0 + t]``.  Returns the rotated q -- in ``q_out`` (which may be q), new
+    memory otherwise; q itself without ``rope``.  Blocks that fill up are quantised in the same call."""
+    cache, code = _kv8(kv)
+    dtype = kv[4].dtype
+    B, q_len, H, d = cache.batch, k.shape[1] if k.dim() == 4 else 0, cache.kv_heads, cache.head_dim
+    kr, vr = (_kv8_rows(t, name, B, q_len, d, dtype) for t, name in ((k, "k"), (v, "v")))
+    if k.shape[2] != H or v.shape[2] != H:
+        raise _lib.BtError(f"k and v must have the cache's {H} heads")
+    if q_len == 0:
+        raise _lib.BtError("no rows to append")
+    qr = qor = None
+    heads = rot = max_pos = 0
+    cos = sin = None
+    if q is not None:
+        qr, heads = _kv8_rows(q, "q", B, q_len, d, dtype), q.shape[2]
+    pos_dev, pos_host = _pos0(pos0)
+    with _on(k.device, *kv, q, v, rope, pos_table, q_out, pos0 if pos_dev else None):
+        if rope is not None:
+            if rope.dim() != 3 or rope.shape[0] != 2 or rope.dtype != torch.float32 or not rope.is_contiguous():
+                raise _lib.BtError("rope must be contiguous float32 [2, max_pos, rot / 2] (rope_tables)")
+            max_pos, rot = rope.shape[1], 2 * rope.shape[2]
+            cos, sin = ptr(rope), ptr(rope) + rope.stride(0) * 4
+            if q is not None:
+                if q_out is None:
+                    q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+                elif q_out.shape != q.shape:
+                    raise _lib.BtError("q_out must have q's shape")
+                qor = _kv8_rows(q_out, "q_out", B, q_len, d, dtype)
+        elif q_out is not None:
+            raise _lib.BtError("q_out without rope: there is nothing to rotate q by")
+        if pos_table is not None and (pos_table.dtype != torch.int32 or pos_table.dim() != 1 or not pos_table.is_contiguous() or
+                                      pos_table.numel() < (cache.n_max if pos_dev else pos_host + q_len)):
+            raise _lib.BtError("pos_table must be contiguous int32 and hold an entry for every row")
+        check(lib().bt_kv8_append(code, ctypes.byref(cache), q_len, heads if rot else 0, qr if rot else None, qor, kr, vr, pos_dev, pos_host,
+                                  ptr(pos_table), rot, cos, sin, max_pos, current_stream()), "bt_kv8_append")
+    return q_out if rot else q
+
+
+def kv8_read(kv: Sequence[torch.Tensor], n: int, first: int = 0, count: Optional[int] = None):
+    """(k, v) [B, kv_heads, count, d]: rows [first, first + count) (default: to the end) of a layer of an 8-bit cache that holds ``n``
+    rows, in the cache's dtype."""
+    cache, code = _kv8(kv)
+    count = n - first if count is None else count
+    if not 0 <= first <= first + count <= n <= cache.n_max:
+        raise _lib.BtError(f"rows [{first}, {first + count}) of {n} in a cache of {cache.n_max}")
+    with _on(kv[0].device, *kv):
+        k = torch.empty(cache.batch, cache.kv_heads, count, cache.head_dim, dtype=kv[4].dtype, device=kv[0].device)
+        v = torch.empty_like(k)
+        check(lib().bt_kv8_read(code, ctypes.byref(cache), n, first, count, ptr(k), ptr(v), current_stream()), "bt_kv8_read")
+    return k, v
+
+
+def attention_kv8(q: torch.Tensor, kv: Sequence[torch.Tensor], pos0, mask: Optional[torch.Tensor] = None,
+                  out: Optional[torch.Tensor] = None, n_split: int = 0, ws: Optional[torch.Tensor] = None):
+    """softmax(q k^T / sqrt(d)) v over a layer of an 8-bit cache: row t of ``q`` [B, q_len, heads, d] (rotated, any outer strides; heads a
+    multiple of the cache's) sees the rows j <= pos0 + t with mask[b, j] != 0 (uint8 or bool [B, >= n]); zeros where none is left.  The
+    rows pos0 .. pos0 + q_len - 1 are in the cache already.  ``n_split``: workgroups that share a head's rows (0: chosen from the sizes;
+    with a device-side pos0 from the cache's size); ``ws``: >= bt_attention_kv8_workspace_bytes, allocated when needed and not given."""
+    cache, code = _kv8(kv)
+    B, q_len, H, d, dtype = cache.batch, q.shape[1] if q.dim() == 4 else 0, cache.kv_heads, cache.head_dim, kv[4].dtype
+    qr = _kv8_rows(q, "q", B, q_len, d, dtype)
+    heads = q.shape[2]
+    if q_len == 0 or heads == 0 or heads % H:
+        raise _lib.BtError(f"{heads} query heads cannot share {H} key/value heads ({q_len} rows)")
+    pos_dev, pos_host = _pos0(pos0)
+    mask_ld = 0
+    if mask is not None:
+        if mask.dim() != 2 or mask.shape[0] != B or mask.dtype not in (torch.uint8, torch.bool) or mask.stride(1) != 1:
+            raise _lib.BtError(f"mask must be uint8 or bool [{B}, rows] with unit inner stride")
+        mask_ld = mask.stride(0) if B > 1 else mask.shape[1]
+        if mask.shape[1] < (cache.n_max if pos_dev else pos_host + q_len):
+            raise _lib.BtError("mask row too short")
+    with _on(q.device, *kv, mask, out, ws, pos0 if pos_dev else None):
+        if out is None:
+            out = torch.empty(B, q_len, heads, d, dtype=dtype, device=q.device)
+        elif out.shape != (B, q_len, heads, d) or out.dtype != dtype or not out.is_contiguous():
+            raise _lib.BtError(f"out must be contiguous {dtype} [{B}, {q_len}, {heads}, {d}]")
+        if n_split <= 0:
+            n_split = lib().bt_attention_kv8_split_count(B, H, heads // H, q_len, cache.n_max if pos_dev else pos_host + q_len)
+        if ws is None and n_split > 1:
+            need = int(lib().bt_attention_kv8_workspace_bytes(B, q_len, heads, d, n_split))
+            ws = torch.empty(need, dtype=torch.uint8, device=q.device)
+        check(lib().bt_attention_kv8(code, ctypes.byref(cache), q_len, heads, qr, pos_dev, pos_host, ptr(mask), mask_ld, ptr(out),
+                                     heads * d, n_split, ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(), current_stream()),
+              "bt_attention_kv8")
+    return out

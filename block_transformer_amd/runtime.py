@@ -66,6 +66,40 @@ class KVCache:
         return self.k.shape[0]
 
 
+class KV8Cache:
+    """A KV cache in 8 bits: codes with one scale per (layer, sequence, head, block of ``block`` rows), the open block's rows in ``dtype``
+    (layout: bt_kv8_cache in include/bt_hip.h).  About half the memory of a bf16 ``KVCache``; ``cache[layer]`` is what ``ops.kv8_append``,
+    ``ops.kv8_read`` and ``ops.attention_kv8`` take."""
+
+    def __init__(self, layers: int, batch: int, kv_heads: int, n_max: int, head_dim: int, dtype, device, block: int = 16):
+        if block not in (16, 32, 64):
+            raise _lib.BtError(f"block {block} is not 16, 32 or 64")
+        dtype_code(dtype)
+        blocks = max(1, -(-n_max // block))
+        lead = (layers, batch, kv_heads)
+        self.k_codes = torch.empty(lead + (blocks * block, head_dim), dtype=torch.int8, device=device)
+        self.v_codes = torch.empty(lead + (blocks, head_dim, block), dtype=torch.int8, device=device)
+        self.k_scale = torch.empty(lead + (blocks,), dtype=torch.float32, device=device)
+        self.v_scale = torch.empty_like(self.k_scale)
+        self.k_tail = torch.empty(lead + (block, head_dim), dtype=dtype, device=device)
+        self.v_tail = torch.empty(lead + (head_dim, block), dtype=dtype, device=device)
+
+    @property
+    def n_max(self) -> int:
+        """Rows per head: what was asked for, rounded up to whole blocks."""
+        return self.k_codes.shape[3]
+
+    @property
+    def block(self) -> int:
+        return self.k_tail.shape[3]
+
+    def __getitem__(self, layer: int):
+        return tuple(t[layer] for t in (self.k_codes, self.v_codes, self.k_scale, self.v_scale, self.k_tail, self.v_tail))
+
+    def __len__(self):
+        return self.k_codes.shape[0]
+
+
 class Workspace:
     """A grow-only scratch tensor per device (activation workspace of bt_decoder_forward)."""
 

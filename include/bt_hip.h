@@ -239,6 +239,83 @@ int bt_topk_sample(int dtype, int64_t M, int64_t V, const void* logits, int64_t 
                    bt_stream stream);   /* row0: RNG row index of logits row 0 (request shards of one batch draw the same
                                            streams as the whole batch would: key = (seed, *step_dev, row0 + r)) */
 
+/* ---- 8-bit serving: linear layers in 8-bit integers, a KV cache held in 8 bits and the attention that reads it ----------------
+ * Quantisation, everywhere: s = fl32(amax / 127), code = clamp(round_half_even(x / s), -127, 127), the quotient rounded as if taken
+ * exactly; s = 0 gives codes 0. */
+
+/* codes[m, :] = x[m, :] quantised with ONE scale per row, scales[m] = s; with ln_w / ln_b the row is LayerNorm(x[m, :]; ln_w, ln_b, eps),
+ * held in fp32 and not rounded to `dtype` in between.  Columns K .. round_up(K, 16) - 1 are written as 0, so a row of codes is a whole
+ * number of 16-byte units: pass round_up(K, 16) as K to bt_linear_q8.  ldc >= round_up(K, 16), ldc % 16 == 0, codes 16-byte aligned; x
+ * may have any row stride.  A row that holds an infinity or NaN gets codes 0 and scale NaN: whatever is computed from it is NaN, as it
+ * would be from the row itself.  Also lays out weights: W[N, K] gives one scale per output channel. */
+int bt_quant_rows(int dtype, int64_t M, int64_t K, const void* x, int64_t ldx, const void* ln_w, const void* ln_b, float eps,
+                  int8_t* codes, int64_t ldc, float* scales, bt_stream stream);
+
+/* out[m, n] = act(sum_k A[m, k] W[n, k] * a_scale[m] * w_scale[n] + bias[n]) + residual[m, n]: bt_linear in 8-bit integers.  The sum is
+ * an exact int32; the rest is fp32, rounded once to `dtype` (of bias, residual and out).  K % 16 == 0, K <= 131056 (the sum cannot
+ * leave int32), lda / ldw % 16 == 0, A / W 16-byte aligned; out, bias and residual may have any alignment and row stride.
+ * `scratch` (16-byte aligned, >= bt_linear_q8_scratch_bytes(M, N, K), which may be 0) lets short problems split K over workgroups;
+ * without it they run unsplit, with the same bits (integer sums do not depend on their order). */
+int64_t bt_linear_q8_scratch_bytes(int64_t M, int64_t N, int64_t K);
+int bt_linear_q8(int dtype, int64_t M, int64_t N, int64_t K, const int8_t* A, int64_t lda, const float* a_scale, const int8_t* W,
+                 int64_t ldw, const float* w_scale, const void* bias, const void* residual, int64_t ldr, void* out, int64_t ldo,
+                 int act, void* scratch, int64_t scratch_bytes, bt_stream stream);
+
+/* One layer of a KV cache in 8 bits: one scale for each block of `block` consecutive rows of a (sequence, head), K and V apart.
+ *   k_codes  [batch][kv_heads][n_max][head_dim]              v_codes  [batch][kv_heads][n_max / block][head_dim][block]
+ *   k_scale, v_scale  [batch][kv_heads][n_max / block]       k_tail   [batch][kv_heads][block][head_dim]   (dtype)
+ *                                                            v_tail   [batch][kv_heads][head_dim][block]   (dtype)
+ * A block is quantised when its last row arrives; until then its rows stand in the tail as they came, in `dtype`.  So what the cache
+ * holds depends on the rows alone, not on how many came at a time, and no row is rounded twice.  V is kept token-innermost because the
+ * product with the probabilities runs over tokens: a matrix instruction's operand is then one 16-byte load.
+ * An infinity or NaN does not count for its block's scale; it is stored as +-127 or 0 (one row, masked or not, must not spoil the rows
+ * it shares a scale with).  In the tail, and so in attention over the open block, it stands as it came. */
+typedef struct bt_kv8_cache {
+    uint32_t struct_size;    /* = sizeof(bt_kv8_cache) */
+    int32_t block;           /* 16, 32 or 64 */
+    int32_t kv_heads;
+    int32_t head_dim;        /* 32, 64 or 128 */
+    int64_t batch;
+    int64_t n_max;           /* rows per head; a multiple of block */
+    int8_t* k_codes; int8_t* v_codes;
+    float* k_scale; float* v_scale;
+    void* k_tail; void* v_tail;
+} bt_kv8_cache;
+
+/* Rows [batch][q_len][heads][head_dim] anywhere in memory: element strides of the three outer axes, unit stride inside a head.  Base and
+ * strides are 16-byte granular. */
+typedef struct bt_kv8_rows {
+    void* p;
+    int64_t b_stride, t_stride, h_stride;
+} bt_kv8_rows;
+
+/* Append q_len rows of k and v at rows pos0 .. pos0 + q_len - 1 (rows [0, pos0) are there already) and rotate q:
+ *   pos0 = pos0_dev ? *pos0_dev : pos0_host, angle position = pos_table ? pos_table[pos0 + t] : pos0 + t (clamped to the tables' max_pos
+ *   rows), partial RoPE over the first `rot` dims of q and k as in bt_rope_kv_append, computed in 64 bits and rounded once.
+ * q -> q_out (heads query heads; may be the same memory; both NULL: only k and v).  rot == 0: no rotation, q must be NULL.  Rows at
+ * n_max and beyond, which only a device-side pos0 can reach, are dropped. */
+int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len, int32_t heads, const bt_kv8_rows* q, const bt_kv8_rows* q_out,
+                  const bt_kv8_rows* k, const bt_kv8_rows* v, const int32_t* pos0_dev, int32_t pos0_host, const int32_t* pos_table,
+                  int32_t rot, const float* cos_tab, const float* sin_tab, int64_t max_pos, bt_stream stream);
+
+/* k_out, v_out [batch][kv_heads][count][head_dim] = rows [first, first + count) of a cache that holds n rows, as `dtype` (either may be
+ * NULL).  first + count <= n <= n_max. */
+int bt_kv8_read(int dtype, const bt_kv8_cache* cache, int64_t n, int64_t first, int64_t count, void* k_out, void* v_out,
+                bt_stream stream);
+
+/* Causal softmax attention over the cache: query row t of head h sees rows j <= pos0 + t (j < n_max) of head h / (heads / kv_heads) with
+ * mask[b, j] != 0 (mask may be NULL);  out[(b * q_len + t) * ldo + h * head_dim + :], zeros where nothing is left to see.  The rows
+ * pos0 .. pos0 + q_len - 1 have been appended.  Scores and probabilities go through the matrix units as integer digits -- two 8-bit
+ * digits for bf16, three for fp32 -- against the codes themselves; sums are exact int32 per 64 rows and fp32 across them.
+ * n_split > 1 splits the rows over that many workgroups (bt_attention_kv8_split_count gives a good number for a batch; it depends on
+ * its arguments alone) and needs a workspace of bt_attention_kv8_workspace_bytes(...).  mask_ld >= pos0_host + q_len, or >= n_max with
+ * a device-side pos0. */
+int32_t bt_attention_kv8_split_count(int64_t batch, int32_t kv_heads, int32_t group, int32_t q_len, int64_t n);
+int64_t bt_attention_kv8_workspace_bytes(int64_t batch, int32_t q_len, int32_t heads, int32_t head_dim, int32_t n_split);
+int bt_attention_kv8(int dtype, const bt_kv8_cache* cache, int32_t q_len, int32_t heads, const bt_kv8_rows* q, const int32_t* pos0_dev,
+                     int32_t pos0_host, const uint8_t* mask, int64_t mask_ld, void* out, int64_t ldo, int32_t n_split, void* ws,
+                     int64_t ws_bytes, bt_stream stream);
+
 /* ---- composite: one GPT-NeoX stack over M = B*q_len rows (what GPTNeoXModel.forward does for inputs_embeds) ---- */
 typedef struct bt_attn_args {
     uint32_t struct_size;    /* = sizeof(bt_attn_args) of the header the caller was compiled against; every entry point rejects
