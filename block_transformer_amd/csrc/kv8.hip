@@ -144,80 +144,493 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(bt_kv8_cache c, int shift
 }
 
 // ---- bt_attention_kv8 ------------------------------------------------------------------------------------------------------
+// The cache's codes are multiplied as they are, by v_mfma_i32_16x16x64_i8: q is written as 8-bit digits, q = (amax / Q) sum_i 256^(ND-1-i)
+// dig_i with Q = 127 * 256^(ND-1) -- two digits for bf16 (an error of 2^-16 of the row's largest, bf16 itself has 2^-9), three for fp32 --
+// and so are the probabilities (three digits).  No code is converted, so a byte of the cache costs one load and 1/64 of a matrix
+// instruction per 16 query rows, and the kernel is bound by reading the cache.
+//
+// A wave works on 16 query rows (rows x heads that share a KV head) and 64 cached rows at a time:
+//   S^T = K Q^T   A = K: lane (m = lane & 15, g = lane >> 4) holds 16 bytes of row tok(i, m) = 16 (m >> 2) + 4 i + (m & 3), i = 0 .. 3.
+//                 In the result lane (query c = lane & 15, g) holds rows 16 g + 4 i + r, r = 0 .. 3: 16 consecutive rows, one block's
+//                 scale, one 16-byte piece of the mask.
+//   O^T = V^T P^T B = P: the lane's own 16 rows are exactly the k-range 16 g .. 16 g + 15 it has to supply: nothing moves between lanes.
+//                 A = V^T: lane m holds 16 consecutive rows of dim 16 j + m, one 16-byte load from v_codes.
+// Softmax: every 64-row tile has its own largest score as the base of its digits (a far larger score elsewhere costs them nothing), and
+// enters a running (max, sum, output) in fp32.  The rows' V scales go into the probabilities, relative to the tile's largest.
+// The open block is one more tile: bf16 or fp32 matrix instructions on its rows as they stand, probabilities as two bf16 (16 bits) or
+// one fp32.
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+
 struct AttnArgs {
     bt_kv8_cache c;
     Rows q;
-    int q_len, heads, pos0_host, shift;
+    int q_len, heads, share, rows, row_groups, n_split, pos0_host, shift;
     const int32_t* pos0_dev;
     const uint8_t* mask;
     int64_t mask_ld;
     void* out;
     int64_t ldo;
+    float* part;      // [batch][kv_heads][rows][n_split][head_dim + 2]: output, max, sum; nullptr: one split
     float scale;      // log2(e) / sqrt(head_dim)
 };
 
-// One wave per (sequence, row, head): a lane scores one cached row of 64, then owns head_dim / 64 columns of the output.
-template <typename T>
-__global__ __launch_bounds__(64) void attention_kv8_kernel(AttnArgs a) {
-    __shared__ float qs[128], ps[64];
-    const int D = a.c.head_dim, bl = a.c.block, lane = threadIdx.x;
-    const int64_t i = blockIdx.x;
-    const int h = (int)(i % a.heads);
-    const int64_t row = i / a.heads;
-    const int64_t b = row / a.q_len;
-    const int t = (int)(row - b * a.q_len);
-    const int pos0 = a.pos0_dev ? *a.pos0_dev : a.pos0_host;
-    const int64_t n = pos0 + (int64_t)a.q_len < a.c.n_max ? pos0 + (int64_t)a.q_len : a.c.n_max;
-    const int64_t lim = pos0 + t + 1 < n ? pos0 + t + 1 : n;
-    const int64_t bh = b * a.c.kv_heads + h / (a.heads / a.c.kv_heads);
-    const int64_t n_blk = a.c.n_max >> a.shift, full = n >> a.shift;
-    const T* q = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
-    for (int d = lane; d < D; d += 64) qs[d] = Elem<T>::load(q + d);
-    float m = -1e30f, l = 0.f, o[2] = {0.f, 0.f};
-    for (int64_t j0 = 0; j0 < lim; j0 += 64) {
-        const int64_t j = j0 + lane;
-        const bool on = j < lim && !(a.mask && a.mask[b * a.mask_ld + j] == 0);
-        float s = -INFINITY;
-        __syncthreads();
-        if (on) {
-            const int64_t blk = j >> a.shift;
-            s = 0.f;
-            if (blk < full) {
-                const int8_t* k = a.c.k_codes + (bh * a.c.n_max + j) * D;
-                for (int d = 0; d < D; ++d) s = fmaf(qs[d], (float)k[d], s);
-                s *= a.c.k_scale[bh * n_blk + blk];
-            } else {
-                const T* k = (const T*)a.c.k_tail + (bh * bl + (j & (bl - 1))) * D;
-                for (int d = 0; d < D; ++d) s = fmaf(qs[d], Elem<T>::load(k + d), s);
+constexpr float M_FLOOR = -1e30f;      // "no score yet": finite, so that differences of two of them are 0
+
+// the largest over the four lanes c, c + 16, c + 32, c + 48, in all of them
+__device__ inline float max_over_groups(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float sum_over_groups(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+template <typename T, int D>
+struct Attend {
+    static constexpr int ND = sizeof(T) == 2 ? 2 : 3;       // digits of q
+    static constexpr int NC = (D + 63) / 64;                // 64-dim pieces of a row of K
+    static constexpr int NJ = D / 16;                       // 16-dim pieces of the output
+    static constexpr int PD = 127 * 65536;                  // full scale of a probability's three digits
+
+    const AttnArgs& a;
+    const int lane, c, g;
+    int64_t bh, n_full, full, n_blk;
+    const int8_t *kc, *vc;
+    const float *ks, *vs;
+    const uint8_t* mask;
+    const T* q;
+    int64_t lim;              // rows that this lane's query sees
+    float qs = 0.f;           // what one unit of its integer scores stands for, times a.scale
+    i32x4 dig[ND][NC];
+    float m = M_FLOOR, l = 0.f;
+    f32x4 o[NJ];
+
+    __device__ Attend(const AttnArgs& a_) : a(a_), lane(threadIdx.x & 63), c(lane & 15), g(lane >> 4) {}
+
+    __device__ inline void load_query(bool real) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        float x[NC][16];
+        float amax = 0.f, bad = 0.f;
+        const bool mine = real && (D >= 64 || g < 2);
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+#pragma unroll
+            for (int e = 0; e < 16; e += Elem<T>::VEC) {
+                float v[Elem<T>::VEC] = {};
+                if (mine) load_vec<T>(q + 64 * k + 16 * g + e, v);
+#pragma unroll
+                for (int i = 0; i < Elem<T>::VEC; ++i) {
+                    x[k][e + i] = v[i];
+                    amax = fmaxf(amax, fabsf(v[i]));
+                    bad = fabsf(v[i]) < INFINITY ? bad : 1.f;
+                }
             }
-            s *= a.scale;
         }
-        const bool nan = __any(s != s);
-        const float mn = fmaxf(m, wave_max(s));
-        const float p = nan ? __int_as_float(0x7fc00000) : __builtin_amdgcn_exp2f(s - mn), al = __builtin_amdgcn_exp2f(m - mn);
-        m = mn;
-        l = l * al + p;
-        ps[lane] = p;
-        __syncthreads();
-        for (int i2 = 0; i2 < 2; ++i2) {
-            const int d = lane + 64 * i2;
-            if (d >= D) break;
-            float acc = o[i2] * al;
-            for (int jj = 0; jj < 64 && j0 + jj < lim; ++jj) {
-                const float pj = ps[jj];
-                if (pj == 0.f) continue;
-                const int64_t blk = (j0 + jj) >> a.shift;
-                const int tt = (int)((j0 + jj) & (bl - 1));
-                const float v = blk < full ? (float)a.c.v_codes[((bh * n_blk + blk) * D + d) * bl + tt] * a.c.v_scale[bh * n_blk + blk]
-                                           : Elem<T>::load((const T*)a.c.v_tail + (bh * D + d) * bl + tt);
-                acc = fmaf(pj, v, acc);
+        amax = max_over_groups(amax);
+        bad = max_over_groups(bad);
+        const float up = amax < 1e-30f ? 0x1p64f : 1.0f;     // keeps Q / amax finite
+        constexpr float Q = ND == 2 ? 127.f * 256.f : 127.f * 65536.f;
+        const float inv = amax > 0.f ? Q / (amax * up) : 0.f;
+        qs = bad != 0.f ? __int_as_float(0x7fc00000) : amax / Q * a.scale;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                uint32_t out[ND] = {};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    int v = bad != 0.f ? 0 : (int)rintf(x[k][4 * w + e] * up * inv);
+#pragma unroll
+                    for (int i = ND - 1; i >= 0; --i) {
+                        const int low = i ? (int)(int8_t)(v & 255) : v;
+                        out[i] |= (uint32_t)(low & 255) << (8 * e);
+                        v = (v - low) >> 8;
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < ND; ++i) dig[i][k][w] = (int)out[i];
             }
-            o[i2] = acc;
         }
     }
-    l = wave_sum(l);
-    for (int i2 = 0; i2 < 2; ++i2)
-        if (lane + 64 * i2 < D) Elem<T>::store((T*)a.out + row * a.ldo + h * D + lane + 64 * i2, l == 0.f ? 0.f : o[i2] / l);
+
+    __device__ inline void load_k(int64_t tile, i32x4 (&k)[4][NC]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int64_t tok = tile * 64 + 16 * (c >> 2) + 4 * i + (c & 3);
+            tok = tok < a.c.n_max ? tok : a.c.n_max - 1;
+            const int8_t* p = kc + tok * D + 16 * (D >= 64 ? g : g & 1);      // D = 32: the upper lanes' digits are zero
+#pragma unroll
+            for (int n = 0; n < NC; ++n) k[i][n] = *(const i32x4*)(p + 64 * n);
+        }
+    }
+    __device__ inline void load_v(int64_t tile, i32x4 (&v)[NJ]) const {
+        const int64_t tok = tile * 64 + 16 * g;
+        int64_t blk = tok >> a.shift;
+        blk = blk < n_blk ? blk : n_blk - 1;
+        const int8_t* p = vc + (blk * D + c) * a.c.block + (tok & (a.c.block - 1));
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) v[j] = *(const i32x4*)(p + (int64_t)16 * j * a.c.block);
+    }
+    // bit e: this lane's query sees row 16 g + e of the tile (all 16 rows begin at tok0)
+    __device__ inline uint32_t visible(int64_t tok0, int count, int64_t end) const {
+        const int64_t left = (end < lim ? end : lim) - tok0;
+        const int most = left < count ? (left < 0 ? 0 : (int)left) : count;
+        uint32_t on = (1u << most) - 1u;
+        if (mask)
+            for (int e = 0; e < count; ++e)
+                if (tok0 + e < end && mask[tok0 + e] == 0) on &= ~(1u << e);
+        return on;
+    }
+
+    // enters a tile with its largest score mt: the factor for what is there already; `gamma` for what comes
+    __device__ inline float enter(float mt, float& gamma) {
+        const float mn = fmaxf(m, mt), alpha = __builtin_amdgcn_exp2f(m - mn);
+        gamma = __builtin_amdgcn_exp2f(mt - mn);
+        m = mn;
+        return alpha;
+    }
+
+    __device__ inline void tile(int64_t at, const i32x4 (&k)[4][NC], const i32x4 (&v)[NJ], bool cut) {
+        const int64_t tok0 = at * 64 + 16 * g, blk = tok0 >> a.shift;
+        const float sk = blk < full ? ks[blk] : 0.f, sv = blk < full ? vs[blk] : 0.f;
+        const float mul = qs * sk;
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            i32x4 acc{0, 0, 0, 0}, low{0, 0, 0, 0};
+#pragma unroll
+            for (int n = 0; n < NC; ++n) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i][n], dig[0][n], acc, 0, 0, 0);
+            acc <<= 8;
+#pragma unroll
+            for (int n = 0; n < NC; ++n) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i][n], dig[1][n], acc, 0, 0, 0);
+            if (ND == 3) {
+#pragma unroll
+                for (int n = 0; n < NC; ++n) low = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i][n], dig[ND - 1][n], low, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[i][r] = (ND == 3 ? fmaf((float)acc[r], 256.f, (float)low[r]) : (float)acc[r]) * mul;
+        }
+        if (cut) {
+            const uint32_t on = visible(tok0, 16, n_full);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[i][r] = (on >> (4 * i + r)) & 1 ? s[i][r] : -INFINITY;
+        }
+        float mt = M_FLOOR;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[i][r]);
+        mt = max_over_groups(mt);
+        const float top = max_over_groups(sv);
+        const float rel = top > 0.f ? sv / top : 0.f;
+        float gamma, sum = 0.f;
+        const float alpha = enter(mt, gamma);
+        i32x4 p[3];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t f[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(s[i][r] - mt);
+                sum += e;
+                // the three digits as the bytes of a float's mantissa: 2^23 + N, N = P + 0x8080, P = round(p PD)
+                f[r] = __float_as_uint(fmaf(e * rel, (float)PD, 8388608.f + 32896.f));
+            }
+            const uint32_t a01 = __builtin_amdgcn_perm(f[1], f[0], 0x05010400), a23 = __builtin_amdgcn_perm(f[3], f[2], 0x05010400);
+            const uint32_t b01 = __builtin_amdgcn_perm(f[1], f[0], 0x06020602), b23 = __builtin_amdgcn_perm(f[3], f[2], 0x06020602);
+            p[0][i] = (int)__builtin_amdgcn_perm(b23, b01, 0x05040100);
+            p[1][i] = (int)(__builtin_amdgcn_perm(a23, a01, 0x07060302) ^ 0x80808080u);
+            p[2][i] = (int)(__builtin_amdgcn_perm(a23, a01, 0x05040100) ^ 0x80808080u);
+        }
+        l = fmaf(l, alpha, sum * gamma);
+        const float beta = top * gamma * (1.0f / (float)PD), beta256 = beta * 256.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            i32x4 acc{0, 0, 0, 0}, low{0, 0, 0, 0};
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[j], p[0], acc, 0, 0, 0);
+            low = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[j], p[2], low, 0, 0, 0);
+            acc <<= 8;
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[j], p[1], acc, 0, 0, 0);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[j][r] = fmaf((float)acc[r], beta256, fmaf((float)low[r], beta, o[j][r] * alpha));
+        }
+    }
+
+    // The open block: rows n_full .. end - 1, row 4 nI g + 4 i + r of it with lane g's (i, r), nI = block / 16.
+    __device__ void tail(int64_t end) {
+        const int bl = a.c.block, nI = bl >> 4, per = bl >> 2;
+        const T* kt = (const T*)a.c.k_tail + bh * bl * D;
+        const T* vt = (const T*)a.c.v_tail + bh * bl * D;
+        float s[4][4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i >= nI) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[i][r] = -INFINITY;
+                continue;
+            }
+            const T* kr = kt + (per * (c >> 2) + 4 * i + (c & 3)) * D;
+            f32x4 acc{0.f, 0.f, 0.f, 0.f};
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int n = 0; n < D / 32; ++n) {
+                    const bf16x8 kf = *(const bf16x8*)(kr + 32 * n + 8 * g), qf = *(const bf16x8*)(q + 32 * n + 8 * g);
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf, acc, 0, 0, 0);
+                }
+            } else {
+#pragma unroll
+                for (int n = 0; n < D / 4; n += 4) {
+                    const f32x4 kf = *(const f32x4*)(kr + D / 4 * g + n), qf = *(const f32x4*)(q + D / 4 * g + n);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], acc, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[i][r] = acc[r] * a.scale;
+        }
+        const int64_t tok0 = n_full + per * g;
+        const uint32_t on = visible(tok0, per, end);
+        uint32_t some = 0;      // rows that any query may see
+        for (int e = 0; e < per; ++e)
+            if (tok0 + e < end && !(mask && mask[tok0 + e] == 0)) some |= 1u << e;
+        float mt = M_FLOOR;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[i][r] = (on >> (4 * i + r)) & 1 ? s[i][r] : -INFINITY;
+                mt = fmaxf(mt, s[i][r]);
+            }
+        mt = max_over_groups(mt);
+        float gamma, sum = 0.f;
+        const float alpha = enter(mt, gamma);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                s[i][r] = __builtin_amdgcn_exp2f(s[i][r] - mt) * gamma;
+                sum += s[i][r];
+            }
+        l = fmaf(l, alpha, sum);
+        bool odd = false;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            o[j] *= alpha;
+            const T* vr = vt + (16 * j + c) * bl + per * g;
+            float v[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                v[e] = e < per ? Elem<T>::load(vr + e) : 0.f;
+                v[e] = (some >> e) & 1 ? v[e] : 0.f;
+                odd |= !(fabsf(v[e]) < INFINITY);
+                v[e] = fabsf(v[e]) < INFINITY ? v[e] : 0.f;
+            }
+#pragma unroll
+            for (int h = 0; h < 16; h += 8) {
+                if (h >= per) continue;
+                if constexpr (sizeof(T) == 2) {
+                    union { uint32_t u[4]; bf16x8 f; } vf, hi, lo;
+#pragma unroll
+                    for (int e = 0; e < 8; e += 2) {
+                        const float p0 = s[(h + e) >> 2][(h + e) & 3], p1 = s[(h + e + 1) >> 2][(h + e + 1) & 3];
+                        vf.u[e >> 1] = pack_bf16x2(v[h + e], v[h + e + 1]);
+                        hi.u[e >> 1] = pack_bf16x2(p0, p1);
+                        lo.u[e >> 1] = pack_bf16x2(p0 - __uint_as_float(hi.u[e >> 1] << 16), p1 - __uint_as_float(hi.u[e >> 1] & 0xffff0000u));
+                    }
+                    o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.f, hi.f, o[j], 0, 0, 0);
+                    o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.f, lo.f, o[j], 0, 0, 0);
+                } else {
+#pragma unroll
+                    for (int e = h; e < h + 8; ++e) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], s[e >> 2][e & 3], o[j], 0, 0, 0);
+                }
+            }
+        }
+        // an infinity or NaN in a row that some queries see and others may not: a matrix product would give it to all of them
+        if (__any(odd)) {
+#pragma unroll 1
+            for (int x = 0; x < bl; ++x) {
+                const int gg = x / per, e = x - gg * per;
+                float p = 0.f;
+#pragma unroll
+                for (int i = 0; i < 16; ++i) p = i == e ? s[i >> 2][i & 3] : p;
+                p = __shfl(p, gg * 16 + c, 64);
+                const bool seen = (__shfl((int)on, gg * 16 + c, 64) >> e) & 1;
+#pragma unroll
+                for (int j = 0; j < NJ; ++j)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float y = Elem<T>::load(vt + (16 * j + 4 * g + r) * bl + x);
+                        if (seen && !(fabsf(y) < INFINITY)) o[j][r] = fmaf(p, y, o[j][r]);
+                    }
+            }
+        }
+    }
+};
+
+template <typename T, int D, int NW>
+__global__ __launch_bounds__(NW * 64, NW == 1 ? 2 : 2) void attention_kv8_kernel(AttnArgs a) {
+    using A = Attend<T, D>;
+    __shared__ float merged[NW > 1 ? NW : 1][NW > 1 ? 16 : 1][D + 4];
+    const int wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
+    A w(a);
+    int64_t id = blockIdx.x;
+    const int split = (int)(id % a.n_split);
+    id /= a.n_split;
+    const int rg = (int)(id % a.row_groups);
+    w.bh = id / a.row_groups;
+    const int64_t b = w.bh / a.c.kv_heads;
+    const int h0 = (int)(w.bh - b * a.c.kv_heads) * a.share;
+    const int pos0 = a.pos0_dev ? *a.pos0_dev : a.pos0_host;
+    const int row = rg * 16 + w.c;
+    const bool real = row < a.rows;
+    const int t = real ? row / a.share : 0, h = h0 + (real ? row - t * a.share : 0);
+    int64_t n = pos0 + (int64_t)a.q_len;
+    n = n < 0 ? 0 : n < a.c.n_max ? n : a.c.n_max;
+    const int last_row = rg * 16 + 15 < a.rows ? rg * 16 + 15 : a.rows - 1;
+    int64_t end = pos0 + (int64_t)last_row / a.share + 1;      // no row of this group sees further
+    end = end < 0 ? 0 : end < n ? end : n;
+    int64_t least = pos0 + (int64_t)(rg * 16) / a.share + 1;   // every row of it sees as far as this
+    w.full = n >> a.shift;
+    w.n_full = w.full << a.shift;
+    w.n_blk = a.c.n_max >> a.shift;
+    w.lim = pos0 + (int64_t)t + 1 < n ? pos0 + (int64_t)t + 1 : n;
+    w.kc = a.c.k_codes + w.bh * a.c.n_max * D;
+    w.vc = a.c.v_codes + w.bh * a.c.n_max * D;
+    w.ks = a.c.k_scale + w.bh * w.n_blk;
+    w.vs = a.c.v_scale + w.bh * w.n_blk;
+    w.mask = a.mask ? a.mask + b * a.mask_ld : nullptr;
+    w.q = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
+    w.load_query(real);
+
+    const int64_t closed = w.n_full < end ? w.n_full : end;      // rows of full blocks that somebody sees
+    const int64_t tiles = (closed + 63) >> 6, all = tiles + (end > w.n_full ? 1 : 0);
+    const int64_t per = (all + a.n_split - 1) / a.n_split;
+    int64_t at = split * per + wave;
+    const int64_t stop = (split + 1) * per < all ? (split + 1) * per : all;
+    i32x4 k[4][A::NC], v[A::NJ];
+    if (at < stop && at < tiles) w.load_k(at, k);
+    for (; at < stop && at < tiles; at += NW) {
+        i32x4 next[4][A::NC];
+        w.load_v(at, v);
+        const bool more = at + NW < stop && at + NW < tiles;
+        if (more) w.load_k(at + NW, next);
+        w.tile(at, k, v, w.mask || at * 64 + 64 > w.n_full || at * 64 + 64 > least);
+        if (more) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int x = 0; x < A::NC; ++x) k[i][x] = next[i][x];
+        }
+    }
+    if (at < stop) w.tail(end);
+    w.l = sum_over_groups(w.l);
+
+    if constexpr (NW > 1) {
+        if (real) {
+#pragma unroll
+            for (int j = 0; j < A::NJ; ++j) *(f32x4*)&merged[wave][w.c][16 * j + 4 * w.g] = w.o[j];
+            if (w.g == 0) {
+                merged[wave][w.c][D] = w.m;
+                merged[wave][w.c][D + 1] = w.l;
+            }
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 16 * (D / 4); i += NW * 64) {
+            const int cc = i / (D / 4), d = (i - cc * (D / 4)) * 4, rr = rg * 16 + cc;
+            if (rr >= a.rows) break;
+            float m = M_FLOOR, l = 0.f;
+            f32x4 o{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < NW; ++x) m = fmaxf(m, merged[x][cc][D]);
+#pragma unroll
+            for (int x = 0; x < NW; ++x) {
+                const float f = __builtin_amdgcn_exp2f(merged[x][cc][D] - m);
+                l = fmaf(merged[x][cc][D + 1], f, l);
+                o += *(const f32x4*)&merged[x][cc][d] * f;
+            }
+            if (a.part) {
+                float* p = a.part + ((w.bh * a.rows + rr) * a.n_split + split) * (D + 2);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[d + r] = o[r];
+                if (d == 0) {
+                    p[D] = m;
+                    p[D + 1] = l;
+                }
+            } else {
+                const int tt = rr / a.share;
+                T* y = (T*)a.out + (b * a.q_len + tt) * a.ldo + (int64_t)(h0 + rr - tt * a.share) * D + d;
+                const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) Elem<T>::store(y + r, o[r] * inv);
+            }
+        }
+    } else if (real) {
+        if (a.part) {
+            float* p = a.part + ((w.bh * a.rows + row) * a.n_split + split) * (D + 2);
+#pragma unroll
+            for (int j = 0; j < A::NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[16 * j + 4 * w.g + r] = w.o[j][r];
+            if (w.g == 0) {
+                p[D] = w.m;
+                p[D + 1] = w.l;
+            }
+        } else {
+            T* y = (T*)a.out + (b * a.q_len + t) * a.ldo + (int64_t)h * D;
+            const float inv = w.l == 0.f ? 0.f : 1.0f / w.l;
+#pragma unroll
+            for (int j = 0; j < A::NJ; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) Elem<T>::store(y + 16 * j + 4 * w.g + r, w.o[j][r] * inv);
+        }
+    }
+}
+
+// joins the splits of one row, a wave each
+template <typename T>
+__global__ __launch_bounds__(64) void attention_kv8_join_kernel(AttnArgs a) {
+    const int D = a.c.head_dim, lane = threadIdx.x;
+    const int64_t bh = blockIdx.x / a.rows;
+    const int row = (int)(blockIdx.x - bh * a.rows);
+    const float* p = a.part + (int64_t)blockIdx.x * a.n_split * (D + 2);
+    float m = M_FLOOR, l = 0.f, o[2] = {0.f, 0.f};
+    for (int s = 0; s < a.n_split; ++s) m = fmaxf(m, p[(int64_t)s * (D + 2) + D]);
+    for (int s = 0; s < a.n_split; ++s) {
+        const float* ps = p + (int64_t)s * (D + 2);
+        const float f = __builtin_amdgcn_exp2f(ps[D] - m);
+        l = fmaf(ps[D + 1], f, l);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            if (lane + 64 * i < D) o[i] = fmaf(ps[lane + 64 * i], f, o[i]);
+    }
+    const int64_t b = bh / a.c.kv_heads;
+    const int t = row / a.share, h = (int)(bh - b * a.c.kv_heads) * a.share + row - t * a.share;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (lane + 64 * i < D) Elem<T>::store((T*)a.out + (b * a.q_len + t) * a.ldo + (int64_t)h * D + lane + 64 * i, o[i] * inv);
+}
+
+template <typename T, int D>
+static void launch_attention(const AttnArgs& a, int64_t groups, hipStream_t s) {
+    const int64_t grid = groups * a.n_split;
+    // four waves to a head's rows where heads are few, one where they fill the card by themselves
+    if (grid >= 4096)
+        hipLaunchKernelGGL((attention_kv8_kernel<T, D, 1>), dim3((unsigned)grid), dim3(64), 0, s, a);
+    else
+        hipLaunchKernelGGL((attention_kv8_kernel<T, D, 4>), dim3((unsigned)grid), dim3(256), 0, s, a);
+    if (a.n_split > 1)
+        hipLaunchKernelGGL((attention_kv8_join_kernel<T>), dim3((unsigned)(a.c.batch * a.c.kv_heads * a.rows)), dim3(64), 0, s, a);
 }
 
 static int check_cache(const char* who, int dtype, const bt_kv8_cache* c, int* shift) {
@@ -322,9 +735,12 @@ extern "C" int bt_kv8_read(int dtype, const bt_kv8_cache* cache, int64_t n, int6
     return BT_OK;
 }
 
+// Enough workgroups of four waves for the card (256 CUs, two of them to a CU), no split shorter than eight 64-row tiles: two a wave.
 extern "C" int32_t bt_attention_kv8_split_count(int64_t batch, int32_t kv_heads, int32_t group, int32_t q_len, int64_t n) {
-    (void)batch; (void)kv_heads; (void)group; (void)q_len; (void)n;
-    return 1;
+    const int64_t groups = batch * kv_heads * ceil_div((int64_t)group * q_len, 16), tiles = ceil_div(n, 64);
+    if (groups <= 0) return 1;
+    const int64_t want = ceil_div(512, groups), most = tiles / 8;
+    return (int32_t)(want < most ? want : most > 1 ? most : 1);
 }
 
 extern "C" int64_t bt_attention_kv8_workspace_bytes(int64_t batch, int32_t q_len, int32_t heads, int32_t head_dim, int32_t n_split) {
@@ -351,12 +767,18 @@ extern "C" int bt_attention_kv8(int dtype, const bt_kv8_cache* cache, int32_t q_
         set_error("bt_attention_kv8: split workspace too small or unaligned (%lld < %lld bytes)", (long long)ws_bytes, (long long)need);
         return BT_ERR_WORKSPACE;
     }
-    const int64_t grid = cache->batch * q_len * heads;
-    BT_CHECK_ARG(grid < (1ll << 31), "bt_attention_kv8: grid too large");
     a.c = *cache;
     a.q = rows_of(q);
     a.q_len = q_len;
     a.heads = heads;
+    a.share = heads / cache->kv_heads;
+    BT_CHECK_ARG((int64_t)q_len * a.share < (1ll << 30), "bt_attention_kv8: too many rows");
+    a.rows = q_len * a.share;
+    a.row_groups = (a.rows + 15) / 16;
+    a.n_split = n_split;
+    a.part = n_split > 1 ? (float*)ws : nullptr;
+    const int64_t groups = cache->batch * cache->kv_heads * a.row_groups;
+    BT_CHECK_ARG(groups * n_split < (1ll << 31) && cache->batch * cache->kv_heads * a.rows < (1ll << 31), "bt_attention_kv8: grid too large");
     a.pos0_host = pos0_host;
     a.pos0_dev = pos0_dev;
     a.mask = mask;
@@ -366,10 +788,13 @@ extern "C" int bt_attention_kv8(int dtype, const bt_kv8_cache* cache, int32_t q_
     a.scale = 1.4426950408889634f / sqrtf((float)cache->head_dim);
     hipStream_t s = (hipStream_t)stream;
     ProfScope ps(BT_PROF_ATTN_ROWS, s);
-    if (dtype == BT_BF16)
-        hipLaunchKernelGGL(attention_kv8_kernel<bf16>, dim3((unsigned)grid), dim3(64), 0, s, a);
-    else
-        hipLaunchKernelGGL(attention_kv8_kernel<float>, dim3((unsigned)grid), dim3(64), 0, s, a);
+#define BT_ATT8(D_) (dtype == BT_BF16 ? launch_attention<bf16, D_>(a, groups, s) : launch_attention<float, D_>(a, groups, s))
+    switch (cache->head_dim) {
+        case 32: BT_ATT8(32); break;
+        case 64: BT_ATT8(64); break;
+        default: BT_ATT8(128);
+    }
+#undef BT_ATT8
     BT_LAUNCH_CHECK("bt_attention_kv8 launch");
     return BT_OK;
 }
