@@ -67,7 +67,13 @@ static int launch_quant_rows(int64_t M, int64_t K, const void* x, int64_t ldx, c
 }
 
 // ---- bt_linear_q8 ----------------------------------------------------------------------------------------------------------
-struct Q8Epi {
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+struct Q8Args {
+    const int8_t* A;
+    const int8_t* W;
+    int64_t lda, ldw;
+    int M, N, K;
     const float* a_scale;
     const float* w_scale;
     const void* bias;
@@ -76,31 +82,38 @@ struct Q8Epi {
     void* out;
     int64_t ldo;
     int act;
+    int wide;           // out (and residual) take 16-byte accesses
+    int tiles_m, tiles_n;
+    int slices, steps;  // K split into `slices` ranges of `steps` 64-byte steps; > 1: sums go to `slab`
+    int* slab;          // [slices][M][N]
 };
 
-template <typename T>
-__device__ inline void q8_store(const Q8Epi& e, int64_t m, int64_t n, int acc) {
-    float y = (float)acc * (e.a_scale[m] * e.w_scale[n]);
-    if (e.bias) y += Elem<T>::load((const T*)e.bias + n);
-    if (e.act == BT_ACT_GELU) y = 0.5f * y * (1.0f + erff(y * 0.70710678118654752440f));
-    if (e.residual) y += Elem<T>::load((const T*)e.residual + m * e.ldr + n);
-    Elem<T>::store((T*)e.out + m * e.ldo + n, y);
+// act(acc * sx * sw + bias): fp32; the residual joins where the row is written
+__device__ inline float q8_value(int acc, float sa, float sw, float bias, int act) {
+    const float y = fmaf((float)acc, sa * sw, bias);
+    return act == BT_ACT_GELU ? 0.5f * y * (1.0f + erff(y * 0.70710678118654752440f)) : y;
 }
 
-// 64 x 64 tile per workgroup, 64 bytes of K at a time through LDS, four products per v_dot4.
 template <typename T>
-__global__ __launch_bounds__(256) void linear_q8_kernel(const int8_t* __restrict__ A, int64_t lda, const int8_t* __restrict__ W,
-                                                       int64_t ldw, int64_t M, int64_t N, int64_t K, Q8Epi e) {
+__device__ inline void q8_store(const Q8Args& e, int m, int n, int acc) {
+    float y = q8_value(acc, e.a_scale[m], e.w_scale[n], e.bias ? Elem<T>::load((const T*)e.bias + n) : 0.f, e.act);
+    if (e.residual) y += Elem<T>::load((const T*)e.residual + (int64_t)m * e.ldr + n);
+    Elem<T>::store((T*)e.out + (int64_t)m * e.ldo + n, y);
+}
+
+// Any K % 16 == 0: 64 x 64 tile per workgroup, 64 bytes of K at a time through LDS, four products per v_dot4.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_q8_dot_kernel(Q8Args e) {
     __shared__ int4 sa[64][5], sw[64][5];
-    const int64_t m0 = (int64_t)blockIdx.y * 64, n0 = (int64_t)blockIdx.x * 64;
+    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
     const int r = threadIdx.x >> 2, c = threadIdx.x & 3;
     const int tm = (threadIdx.x >> 4) * 4, tn = (threadIdx.x & 15) * 4;
     int acc[4][4] = {};
-    for (int64_t k0 = 0; k0 < K; k0 += 64) {
-        const int64_t k = k0 + c * 16;
+    for (int k0 = 0; k0 < e.K; k0 += 64) {
+        const int k = k0 + c * 16;
         int4 a{0, 0, 0, 0}, w{0, 0, 0, 0};
-        if (k < K && m0 + r < M) a = *(const int4*)(A + (m0 + r) * lda + k);
-        if (k < K && n0 + r < N) w = *(const int4*)(W + (n0 + r) * ldw + k);
+        if (k < e.K && m0 + r < e.M) a = *(const int4*)(e.A + (m0 + r) * e.lda + k);
+        if (k < e.K && n0 + r < e.N) w = *(const int4*)(e.W + (n0 + r) * e.ldw + k);
         __syncthreads();
         sa[r][c] = a;
         sw[r][c] = w;
@@ -128,15 +141,200 @@ __global__ __launch_bounds__(256) void linear_q8_kernel(const int8_t* __restrict
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-            if (m0 + tm + i < M && n0 + tn + j < N) q8_store<T>(e, m0 + tm + i, n0 + tn + j, acc[i][j]);
+            if (m0 + tm + i < e.M && n0 + tn + j < e.N) q8_store<T>(e, m0 + tm + i, n0 + tn + j, acc[i][j]);
+}
+
+// 16 bytes per lane from base + off (unsigned) straight into LDS at lds + 16 * lane.  The waits cover an M0 write right before the load
+// (1) and a base that a v_readlane may just have brought back from a spill (5): neither is padded inside an asm string.
+__device__ inline void dma16(const int8_t* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(off), "s"(base), "s"(lds) : "memory");
+}
+template <int N>
+__device__ inline void wait_loads() {
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
+}
+
+// The tile kernel: 32 MI x 32 NB per workgroup of 2 x 2 waves, 64 bytes of K a step, K % 64 == 0.
+//  * Two workgroups to a CU: while one waits at its barrier or writes its tile, the other's waves have the matrix units.  So a K step
+//    needs one barrier and the epilogue no software overlap.
+//  * A and W travel global -> LDS without registers, NS - 1 steps ahead, in a ring of NS stages.  A wave waits for its own loads of step t
+//    (in order: at most those of the younger steps stay out), then for the others at the barrier; behind it everybody has also consumed
+//    step t - 1, whose stage takes the loads of step t + NS - 1.
+//  * LDS rows are 64 bytes; the four 16-byte pieces of row r are stored in the order p ^ ((r >> 1) & 3) ^ ((r >> 3) & 1): the 16 rows that
+//    a fragment read touches at once are spread over all banks.
+//  * mfma(W, A): a lane gets four neighbouring columns of one row; rows are put together in LDS and leave as 16-byte pieces.
+template <typename T, int MI, int NB, int NS>
+__global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
+    constexpr int BM = 32 * MI, BN = 32 * NB, STAGE = (BM + BN) * 64;
+    constexpr int LA = BM / 64, LW = BN / 64, LOADS = LA + LW;      // 1 KiB loads of a wave and step
+    constexpr int PITCH = 16 * NB * sizeof(T) + 16;                 // a row of the wave's patch: its 16 NB columns
+    constexpr int RING = NS * STAGE, PATCH = 4 * 16 * PITCH;
+    __shared__ __attribute__((aligned(16))) char smem[RING > PATCH ? RING : PATCH];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 1, wn = wave & 1, c = lane & 15, g = lane >> 4;
+
+    // workgroups of one XCD (ids that are equal mod 8) take neighbouring tiles, in columns of 8 tile rows: its L2 serves them with each
+    // other's panels
+    const int tiles = e.tiles_m * e.tiles_n, id = blockIdx.x;
+    const int per = tiles >> 3, rest = tiles & 7, xcd = id & 7, local = id >> 3;
+    const int at = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + local;
+    const int group = at / (8 * e.tiles_n), first = group * 8, high = min(e.tiles_m - first, 8), in = at - group * 8 * e.tiles_n;
+    const int m0 = (first + in % high) * BM, n0 = (in / high) * BN;
+
+    const int k0 = blockIdx.y * e.steps * 64, steps = min(e.steps, (e.K - k0) >> 6);
+    const int8_t* A = e.A + (int64_t)m0 * e.lda + k0;
+    const int8_t* W = e.W + (int64_t)n0 * e.ldw + k0;
+    uint32_t off[LOADS];
+    const int row16 = lane >> 2, piece = (lane & 3) ^ ((row16 >> 1) & 3) ^ ((row16 >> 3) & 1);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        int row = i < LA ? (wave * LA + i) * 16 + row16 : (wave * LW + i - LA) * 16 + row16;
+        const int last = i < LA ? e.M - 1 - m0 : e.N - 1 - n0;      // rows beyond the matrix repeat its last one
+        row = row < last ? row : last;
+        off[i] = (uint32_t)row * (uint32_t)(i < LA ? e.lda : e.ldw) + piece * 16;
+    }
+    const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)smem;
+    auto load = [&](int t) {
+        const uint32_t stage = ring + (t % NS) * STAGE;
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i)
+            if (i < LA) dma16(A + (int64_t)t * 64, off[i], stage + (wave * LA + i) * 1024);
+            else dma16(W + (int64_t)t * 64, off[i], stage + BM * 64 + (wave * LW + i - LA) * 1024);
+    };
+    i32x4 acc[MI][NB];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int t = 0; t < NS - 1; ++t)
+        if (t < steps) load(t);
+
+    const int frag = c * 64 + (g ^ ((c >> 1) & 3) ^ ((c >> 3) & 1)) * 16;
+    int stage = 0;
+    for (int t = 0; t < steps; ++t) {
+        if (t + NS - 2 < steps) wait_loads<LOADS * (NS - 2)>();
+        else if (NS > 3 && t + 1 < steps) wait_loads<LOADS>();
+        else wait_loads<0>();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + NS - 1 < steps) load(t + NS - 1);
+        const char* a = smem + stage * STAGE + wm * MI * 1024 + frag;
+        const char* w = smem + stage * STAGE + BM * 64 + wn * NB * 1024 + frag;
+        i32x4 af[MI], wf[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) wf[j] = *(const i32x4*)(w + j * 1024);
+#pragma unroll
+        for (int i = 0; i < MI; ++i) af[i] = *(const i32x4*)(a + i * 1024);
+#pragma unroll
+        for (int i = 0; i < MI; ++i)
+#pragma unroll
+            for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], af[i], acc[i][j], 0, 0, 0);
+        stage = stage + 1 == NS ? 0 : stage + 1;
+    }
+
+    const int m_w = m0 + wm * MI * 16, n_w = n0 + wn * NB * 16;
+    if (e.slices > 1) {
+        int* slab = e.slab + (int64_t)blockIdx.y * e.M * e.N;
+#pragma unroll
+        for (int i = 0; i < MI; ++i) {
+            const int m = m_w + i * 16 + c;
+            if (m >= e.M) continue;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int n = n_w + j * 16 + g * 4;
+                if (n + 4 <= e.N && (e.N & 3) == 0) *(i32x4*)(slab + (int64_t)m * e.N + n) = acc[i][j];
+                else
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (n + r < e.N) slab[(int64_t)m * e.N + n + r] = acc[i][j][r];
+            }
+        }
+        return;
+    }
+    float sw[NB][4], bias[NB][4];
+#pragma unroll
+    for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int n = n_w + j * 16 + g * 4 + r < e.N ? n_w + j * 16 + g * 4 + r : e.N - 1;
+            sw[j][r] = e.w_scale[n];
+            bias[j][r] = e.bias ? Elem<T>::load((const T*)e.bias + n) : 0.f;
+        }
+    __syncthreads();      // the ring is the patches' now
+    char* patch = smem + wave * 16 * PITCH;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const int m = m_w + i * 16 + c;
+        const float sa = e.a_scale[m < e.M ? m : e.M - 1];
+        float res[NB][4] = {};      // joins before the one rounding
+        if (e.residual && m < e.M) {
+            const T* p = (const T*)e.residual + (int64_t)m * e.ldr + n_w + g * 4;
+#pragma unroll
+            for (int j = 0; j < NB; ++j) {
+                const int n = n_w + j * 16 + g * 4;
+                if (e.wide && n + 4 <= e.N) {
+                    if constexpr (sizeof(T) == 2) {
+                        const uint2 u = *(const uint2*)(p + j * 16);
+                        res[j][0] = __uint_as_float(u.x << 16), res[j][1] = __uint_as_float(u.x & 0xffff0000u);
+                        res[j][2] = __uint_as_float(u.y << 16), res[j][3] = __uint_as_float(u.y & 0xffff0000u);
+                    } else {
+                        const float4 u = *(const float4*)(p + j * 16);
+                        res[j][0] = u.x, res[j][1] = u.y, res[j][2] = u.z, res[j][3] = u.w;
+                    }
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (n + r < e.N) res[j][r] = Elem<T>::load(p + j * 16 + r);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            float y[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = q8_value(acc[i][j][r], sa, sw[j][r], bias[j][r], e.act) + res[j][r];
+            if constexpr (sizeof(T) == 2) *(uint2*)(patch + c * PITCH + (j * 16 + g * 4) * 2) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+            else *(float4*)(patch + c * PITCH + (j * 16 + g * 4) * 4) = float4{y[0], y[1], y[2], y[3]};
+        }
+        asm volatile("" ::: "memory");      // the patch is the wave's own, and a wave's LDS accesses stay in order
+        constexpr int V = Elem<T>::VEC, CH = 16 * NB / V;      // 16-byte pieces of a row
+#pragma unroll
+        for (int x = 0; x < 16 * CH; x += 64) {
+            const int r = (x + lane) / CH, d = ((x + lane) - r * CH) * V, mm = m_w + i * 16 + r, n = n_w + d;
+            if (mm >= e.M || n >= e.N) continue;
+            float y[V];
+            load_vec<T>((const T*)(patch + r * PITCH) + d, y);
+            T* out = (T*)e.out + (int64_t)mm * e.ldo + n;
+            if (e.wide && n + V <= e.N) store_vec<T>(out, y);
+            else
+#pragma unroll
+                for (int q = 0; q < V; ++q)
+                    if (n + q < e.N) Elem<T>::store(out + q, y[q]);
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
+template <typename T, int MI, int NB, int NS>
+static void launch_tile(Q8Args& e, hipStream_t s) {
+    e.tiles_m = (int)ceil_div(e.M, 32 * MI);
+    e.tiles_n = (int)ceil_div(e.N, 32 * NB);
+    e.slices = 1;
+    e.steps = e.K / 64;
+    hipLaunchKernelGGL((linear_q8_tile_kernel<T, MI, NB, NS>), dim3((unsigned)(e.tiles_m * e.tiles_n), 1), dim3(256), 0, s, e);
 }
 
 template <typename T>
-static int launch_linear_q8(int64_t M, int64_t N, int64_t K, const int8_t* A, int64_t lda, const int8_t* W, int64_t ldw, const Q8Epi& e,
-                            hipStream_t s) {
+static int launch_linear_q8(Q8Args& e, hipStream_t s) {
     ProfScope ps(BT_PROF_LINEAR_MFMA, s);
-    hipLaunchKernelGGL((linear_q8_kernel<T>), dim3((unsigned)ceil_div(N, 64), (unsigned)ceil_div(M, 64)), dim3(256), 0, s, A, lda, W, ldw,
-                       M, N, K, e);
+    if (e.K % 64 == 0 && e.lda < (1 << 23) && e.ldw < (1 << 23)) {
+        const int64_t big = ceil_div(e.M, 256) * ceil_div(e.N, 128);
+        if (big >= 512) launch_tile<T, 8, 4, 3>(e, s);
+        else if (ceil_div(e.M, 128) * ceil_div(e.N, 128) >= 256) launch_tile<T, 4, 4, 4>(e, s);
+        else launch_tile<T, 2, 2, 4>(e, s);
+    } else
+        hipLaunchKernelGGL((linear_q8_dot_kernel<T>), dim3((unsigned)ceil_div(e.N, 64), (unsigned)ceil_div(e.M, 64)), dim3(256), 0, s, e);
     BT_LAUNCH_CHECK("bt_linear_q8 launch");
     return BT_OK;
 }
@@ -169,7 +367,7 @@ extern "C" int bt_linear_q8(int dtype, int64_t M, int64_t N, int64_t K, const in
                             const int8_t* W, int64_t ldw, const float* w_scale, const void* bias, const void* residual, int64_t ldr,
                             void* out, int64_t ldo, int act, void* scratch, int64_t scratch_bytes, bt_stream stream) {
     BT_CHECK_ARG(dtype == BT_F32 || dtype == BT_BF16, "bt_linear_q8: bad dtype %d", dtype);
-    BT_CHECK_ARG(M >= 0 && N > 0 && K > 0 && M < (1ll << 22) && N < (1ll << 31), "bt_linear_q8: bad shape M=%lld N=%lld K=%lld",
+    BT_CHECK_ARG(M >= 0 && N > 0 && K > 0 && M < (1ll << 22) && N < (1ll << 22), "bt_linear_q8: bad shape M=%lld N=%lld K=%lld",
                  (long long)M, (long long)N, (long long)K);
     BT_CHECK_ARG(K % 16 == 0 && K <= 131056, "bt_linear_q8: K = %lld is not a multiple of 16 up to 131056", (long long)K);
     if (M == 0) return BT_OK;      // (an empty tensor has no pointer)
@@ -179,7 +377,23 @@ extern "C" int bt_linear_q8(int dtype, int64_t M, int64_t N, int64_t K, const in
     BT_CHECK_ARG(ldo >= N && (!residual || ldr >= N), "bt_linear_q8: row stride smaller than row");
     BT_CHECK_ARG(act == BT_ACT_NONE || act == BT_ACT_GELU, "bt_linear_q8: bad act %d", act);
     BT_CHECK_ARG(!scratch || (scratch_bytes >= 0 && aligned16(scratch)), "bt_linear_q8: scratch must be 16-byte aligned");
-    const Q8Epi e{a_scale, w_scale, bias, residual, ldr, out, ldo, act};
-    if (dtype == BT_BF16) return launch_linear_q8<bf16>(M, N, K, A, lda, W, ldw, e, (hipStream_t)stream);
-    return launch_linear_q8<float>(M, N, K, A, lda, W, ldw, e, (hipStream_t)stream);
+    Q8Args e{};
+    e.A = A;
+    e.W = W;
+    e.lda = lda;
+    e.ldw = ldw;
+    e.M = (int)M;
+    e.N = (int)N;
+    e.K = (int)K;
+    e.a_scale = a_scale;
+    e.w_scale = w_scale;
+    e.bias = bias;
+    e.residual = residual;
+    e.ldr = ldr;
+    e.out = out;
+    e.ldo = ldo;
+    e.act = act;
+    const int V = dtype == BT_BF16 ? 8 : 4;
+    e.wide = aligned16(out) && ldo % V == 0 && (!residual || (aligned16(residual) && ldr % V == 0));
+    return dtype == BT_BF16 ? launch_linear_q8<bf16>(e, (hipStream_t)stream) : launch_linear_q8<float>(e, (hipStream_t)stream);
 }
