@@ -108,8 +108,8 @@ __global__ __launch_bounds__(64) void kv8_append_kernel(AppendArgs a) {
                 const float v = at < 0 ? Elem<T>::load(vt + d * bl + t) : Elem<T>::load(vsrc + at * a.v.t + d);
                 T kr;
                 Elem<T>::store(&kr, k);
-                a.c.k_codes[(bh * a.c.n_max + row0 + t) * D + d] = (int8_t)qk.code(Elem<T>::load(&kr));
-                a.c.v_codes[((bh * n_blk + blk) * D + d) * bl + t] = (int8_t)qv.code(v);
+                a.c.k_codes[(bh * a.c.n_max + row0 + t) * D + d] = (int8_t)qk.exact(Elem<T>::load(&kr));
+                a.c.v_codes[((bh * n_blk + blk) * D + d) * bl + t] = (int8_t)qv.exact(v);
             }
         } else {
             for (int e = lane; e < bl * D; e += 64) {
@@ -596,29 +596,43 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 2 : 2) void attention_kv8_kernel
     }
 }
 
-// joins the splits of one row, a wave each
-template <typename T>
-__global__ __launch_bounds__(64) void attention_kv8_join_kernel(AttnArgs a) {
-    const int D = a.c.head_dim, lane = threadIdx.x;
+// Joins the splits of one row: a workgroup each.  Thread x sums column x % D of every (256 / D)-th split, so that the loads of a row are
+// 256 / D splits abreast and independent of each other; the 256 / D partial sums meet in LDS.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attention_kv8_join_kernel(AttnArgs a) {
+    constexpr int G = 256 / D;
+    __shared__ float part[G][D + 1], most[4];
+    const int tid = threadIdx.x, d = tid % D, sub = tid / D;
     const int64_t bh = blockIdx.x / a.rows;
     const int row = (int)(blockIdx.x - bh * a.rows);
     const float* p = a.part + (int64_t)blockIdx.x * a.n_split * (D + 2);
-    float m = M_FLOOR, l = 0.f, o[2] = {0.f, 0.f};
-    for (int s = 0; s < a.n_split; ++s) m = fmaxf(m, p[(int64_t)s * (D + 2) + D]);
-    for (int s = 0; s < a.n_split; ++s) {
+    float m = M_FLOOR;
+    for (int s = tid; s < a.n_split; s += 256) m = fmaxf(m, p[(int64_t)s * (D + 2) + D]);
+    m = wave_max(m);
+    if ((tid & 63) == 0) most[tid >> 6] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));
+    float l = 0.f, o = 0.f;
+#pragma unroll 4
+    for (int s = sub; s < a.n_split; s += G) {
         const float* ps = p + (int64_t)s * (D + 2);
         const float f = __builtin_amdgcn_exp2f(ps[D] - m);
         l = fmaf(ps[D + 1], f, l);
+        o = fmaf(ps[d], f, o);
+    }
+    part[sub][d] = o;
+    if (d == 0) part[sub][D] = l;
+    __syncthreads();
+    if (tid >= D) return;
+    l = o = 0.f;
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-            if (lane + 64 * i < D) o[i] = fmaf(ps[lane + 64 * i], f, o[i]);
+    for (int x = 0; x < G; ++x) {
+        o += part[x][d];
+        l += part[x][D];
     }
     const int64_t b = bh / a.c.kv_heads;
     const int t = row / a.share, h = (int)(bh - b * a.c.kv_heads) * a.share + row - t * a.share;
-    const float inv = l == 0.f ? 0.f : 1.0f / l;
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (lane + 64 * i < D) Elem<T>::store((T*)a.out + (b * a.q_len + t) * a.ldo + (int64_t)h * D + lane + 64 * i, o[i] * inv);
+    Elem<T>::store((T*)a.out + (b * a.q_len + t) * a.ldo + (int64_t)h * D + d, l == 0.f ? 0.f : o / l);
 }
 
 template <typename T, int D>
@@ -630,7 +644,7 @@ static void launch_attention(const AttnArgs& a, int64_t groups, hipStream_t s) {
     else
         hipLaunchKernelGGL((attention_kv8_kernel<T, D, 4>), dim3((unsigned)grid), dim3(256), 0, s, a);
     if (a.n_split > 1)
-        hipLaunchKernelGGL((attention_kv8_join_kernel<T>), dim3((unsigned)(a.c.batch * a.c.kv_heads * a.rows)), dim3(64), 0, s, a);
+        hipLaunchKernelGGL((attention_kv8_join_kernel<T, D>), dim3((unsigned)(a.c.batch * a.c.kv_heads * a.rows)), dim3(256), 0, s, a);
 }
 
 static int check_cache(const char* who, int dtype, const bt_kv8_cache* c, int* shift) {

@@ -5,63 +5,190 @@
 namespace bt {
 
 // ---- bt_quant_rows ---------------------------------------------------------------------------------------------------------
-// One wave per row, 4 rows per workgroup: LayerNorm statistics (two-pass, as bt_layernorm), the largest magnitude, the codes.
-template <typename T, bool LN>
+// A row is read once into registers -- NV 16-byte pieces a lane, all loads in flight together -- and everything else happens there:
+// LayerNorm statistics (two-pass, fp32), the largest magnitude, the codes.  R waves to a row: one where there are rows enough for
+// the card (no barrier), four where there are not or where the row does not fit one wave's registers.  Bound by memory: x in, one
+// byte a value out.
+template <int R>
+struct RowReduce {      // over the R waves of a row (R = 4: the workgroup)
+    float* slot;
+    int wave;
+    __device__ inline float sum(float v) {
+        v = wave_sum(v);
+        if (R == 1) return v;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) slot[wave] = v;
+        __syncthreads();
+        return slot[0] + slot[1] + slot[2] + slot[3];
+    }
+    __device__ inline float max(float v) {
+        v = wave_max(v);
+        if (R == 1) return v;
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) slot[wave] = v;
+        __syncthreads();
+        return fmaxf(fmaxf(slot[0], slot[1]), fmaxf(slot[2], slot[3]));
+    }
+};
+
+// values c .. c + V - 1 of a row of K (zero beyond); VEC: the row is 16-byte aligned
+template <typename T, bool VEC>
+__device__ inline void load_piece(const T* row, int c, int K, float (&v)[Elem<T>::VEC]) {
+    constexpr int V = Elem<T>::VEC;
+    if (VEC && c + V <= K) load_vec<T>(row + c, v);
+    else
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = c + i < K ? Elem<T>::load(row + c + i) : 0.f;
+}
+
+template <typename T, bool LN, bool VEC, int NV, int R>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
                                                         const T* __restrict__ b, float eps, int8_t* __restrict__ codes, int64_t ldc,
-                                                        float* __restrict__ scales, int64_t M, int64_t K) {
-    const int lane = threadIdx.x & 63;
-    const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+                                                        float* __restrict__ scales, int64_t M, int K) {
+    constexpr int V = Elem<T>::VEC;
+    __shared__ float slot[4];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int64_t row = R == 1 ? (int64_t)blockIdx.x * 4 + wave : blockIdx.x;
     if (row >= M) return;
+    const int at = R == 1 ? lane : threadIdx.x;      // piece i of this lane begins at column (i * 64 R + at) * V
+    RowReduce<R> all{slot, wave};
+    const T* xr = x + row * ldx;
+    float v[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_piece<T, VEC>(xr, (i * 64 * R + at) * V, K, v[i]);
+    if (LN) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) sum += v[i][e];
+        const float mean = all.sum(sum) / (float)K;
+        float sq = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                v[i][e] -= mean;
+                if ((i * 64 * R + at) * V + e < K) sq = fmaf(v[i][e], v[i][e], sq);
+            }
+        const float rstd = rsqrtf(all.sum(sq) / (float)K + eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 64 * R + at) * V;
+            float wv[V], bv[V];
+            load_piece<T, VEC>(w, c, K, wv);
+            load_piece<T, VEC>(b, c, K, bv);
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, wv[e], bv[e]);      // 0 beyond K, as wv and bv are
+        }
+    }
+    float amax = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+            if (LN && v[i][e] != v[i][e] && (i * 64 * R + at) * V + e >= K) v[i][e] = 0.f;      // (0 * an infinite rstd)
+            amax = fmaxf(amax, fabsf(v[i][e]));
+            odd |= !(fabsf(v[i][e]) < INFINITY);
+        }
+    amax = all.max(odd ? INFINITY : amax);
+    const bool bad = amax == INFINITY;
+    const Quantiser q(bad ? 0.f : amax);
+    if (at == 0) scales[row] = bad ? __int_as_float(0x7fc00000) : q.scale;
+    int8_t* cr = codes + row * ldc;
+    const int Kp = (K + 15) & ~15;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (i * 64 * R + at) * V;
+        if (c >= Kp) continue;
+        uint32_t out[V / 4];
+#pragma unroll
+        for (int e = 0; e < V; e += 4)
+            out[e / 4] = bad ? 0u : q.direct ? q.pack4(v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3])
+                                             : q.pack4_exact(v[i][e], v[i][e + 1], v[i][e + 2], v[i][e + 3]);
+        if constexpr (V == 8) *(uint2*)(cr + c) = uint2{out[0], out[1]};
+        else *(uint32_t*)(cr + c) = out[0];
+    }
+}
+
+// Rows longer than four waves' registers: a workgroup passes over the row once for each of the steps above.
+template <typename T, bool LN>
+__global__ __launch_bounds__(256) void quant_long_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
+                                                             const T* __restrict__ b, float eps, int8_t* __restrict__ codes, int64_t ldc,
+                                                             float* __restrict__ scales, int64_t K) {
+    __shared__ float slot[4];
+    RowReduce<4> all{slot, (int)threadIdx.x >> 6};
+    const int64_t row = blockIdx.x;
     const T* xr = x + row * ldx;
     float mean = 0.f, rstd = 1.f;
     if (LN) {
-        float sum = 0.f;
-        for (int64_t c = lane; c < K; c += 64) sum += Elem<T>::load(xr + c);
-        mean = wave_sum(sum) / (float)K;
-        float sq = 0.f;
-        for (int64_t c = lane; c < K; c += 64) {
+        float sum = 0.f, sq = 0.f;
+        for (int64_t c = threadIdx.x; c < K; c += 256) sum += Elem<T>::load(xr + c);
+        mean = all.sum(sum) / (float)K;
+        for (int64_t c = threadIdx.x; c < K; c += 256) {
             const float d = Elem<T>::load(xr + c) - mean;
             sq = fmaf(d, d, sq);
         }
-        rstd = rsqrtf(wave_sum(sq) / (float)K + eps);
+        rstd = rsqrtf(all.sum(sq) / (float)K + eps);
     }
+    auto value = [&](int64_t c) {
+        const float v = Elem<T>::load(xr + c);
+        return LN ? fmaf((v - mean) * rstd, Elem<T>::load(w + c), Elem<T>::load(b + c)) : v;
+    };
     float amax = 0.f;
-    bool bad = false;
-    for (int64_t c = lane; c < K; c += 64) {
-        float v = Elem<T>::load(xr + c);
-        if (LN) v = fmaf((v - mean) * rstd, Elem<T>::load(w + c), Elem<T>::load(b + c));
-        amax = fmaxf(amax, fabsf(v));
-        bad |= !(fabsf(v) < INFINITY);
+    for (int64_t c = threadIdx.x; c < K; c += 256) {
+        const float v = fabsf(value(c));
+        amax = v < INFINITY ? fmaxf(amax, v) : INFINITY;
     }
-    amax = wave_max(amax);
-    bad = __any(bad);
+    amax = all.max(amax);
+    const bool bad = amax == INFINITY;
     const Quantiser q(bad ? 0.f : amax);
-    if (lane == 0) scales[row] = bad ? __int_as_float(0x7fc00000) : q.scale;
+    if (threadIdx.x == 0) scales[row] = bad ? __int_as_float(0x7fc00000) : q.scale;
     int8_t* cr = codes + row * ldc;
     const int64_t Kp = (K + 15) / 16 * 16;
-    for (int64_t c = lane; c < Kp; c += 64) {
-        int code = 0;
-        if (c < K && !bad) {
-            float v = Elem<T>::load(xr + c);
-            if (LN) v = fmaf((v - mean) * rstd, Elem<T>::load(w + c), Elem<T>::load(b + c));
-            code = q.code(v);
-        }
-        cr[c] = (int8_t)code;
-    }
+    for (int64_t c = threadIdx.x; c < Kp; c += 256) cr[c] = (int8_t)(c < K && !bad ? q.exact(value(c)) : 0);
 }
 
 template <typename T>
 static int launch_quant_rows(int64_t M, int64_t K, const void* x, int64_t ldx, const void* w, const void* b, float eps, int8_t* codes,
                              int64_t ldc, float* scales, hipStream_t s) {
+    constexpr int V = Elem<T>::VEC;
     ProfScope ps(BT_PROF_LAYERNORM, s);
-    const dim3 grid((unsigned)ceil_div(M, 4));
-    if (w)
-        hipLaunchKernelGGL((quant_rows_kernel<T, true>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, codes,
-                           ldc, scales, M, K);
-    else
-        hipLaunchKernelGGL((quant_rows_kernel<T, false>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, codes,
-                           ldc, scales, M, K);
+    const bool vec = aligned16(x) && (ldx % V == 0 || M == 1) && (!w || (aligned16(w) && aligned16(b)));
+    const int64_t wave_pieces = ceil_div(K, 64 * V), group_pieces = ceil_div(K, 256 * V);
+    // one wave to a row from 2048 rows (8 waves to a CU) while it has at most 8 pieces a lane
+    const bool one = wave_pieces <= 8 && M >= 2048;
+    const int64_t pieces = one ? wave_pieces : group_pieces;
+    const dim3 grid((unsigned)(one ? ceil_div(M, 4) : M));
+#define BT_QR(LN_, VEC_, NV_, R_)                                                                                                    \
+    hipLaunchKernelGGL((quant_rows_kernel<T, LN_, VEC_, NV_, R_>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, \
+                       codes, ldc, scales, M, (int)K)
+#define BT_QR_PIECES(LN_, VEC_, R_)              \
+    do {                                         \
+        if (pieces <= 1) BT_QR(LN_, VEC_, 1, R_); \
+        else if (pieces <= 2) BT_QR(LN_, VEC_, 2, R_); \
+        else if (pieces <= 4) BT_QR(LN_, VEC_, 4, R_); \
+        else BT_QR(LN_, VEC_, 8, R_);            \
+    } while (0)
+#define BT_QR_ROW(LN_, VEC_)                     \
+    do {                                         \
+        if (one) BT_QR_PIECES(LN_, VEC_, 1);     \
+        else BT_QR_PIECES(LN_, VEC_, 4);         \
+    } while (0)
+    if (pieces > 8) {
+        if (w) hipLaunchKernelGGL((quant_long_rows_kernel<T, true>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, codes, ldc, scales, K);
+        else hipLaunchKernelGGL((quant_long_rows_kernel<T, false>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, codes, ldc, scales, K);
+    } else if (w) {
+        if (vec) BT_QR_ROW(true, true);
+        else BT_QR_ROW(true, false);
+    } else {
+        if (vec) BT_QR_ROW(false, true);
+        else BT_QR_ROW(false, false);
+    }
+#undef BT_QR_ROW
+#undef BT_QR_PIECES
+#undef BT_QR
     BT_LAUNCH_CHECK("bt_quant_rows launch");
     return BT_OK;
 }
