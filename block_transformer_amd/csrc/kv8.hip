@@ -15,8 +15,10 @@ struct AppendArgs {
     bt_kv8_cache c;
     Rows q, q_out, k, v;
     int64_t kv_items;      // waves for keys and values: batch * kv_heads * blocks
+    int64_t q_rows;        // batch * q_len * heads
     int blocks;            // blocks that q_len rows can touch
-    int q_len, heads, rot, pos0_host, shift;
+    int q_len, heads, rot, pos0_host;
+    bool vec_rope;
     const int32_t* pos0_dev;
     const int32_t* pos_table;
     const float* cos_tab;
@@ -24,122 +26,300 @@ struct AppendArgs {
     int64_t max_pos;
 };
 
-template <typename T>
-__device__ inline float rotated(const T* row, int e, int rot, int64_t angle, const float* cos_tab, const float* sin_tab) {
-    const float x = Elem<T>::load(row + e);
-    const int half = rot >> 1;
-    if (e >= 2 * half) return x;
-    const int j = e < half ? e : e - half;
-    const double c = cos_tab[angle * half + j], s = sin_tab[angle * half + j];
-    const double o = Elem<T>::load(row + (e < half ? e + half : e - half));
-    return (float)(e < half ? (double)x * c - o * s : (double)x * c + o * s);
-}
-
 __device__ inline int64_t angle_of(const AppendArgs& a, int pos) {
     int64_t r = a.pos_table ? a.pos_table[pos] : pos;
     r = r < 0 ? 0 : r;
     return r < a.max_pos ? r : a.max_pos - 1;
 }
 
-// One wave per (sequence, head, block) that the new rows touch; the waves behind them rotate q, one (row, head) each.
+// Dims e0 .. e0 + V - 1 of a row, rotated.  The two products of 24-bit numbers are exact in fp64, so the result is the exact one rounded
+// once: codes (and so what is compared bit for bit) do not depend on how a sum was fused.  Costs nothing here: memory is the bound.
 template <typename T>
-__global__ __launch_bounds__(64) void kv8_append_kernel(AppendArgs a) {
-    const int D = a.c.head_dim, bl = a.c.block, lane = threadIdx.x;
-    const int pos0 = a.pos0_dev ? *a.pos0_dev : a.pos0_host;
-    if (pos0 < 0) return;
-    if (blockIdx.x >= a.kv_items) {
-        const int64_t i = blockIdx.x - a.kv_items;
-        const int64_t b = i / ((int64_t)a.q_len * a.heads);
-        const int th = (int)(i - b * a.q_len * a.heads), t = th / a.heads, h = th - t * a.heads;
-        const T* src = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
-        T* dst = (T*)a.q_out.p + b * a.q_out.b + t * a.q_out.t + h * a.q_out.h;
-        const int64_t ang = angle_of(a, pos0 + t);
-        float y[2];
-        for (int i2 = 0; i2 < 2; ++i2)
-            if (lane + 64 * i2 < D) y[i2] = rotated<T>(src, lane + 64 * i2, a.rot, ang, a.cos_tab, a.sin_tab);
-        __syncthreads();
-        for (int i2 = 0; i2 < 2; ++i2)
-            if (lane + 64 * i2 < D) Elem<T>::store(dst + lane + 64 * i2, y[i2]);
-        return;
-    }
-    const int64_t bh = blockIdx.x / a.blocks;
-    const int item = (int)(blockIdx.x - bh * a.blocks);
-    const int64_t b = bh / a.c.kv_heads;
-    const int h = (int)(bh - b * a.c.kv_heads);
-    const int64_t end = pos0 + (int64_t)a.q_len < a.c.n_max ? pos0 + (int64_t)a.q_len : a.c.n_max;
-    const int first = pos0 >> a.shift;
-    const T* ksrc = (const T*)a.k.p + b * a.k.b + h * a.k.h;
-    const T* vsrc = (const T*)a.v.p + b * a.v.b + h * a.v.h;
-    T* kt = (T*)a.c.k_tail + bh * bl * D;
-    T* vt = (T*)a.c.v_tail + bh * bl * D;
-    const int64_t n_blk = a.c.n_max >> a.shift;
-    const int last = (int)(end >> a.shift);      // the block that stays open
-    // the open block's rows take the places that the first block's old rows leave: the same wave does both, in that order
-    for (int pass = 0; pass < 2; ++pass) {
-        const int blk = pass == 0 ? first + item : last;
-        if (pass == 1 && (item != 0 || last == first)) return;
-        if (pass == 0 && blk > first && blk >= last) return;
-        const int64_t row0 = (int64_t)blk * bl;
-        if (row0 >= end) continue;
-        if (row0 + bl <= end) {
-            float ka = 0.f, va = 0.f;
-            for (int e = lane; e < bl * D; e += 64) {
-                const int t = e / D, d = e - t * D;
-                const int64_t at = row0 + t - pos0;
-                const float k = at < 0 ? Elem<T>::load(kt + t * D + d)
-                                       : rotated<T>(ksrc + at * a.k.t, d, a.rot, angle_of(a, pos0 + (int)at), a.cos_tab, a.sin_tab);
-                const float v = at < 0 ? Elem<T>::load(vt + d * bl + t) : Elem<T>::load(vsrc + at * a.v.t + d);
-                T kr;
-                Elem<T>::store(&kr, k);
-                const float kf = Elem<T>::load(&kr);
-                if (fabsf(kf) < INFINITY) ka = fmaxf(ka, fabsf(kf));
-                if (fabsf(v) < INFINITY) va = fmaxf(va, fabsf(v));
+__device__ inline void rotated_piece(const AppendArgs& a, const T* row, int e0, int64_t angle, float (&v)[Elem<T>::VEC]) {
+    constexpr int V = Elem<T>::VEC;
+    load_vec<T>(row + e0, v);
+    if (e0 >= a.rot) return;
+    const int half = a.rot >> 1;
+    if (a.vec_rope) {      // half is a multiple of V: the other halves are one piece too
+        const bool low = e0 < half;
+        const int j = low ? e0 : e0 - half;
+        float o[V];
+        load_vec<T>(row + (low ? e0 + half : j), o);
+        const float* c = a.cos_tab + angle * half + j;
+        const float* s = a.sin_tab + angle * half + j;
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 cc = *(const float4*)(c + i), ss = *(const float4*)(s + i);
+            const float cs[4] = {cc.x, cc.y, cc.z, cc.w}, sn[4] = {ss.x, ss.y, ss.z, ss.w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const double p = (double)o[i + k] * (low ? -sn[k] : sn[k]);
+                v[i + k] = (float)fma((double)v[i + k], (double)cs[k], p);
             }
-            const Quantiser qk(wave_max(ka)), qv(wave_max(va));
-            if (lane == 0) {
-                a.c.k_scale[bh * n_blk + blk] = qk.scale;
-                a.c.v_scale[bh * n_blk + blk] = qv.scale;
-            }
-            for (int e = lane; e < bl * D; e += 64) {
-                const int t = e / D, d = e - t * D;
-                const int64_t at = row0 + t - pos0;
-                const float k = at < 0 ? Elem<T>::load(kt + t * D + d)
-                                       : rotated<T>(ksrc + at * a.k.t, d, a.rot, angle_of(a, pos0 + (int)at), a.cos_tab, a.sin_tab);
-                const float v = at < 0 ? Elem<T>::load(vt + d * bl + t) : Elem<T>::load(vsrc + at * a.v.t + d);
-                T kr;
-                Elem<T>::store(&kr, k);
-                a.c.k_codes[(bh * a.c.n_max + row0 + t) * D + d] = (int8_t)qk.exact(Elem<T>::load(&kr));
-                a.c.v_codes[((bh * n_blk + blk) * D + d) * bl + t] = (int8_t)qv.exact(v);
-            }
-        } else {
-            for (int e = lane; e < bl * D; e += 64) {
-                const int t = e / D, d = e - t * D;
-                const int64_t at = row0 + t - pos0;
-                if (at < 0 || row0 + t >= end) continue;
-                Elem<T>::store(kt + t * D + d, rotated<T>(ksrc + at * a.k.t, d, a.rot, angle_of(a, pos0 + (int)at), a.cos_tab, a.sin_tab));
-                Elem<T>::store(vt + d * bl + t, Elem<T>::load(vsrc + at * a.v.t + d));
-            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int e = e0 + i;
+            if (e >= a.rot) break;
+            const int j = e < half ? e : e - half;
+            const double o = Elem<T>::load(row + (e < half ? e + half : j)), c = a.cos_tab[angle * half + j], s = a.sin_tab[angle * half + j];
+            v[i] = (float)fma((double)v[i], c, e < half ? -o * s : o * s);
         }
     }
 }
 
-// ---- bt_kv8_read -----------------------------------------------------------------------------------------------------------
 template <typename T>
-__global__ __launch_bounds__(256) void kv8_read_kernel(bt_kv8_cache c, int shift, int64_t n, int64_t first, int64_t count,
+__device__ inline float rounded(float v) {
+    if constexpr (sizeof(T) == 2) return bf16_to_f32(f32_to_bf16(v));
+    return v;
+}
+
+// the scale of a block: the largest finite magnitude; `odd`: not everything was finite
+struct BlockMax {
+    float amax = 0.f;
+    bool odd = false;
+    __device__ inline void see(float v) {
+        const float x = fabsf(v);
+        const bool fine = x < INFINITY;
+        odd |= !fine;
+        amax = fmaxf(amax, fine ? x : 0.f);
+    }
+    __device__ inline void join() {
+        amax = wave_max(amax);
+        odd = __any(odd);
+    }
+};
+
+// One wave per (sequence, head, block) that the new rows touch; the waves behind them rotate q.
+//   K: a lane has 16-byte pieces of rows, as memory has them.
+//   V: a lane has columns 2 x, 2 x + 1 of 16 rows, that is two 16-byte runs of v_codes: rows are read 256 bytes a wave and instruction,
+//      and no transpose is needed.  Rows of the open block come in runs from v_tail, which is transposed already.
+// Bound by memory; K and V are each held in registers between the search for the scale and the codes.
+template <typename T, int D, int BL>
+__global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
+    constexpr int V = Elem<T>::VEC, RP = D / V;      // pieces of a row
+    const int lane = threadIdx.x & 63;
+    const int pos0 = a.pos0_dev ? *a.pos0_dev : a.pos0_host;
+    if (pos0 < 0) return;
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= a.kv_items) {
+        const int64_t i = (item - a.kv_items) * (64 / RP) + lane / RP;      // row (b, t, h) of q
+        if (i >= a.q_rows) return;
+        const int64_t bt = i / a.heads, b = bt / a.q_len;
+        const int h = (int)(i - bt * a.heads), t = (int)(bt - b * a.q_len), e0 = (lane & (RP - 1)) * V;
+        float v[V];
+        rotated_piece<T>(a, (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h, e0, angle_of(a, pos0 + t), v);
+        asm volatile("" ::: "memory");      // q_out may be q: every lane of the row has read before one writes
+        store_vec<T>((T*)a.q_out.p + b * a.q_out.b + t * a.q_out.t + h * a.q_out.h + e0, v);
+        return;
+    }
+    const int64_t bh = item / a.blocks;
+    const int nth = (int)(item - bh * a.blocks);
+    const int64_t b = bh / a.c.kv_heads;
+    const int h = (int)(bh - b * a.c.kv_heads);
+    const int64_t end = pos0 + (int64_t)a.q_len < a.c.n_max ? pos0 + (int64_t)a.q_len : a.c.n_max;
+    const T* ksrc = (const T*)a.k.p + b * a.k.b + h * a.k.h;
+    const T* vsrc = (const T*)a.v.p + b * a.v.b + h * a.v.h;
+    T* kt = (T*)a.c.k_tail + bh * BL * D;
+    T* vt = (T*)a.c.v_tail + bh * BL * D;
+    const int64_t n_blk = a.c.n_max / BL;
+    const int first = pos0 / BL, last = (int)(end / BL);      // `last` stays open
+    if (nth > 0 && first + nth >= last) return;
+    const int64_t row0 = (int64_t)(first + nth) * BL;
+    if (row0 >= end) return;
+    const int old = nth == 0 ? pos0 - (int)row0 : 0;          // rows of the block that stand in the tail
+    if (row0 + BL <= end) {
+        const int64_t blk = first + nth;
+        {
+            constexpr int NP = BL * RP / 64 > 0 ? BL * RP / 64 : 1;
+            float x[NP][V];
+            BlockMax top;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int idx = i * 64 + lane, t = idx / RP, e0 = (idx & (RP - 1)) * V;
+#pragma unroll
+                for (int e = 0; e < V; ++e) x[i][e] = 0.f;
+                if (t >= BL) continue;
+                if (t < old) load_vec<T>(kt + t * D + e0, x[i]);
+                else {
+                    const int64_t at = row0 + t - pos0;
+                    rotated_piece<T>(a, ksrc + at * a.k.t, e0, a.rot ? angle_of(a, pos0 + (int)at) : 0, x[i]);
+                }
+#pragma unroll
+                for (int e = 0; e < V; ++e) {
+                    x[i][e] = rounded<T>(x[i][e]);
+                    top.see(x[i][e]);
+                }
+            }
+            top.join();
+            const Quantiser q(top.amax);
+            const bool quick = q.direct && !top.odd;
+            if (lane == 0) a.c.k_scale[bh * n_blk + blk] = q.scale;
+            int8_t* out = a.c.k_codes + (bh * a.c.n_max + row0) * D;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int idx = i * 64 + lane;
+                if (idx >= BL * RP) continue;
+                uint32_t w[V / 4];
+#pragma unroll
+                for (int e = 0; e < V; e += 4)
+                    w[e / 4] = quick ? q.pack4(x[i][e], x[i][e + 1], x[i][e + 2], x[i][e + 3])
+                                     : q.pack4_exact(x[i][e], x[i][e + 1], x[i][e + 2], x[i][e + 3]);
+                if constexpr (V == 8) *(uint2*)(out + idx * V) = uint2{w[0], w[1]};
+                else *(uint32_t*)(out + idx * V) = w[0];
+            }
+        }
+        {
+            constexpr int UNITS = D / 2 * (BL / 16), NU = (UNITS + 63) / 64;      // (pair of columns, run of 16 rows)
+            float x[NU][2][16];
+            BlockMax top;
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const int idx = u * 64 + lane, d = (idx % (D / 2)) * 2, t0 = idx / (D / 2) * 16;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) x[u][0][e] = x[u][1][e] = 0.f;
+                if (idx >= UNITS) continue;
+                if (t0 < old) {
+#pragma unroll
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int e = 0; e < 16; e += V) {
+                            float v[V];
+                            load_vec<T>(vt + (d + c) * BL + t0 + e, v);
+#pragma unroll
+                            for (int k = 0; k < V; ++k) x[u][c][e + k] = v[k];
+                        }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    if (t0 + e >= old) {
+                        const T* p = vsrc + (row0 + t0 + e - pos0) * a.v.t + d;
+                        if constexpr (sizeof(T) == 2) {
+                            const uint32_t two = *(const uint32_t*)p;
+                            x[u][0][e] = __uint_as_float(two << 16);
+                            x[u][1][e] = __uint_as_float(two & 0xffff0000u);
+                        } else {
+                            const float2 two = *(const float2*)p;
+                            x[u][0][e] = two.x;
+                            x[u][1][e] = two.y;
+                        }
+                    }
+                    top.see(x[u][0][e]);
+                    top.see(x[u][1][e]);
+                }
+            }
+            top.join();
+            const Quantiser q(top.amax);
+            const bool quick = q.direct && !top.odd;
+            if (lane == 0) a.c.v_scale[bh * n_blk + blk] = q.scale;
+            int8_t* out = a.c.v_codes + (bh * n_blk + blk) * D * BL;
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const int idx = u * 64 + lane, d = (idx % (D / 2)) * 2, t0 = idx / (D / 2) * 16;
+                if (idx >= UNITS) continue;
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    const float* y = x[u][c];
+                    uint32_t w[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        w[e] = quick ? q.pack4(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3])
+                                     : q.pack4_exact(y[4 * e], y[4 * e + 1], y[4 * e + 2], y[4 * e + 3]);
+                    *(uint4*)(out + (d + c) * BL + t0) = uint4{w[0], w[1], w[2], w[3]};
+                }
+            }
+        }
+    }
+    // The open block's rows take the places that the first block's old rows leave, so the first wave writes them, after it has read those.
+    if (nth != 0) return;
+    const int64_t open0 = (int64_t)last * BL;
+    const int from = open0 > pos0 ? 0 : (int)(pos0 - open0), to = (int)(end - open0);
+    for (int idx = from * RP + lane; idx < to * RP; idx += 64) {
+        const int t = idx / RP, e0 = (idx & (RP - 1)) * V;
+        const int64_t at = open0 + t - pos0;
+        float v[V];
+        rotated_piece<T>(a, ksrc + at * a.k.t, e0, a.rot ? angle_of(a, pos0 + (int)at) : 0, v);
+        store_vec<T>(kt + t * D + e0, v);
+    }
+    for (int t = from; t < to; ++t)
+        for (int d = lane; d < D; d += 64) vt[d * BL + t] = vsrc[(open0 + t - pos0) * a.v.t + d];
+}
+
+// ---- bt_kv8_read -----------------------------------------------------------------------------------------------------------
+// One wave per (sequence, head, block): K by pieces of 16 codes, V by pairs of columns and runs of 16 rows, as append has them.
+template <typename T, int D, int BL>
+__global__ __launch_bounds__(256) void kv8_read_kernel(bt_kv8_cache c, int64_t n, int64_t first, int64_t count, int blocks,
                                                       T* __restrict__ ko, T* __restrict__ vo) {
-    const int D = c.head_dim, bl = c.block;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= c.batch * c.kv_heads * count * D) return;
-    const int d = (int)(i % D);
-    const int64_t bh = i / D / count, row = first + i / D - bh * count;
-    const int64_t blk = row >> shift, n_blk = c.n_max >> shift;
-    const int t = (int)(row & (bl - 1));
-    if (blk < n >> shift) {
-        if (ko) Elem<T>::store(ko + i, (float)c.k_codes[(bh * c.n_max + row) * D + d] * c.k_scale[bh * n_blk + blk]);
-        if (vo) Elem<T>::store(vo + i, (float)c.v_codes[((bh * n_blk + blk) * D + d) * bl + t] * c.v_scale[bh * n_blk + blk]);
-    } else {
-        if (ko) ko[i] = ((const T*)c.k_tail)[(bh * bl + t) * D + d];
-        if (vo) vo[i] = ((const T*)c.v_tail)[(bh * D + d) * bl + t];
+    constexpr int V = Elem<T>::VEC;
+    const int lane = threadIdx.x & 63;
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (item >= c.batch * c.kv_heads * blocks) return;
+    const int64_t bh = item / blocks, n_blk = c.n_max / BL, blk = first / BL + (item - bh * blocks);
+    const int64_t out0 = (bh * count + blk * BL - first) * D;      // where row 0 of the block would go
+    const int from = first > blk * BL ? (int)(first - blk * BL) : 0;
+    const int to = first + count < (blk + 1) * BL ? (int)(first + count - blk * BL) : BL;
+    const bool open = blk >= n / BL;
+    if (ko) {
+        const float s = open ? 0.f : c.k_scale[bh * n_blk + blk];
+        const int8_t* kc = c.k_codes + (bh * c.n_max + blk * BL) * D;
+        const T* kt = (const T*)c.k_tail + bh * BL * D;
+#pragma unroll
+        for (int i = 0; i < (BL * D / 16 + 63) / 64; ++i) {
+            const int idx = i * 64 + lane, t = idx / (D / 16), e0 = idx % (D / 16) * 16;
+            if (t < from || t >= to) continue;
+            T* o = ko + out0 + t * D + e0;
+            if (open) {
+#pragma unroll
+                for (int e = 0; e < 16; e += V) *(uint4*)(o + e) = *(const uint4*)(kt + t * D + e0 + e);
+            } else {
+                const int4 w = *(const int4*)(kc + t * D + e0);
+                const int words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                for (int e = 0; e < 16; e += V) {
+                    float v[V];
+#pragma unroll
+                    for (int k = 0; k < V; ++k) v[k] = (float)(int8_t)(words[(e + k) >> 2] >> (8 * (k & 3))) * s;
+                    store_vec<T>(o + e, v);
+                }
+            }
+        }
+    }
+    if (vo) {
+        const float s = open ? 0.f : c.v_scale[bh * n_blk + blk];
+        const int8_t* vc = c.v_codes + (bh * n_blk + blk) * D * BL;
+        const T* vt = (const T*)c.v_tail + bh * BL * D;
+        constexpr int UNITS = D / 2 * (BL / 16);
+#pragma unroll
+        for (int u = 0; u < (UNITS + 63) / 64; ++u) {
+            const int idx = u * 64 + lane, d = (idx % (D / 2)) * 2, t0 = idx / (D / 2) * 16;
+            if (idx >= UNITS) continue;
+            float x[2][16];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                if (open) {
+#pragma unroll
+                    for (int e = 0; e < 16; e += V) {
+                        float v[V];
+                        load_vec<T>(vt + (d + k) * BL + t0 + e, v);
+#pragma unroll
+                        for (int y = 0; y < V; ++y) x[k][e + y] = v[y];
+                    }
+                } else {
+                    const int4 w = *(const int4*)(vc + (d + k) * BL + t0);
+                    const int words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) x[k][e] = (float)(int8_t)(words[e >> 2] >> (8 * (e & 3))) * s;
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                if (t0 + e < from || t0 + e >= to) continue;
+                T* o = vo + out0 + (t0 + e) * D + d;
+                if constexpr (sizeof(T) == 2) *(uint32_t*)o = pack_bf16x2(x[0][e], x[1][e]);
+                else *(float2*)o = float2{x[0][e], x[1][e]};
+            }
+        }
     }
 }
 
@@ -673,6 +853,11 @@ static int check_rows(const char* who, const char* name, int dtype, const bt_kv8
     return BT_OK;
 }
 
+// BT_KV8(type, head_dim, block) for the cache's
+#define BT_KV8_BLOCK(T, D_, block) ((block) == 16 ? (void)(BT_KV8(T, D_, 16)) : (block) == 32 ? (void)(BT_KV8(T, D_, 32)) : (void)(BT_KV8(T, D_, 64)))
+#define BT_KV8_DIM(T, d, block) ((d) == 32 ? BT_KV8_BLOCK(T, 32, block) : (d) == 64 ? BT_KV8_BLOCK(T, 64, block) : BT_KV8_BLOCK(T, 128, block))
+#define BT_KV8_DISPATCH(dtype, d, block) ((dtype) == BT_BF16 ? BT_KV8_DIM(bf16, d, block) : BT_KV8_DIM(float, d, block))
+
 static Rows rows_of(const bt_kv8_rows* r) { return r ? Rows{(char*)r->p, r->b_stride, r->t_stride, r->h_stride} : Rows{nullptr, 0, 0, 0}; }
 
 }  // namespace bt
@@ -684,7 +869,8 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
                              int32_t pos0_host, const int32_t* pos_table, int32_t rot, const float* cos_tab, const float* sin_tab,
                              int64_t max_pos, bt_stream stream) {
     AppendArgs a{};
-    BT_TRY(check_cache("bt_kv8_append", dtype, cache, &a.shift));
+    int shift;
+    BT_TRY(check_cache("bt_kv8_append", dtype, cache, &shift));
     BT_CHECK_ARG(q_len > 0, "bt_kv8_append: bad q_len %d", q_len);
     if (cache->batch == 0) return BT_OK;
     BT_CHECK_ARG(rot >= 0 && rot % 2 == 0 && rot <= cache->head_dim, "bt_kv8_append: bad rotary_ndims %d", rot);
@@ -716,14 +902,17 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.cos_tab = cos_tab;
     a.sin_tab = sin_tab;
     a.max_pos = max_pos;
-    const int64_t grid = a.kv_items + (q ? cache->batch * q_len * heads : 0);
-    BT_CHECK_ARG(grid < (1ll << 31), "bt_kv8_append: grid too large");
+    const int V = dtype == BT_BF16 ? 8 : 4;
+    a.vec_rope = (rot / 2) % V == 0 && aligned16(cos_tab) && aligned16(sin_tab);
+    a.q_rows = q ? cache->batch * q_len * heads : 0;
+    const int64_t waves = a.kv_items + ceil_div(a.q_rows * cache->head_dim, 64 * V);
+    BT_CHECK_ARG(waves < (1ll << 31), "bt_kv8_append: grid too large");
+    const dim3 grid((unsigned)ceil_div(waves, 4));
     hipStream_t s = (hipStream_t)stream;
     ProfScope ps(BT_PROF_ROPE, s);
-    if (dtype == BT_BF16)
-        hipLaunchKernelGGL(kv8_append_kernel<bf16>, dim3((unsigned)grid), dim3(64), 0, s, a);
-    else
-        hipLaunchKernelGGL(kv8_append_kernel<float>, dim3((unsigned)grid), dim3(64), 0, s, a);
+#define BT_KV8(T, D_, BL_) kv8_append_kernel<T, D_, BL_><<<grid, dim3(256), 0, s>>>(a)
+    BT_KV8_DISPATCH(dtype, cache->head_dim, cache->block);
+#undef BT_KV8
     BT_LAUNCH_CHECK("bt_kv8_append launch");
     return BT_OK;
 }
@@ -735,16 +924,15 @@ extern "C" int bt_kv8_read(int dtype, const bt_kv8_cache* cache, int64_t n, int6
     BT_CHECK_ARG(n >= 0 && n <= cache->n_max && first >= 0 && count >= 0 && first + count <= n, "bt_kv8_read: rows out of range");
     BT_CHECK_ARG((!k_out || aligned16(k_out)) && (!v_out || aligned16(v_out)), "bt_kv8_read: outputs must be 16-byte aligned");
     if (cache->batch == 0 || count == 0 || (!k_out && !v_out)) return BT_OK;
-    const int64_t grid = ceil_div(cache->batch * cache->kv_heads * count * cache->head_dim, 256);
-    BT_CHECK_ARG(grid < (1ll << 31), "bt_kv8_read: grid too large");
+    const int blocks = (int)((first + count - 1) / cache->block - first / cache->block) + 1;
+    const int64_t waves = cache->batch * cache->kv_heads * blocks;
+    BT_CHECK_ARG(waves < (1ll << 31), "bt_kv8_read: grid too large");
+    const dim3 grid((unsigned)ceil_div(waves, 4));
     hipStream_t s = (hipStream_t)stream;
     ProfScope ps(BT_PROF_ROPE, s);
-    if (dtype == BT_BF16)
-        hipLaunchKernelGGL(kv8_read_kernel<bf16>, dim3((unsigned)grid), dim3(256), 0, s, *cache, shift, n, first, count, (bf16*)k_out,
-                           (bf16*)v_out);
-    else
-        hipLaunchKernelGGL(kv8_read_kernel<float>, dim3((unsigned)grid), dim3(256), 0, s, *cache, shift, n, first, count, (float*)k_out,
-                           (float*)v_out);
+#define BT_KV8(T, D_, BL_) kv8_read_kernel<T, D_, BL_><<<grid, dim3(256), 0, s>>>(*cache, n, first, count, blocks, (T*)k_out, (T*)v_out)
+    BT_KV8_DISPATCH(dtype, cache->head_dim, cache->block);
+#undef BT_KV8
     BT_LAUNCH_CHECK("bt_kv8_read launch");
     return BT_OK;
 }

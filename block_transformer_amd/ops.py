@@ -176,21 +176,28 @@ def rope_tables(max_pos: int, rot: int, base: float, device) -> torch.Tensor:
 
 
 # ---- 8-bit serving ----------------------------------------------------------------------------------------------------------------
-_ON_DEVICE = contextlib.nullcontext()
+_HERE = contextlib.nullcontext()
+# the current stream's handle and the current device without the Python objects around them: together 5 us of a call that takes 10
+_raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
-def _on(device, *tensors):
-    """A context in which `device` is the current one; every tensor (None: left out) has to live there."""
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise _lib.BtError(f"all tensors must be on {device}, got one on {t.device}")
-    if device.type != "cuda":
+def _on(index: int, *tensors):
+    """A context in which device `index` is the current one; every tensor (None: left out) has to live there."""
+    if index < 0:
         raise _lib.BtError("libbt_hip operates on GPU memory only; got a CPU tensor (move the model/inputs to 'cuda')")
-    return _ON_DEVICE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    for t in tensors:
+        if t is not None and t.get_device() != index:
+            raise _lib.BtError(f"all tensors must be on cuda:{index}, got one on {t.device}")
+    return _HERE if index == _device() else torch.cuda.device(index)
+
+
+def _at(t: Optional[torch.Tensor]):
+    """Device pointer of a tensor that `_on` has seen (None -> NULL)."""
+    return None if t is None else t.data_ptr()
 
 
 def _expect(t: torch.Tensor, what: str, shape, dtype) -> None:
-    if tuple(t.shape) != tuple(shape) or t.dtype != dtype or not t.is_contiguous():
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise _lib.BtError(f"{what} must be contiguous {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
 
 
@@ -208,11 +215,12 @@ def quantize_rows(x: torch.Tensor, ln_w: Optional[torch.Tensor] = None, ln_b: Op
         if w is not None:
             _expect(w, "LayerNorm weight", (K,), x.dtype)
     Kp = (K + 15) // 16 * 16
-    with _on(x.device, ln_w, ln_b):
+    code, index = dtype_code(x.dtype), x.get_device()
+    with _on(index, ln_w, ln_b):
         codes = torch.empty(x.shape[:-1] + (Kp,), dtype=torch.int8, device=x.device)
         scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        check(lib().bt_quant_rows(dtype_code(x.dtype), M, K, ptr(x2), ldx, ptr(ln_w), ptr(ln_b), float(eps), ptr(codes), Kp, ptr(scales),
-                                  current_stream()), "bt_quant_rows")
+        check(lib().bt_quant_rows(code, M, K, x2.data_ptr(), ldx, _at(ln_w), _at(ln_b), eps, codes.data_ptr(), Kp, scales.data_ptr(),
+                                  _raw_stream(index)), "bt_quant_rows")
     return codes, scales
 
 
@@ -258,7 +266,8 @@ def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight:
         if residual.shape != shape or residual.dtype != dtype:
             raise _lib.BtError(f"residual must be {dtype} {tuple(shape)}")
         r2, ldr = _rows(residual)
-    with _on(xc.device, xs, wc, ws, bias, residual, out, scratch):
+    index = xc.get_device()
+    with _on(index, xs, wc, ws, bias, residual, out, scratch):
         if out is None:
             out = torch.empty(shape, dtype=dtype, device=xc.device)
         elif out.shape != shape or out.dtype != dtype:
@@ -268,9 +277,10 @@ def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight:
             need = int(lib().bt_linear_q8_scratch_bytes(M, N, K))
             if need:
                 scratch = torch.empty(need, dtype=torch.uint8, device=xc.device)
-        check(lib().bt_linear_q8(code, M, N, K, ptr(a2), lda, ptr(xs), ptr(wc), wc.stride(0) if N > 1 else K, ptr(ws), ptr(bias), ptr(r2), ldr, ptr(o2), ldo,
-                                 _lib.BT_ACT_GELU if act == "gelu" else _lib.BT_ACT_NONE, ptr(scratch),
-                                 0 if scratch is None else scratch.numel() * scratch.element_size(), current_stream()), "bt_linear_q8")
+        check(lib().bt_linear_q8(code, M, N, K, a2.data_ptr(), lda, xs.data_ptr(), wc.data_ptr(), wc.stride(0) if N > 1 else K,
+                                 ws.data_ptr(), _at(bias), _at(r2), ldr, o2.data_ptr(), ldo,
+                                 _lib.BT_ACT_GELU if act == "gelu" else _lib.BT_ACT_NONE, _at(scratch),
+                                 0 if scratch is None else scratch.numel() * scratch.element_size(), _raw_stream(index)), "bt_linear_q8")
     return out
 
 
@@ -288,22 +298,26 @@ def _kv8(kv: Sequence[torch.Tensor]):
                                   (kt, "k_tail", (B, H, block, d), kt.dtype), (vt, "v_tail", (B, H, d, block), kt.dtype)):
         if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
             _expect(t, what, shape, dtype)
-    return _lib.bt_kv8_cache(block, H, d, B, n_max, ptr(kc), ptr(vc), ptr(ks), ptr(vs), ptr(kt), ptr(vt)), dtype_code(kt.dtype)
+    return (_lib.bt_kv8_cache(block, H, d, B, n_max, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt.data_ptr(),
+                              vt.data_ptr()), dtype_code(kt.dtype))
 
 
 def _kv8_rows(t: torch.Tensor, what: str, batch: int, q_len: int, d: int, dtype):
-    if t.dim() != 4 or t.shape[0] != batch or t.shape[1] != q_len or t.shape[3] != d or t.dtype != dtype:
-        raise _lib.BtError(f"{what} must be {dtype} [{batch}, {q_len}, heads, {d}], got {t.dtype} {tuple(t.shape)}")
-    if t.stride(3) != 1:
+    shape = t.shape
+    if len(shape) != 4 or shape[0] != batch or shape[1] != q_len or shape[3] != d or t.dtype != dtype:
+        raise _lib.BtError(f"{what} must be {dtype} [{batch}, {q_len}, heads, {d}], got {t.dtype} {tuple(shape)}")
+    sb, st, sh, one = t.stride()
+    if one != 1:
         raise _lib.BtError(f"{what} must have unit inner stride")
-    return _lib.bt_kv8_rows(ptr(t), *(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)))     # the stride of one row says nothing
+    # (the stride of a single row says nothing)
+    return _lib.bt_kv8_rows(t.data_ptr(), sb if batch > 1 else 0, st if q_len > 1 else 0, sh if shape[2] > 1 else 0)
 
 
 def _pos0(pos0):
     if isinstance(pos0, torch.Tensor):
         if pos0.dtype != torch.int32 or pos0.numel() != 1:
             raise _lib.BtError("a device-side pos0 is one int32")
-        return ptr(pos0), 0
+        return pos0.data_ptr(), 0
     return None, int(pos0)
 
 
@@ -327,12 +341,14 @@ def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.T
     if q is not None:
         qr, heads = _kv8_rows(q, "q", B, q_len, d, dtype), q.shape[2]
     pos_dev, pos_host = _pos0(pos0)
-    with _on(k.device, *kv, q, v, rope, pos_table, q_out, pos0 if pos_dev else None):
+    index = k.get_device()
+    with _on(index, *kv, q, v, rope, pos_table, q_out, pos0 if pos_dev else None):
         if rope is not None:
             if rope.dim() != 3 or rope.shape[0] != 2 or rope.dtype != torch.float32 or not rope.is_contiguous():
                 raise _lib.BtError("rope must be contiguous float32 [2, max_pos, rot / 2] (rope_tables)")
             max_pos, rot = rope.shape[1], 2 * rope.shape[2]
-            cos, sin = ptr(rope), ptr(rope) + rope.stride(0) * 4
+            cos = rope.data_ptr()
+            sin = cos + rope.stride(0) * 4
             if q is not None:
                 if q_out is None:
                     q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
@@ -345,7 +361,7 @@ def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.T
                                       pos_table.numel() < (cache.n_max if pos_dev else pos_host + q_len)):
             raise _lib.BtError("pos_table must be contiguous int32 and hold an entry for every row")
         check(lib().bt_kv8_append(code, ctypes.byref(cache), q_len, heads if rot else 0, qr if rot else None, qor, kr, vr, pos_dev, pos_host,
-                                  ptr(pos_table), rot, cos, sin, max_pos, current_stream()), "bt_kv8_append")
+                                  _at(pos_table), rot, cos, sin, max_pos, _raw_stream(index)), "bt_kv8_append")
     return q_out if rot else q
 
 
@@ -356,10 +372,11 @@ def kv8_read(kv: Sequence[torch.Tensor], n: int, first: int = 0, count: Optional
     count = n - first if count is None else count
     if not 0 <= first <= first + count <= n <= cache.n_max:
         raise _lib.BtError(f"rows [{first}, {first + count}) of {n} in a cache of {cache.n_max}")
-    with _on(kv[0].device, *kv):
+    index = kv[0].get_device()
+    with _on(index, *kv):
         k = torch.empty(cache.batch, cache.kv_heads, count, cache.head_dim, dtype=kv[4].dtype, device=kv[0].device)
         v = torch.empty_like(k)
-        check(lib().bt_kv8_read(code, ctypes.byref(cache), n, first, count, ptr(k), ptr(v), current_stream()), "bt_kv8_read")
+        check(lib().bt_kv8_read(code, ctypes.byref(cache), n, first, count, k.data_ptr(), v.data_ptr(), _raw_stream(index)), "bt_kv8_read")
     return k, v
 
 
@@ -383,7 +400,8 @@ def attention_kv8(q: torch.Tensor, kv: Sequence[torch.Tensor], pos0, mask: Optio
         mask_ld = mask.stride(0) if B > 1 else mask.shape[1]
         if mask.shape[1] < (cache.n_max if pos_dev else pos_host + q_len):
             raise _lib.BtError("mask row too short")
-    with _on(q.device, *kv, mask, out, ws, pos0 if pos_dev else None):
+    index = q.get_device()
+    with _on(index, *kv, mask, out, ws, pos0 if pos_dev else None):
         if out is None:
             out = torch.empty(B, q_len, heads, d, dtype=dtype, device=q.device)
         elif out.shape != (B, q_len, heads, d) or out.dtype != dtype or not out.is_contiguous():
@@ -393,7 +411,7 @@ def attention_kv8(q: torch.Tensor, kv: Sequence[torch.Tensor], pos0, mask: Optio
         if ws is None and n_split > 1:
             need = int(lib().bt_attention_kv8_workspace_bytes(B, q_len, heads, d, n_split))
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
-        check(lib().bt_attention_kv8(code, ctypes.byref(cache), q_len, heads, qr, pos_dev, pos_host, ptr(mask), mask_ld, ptr(out),
-                                     heads * d, n_split, ptr(ws), 0 if ws is None else ws.numel() * ws.element_size(), current_stream()),
+        check(lib().bt_attention_kv8(code, ctypes.byref(cache), q_len, heads, qr, pos_dev, pos_host, _at(mask), mask_ld, out.data_ptr(),
+                                     heads * d, n_split, _at(ws), 0 if ws is None else ws.numel() * ws.element_size(), _raw_stream(index)),
               "bt_attention_kv8")
     return out
