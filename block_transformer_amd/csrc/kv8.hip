@@ -3,6 +3,8 @@
 #include "bt_common.h"
 #include "bt_quant.h"
 
+#include <type_traits>
+
 namespace bt {
 
 struct Rows {      // bt_kv8_rows on the device
@@ -14,8 +16,8 @@ struct Rows {      // bt_kv8_rows on the device
 struct AppendArgs {
     bt_kv8_cache c;
     Rows q, q_out, k, v;
-    int64_t kv_items;      // waves for keys and values: batch * kv_heads * blocks
-    int64_t q_rows;        // batch * q_len * heads
+    uint32_t kv_items;     // waves for keys and values: batch * kv_heads * blocks
+    uint32_t q_rows;       // batch * q_len * heads
     int blocks;            // blocks that q_len rows can touch
     int q_len, heads, rot, pos0_host;
     bool vec_rope;
@@ -69,118 +71,175 @@ __device__ inline void rotated_piece(const AppendArgs& a, const T* row, int e0, 
     }
 }
 
+// v as `T` holds it
 template <typename T>
-__device__ inline float rounded(float v) {
-    if constexpr (sizeof(T) == 2) return bf16_to_f32(f32_to_bf16(v));
-    return v;
+__device__ inline void round_piece(float (&v)[Elem<T>::VEC]) {
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) {
+            const uint32_t two = pack_bf16x2(v[i], v[i + 1]);
+            v[i] = __uint_as_float(two << 16);
+            v[i + 1] = __uint_as_float(two & 0xffff0000u);
+        }
+    }
 }
 
-// the scale of a block: the largest finite magnitude; `odd`: not everything was finite
+// The scale of a block: the largest finite magnitude.  Two instructions a value; `odd` (a NaN or infinity: 0 * v is not 0) is rare, and
+// then the largest is looked for again without those.
 struct BlockMax {
-    float amax = 0.f;
-    bool odd = false;
+    float amax = 0.f, zero = 0.f;
     __device__ inline void see(float v) {
-        const float x = fabsf(v);
-        const bool fine = x < INFINITY;
-        odd |= !fine;
-        amax = fmaxf(amax, fine ? x : 0.f);
+        amax = fmaxf(amax, fabsf(v));
+        zero = fmaf(v, 0.f, zero);
     }
-    __device__ inline void join() {
-        amax = wave_max(amax);
-        odd = __any(odd);
+    __device__ inline bool odd() const { return __any(zero != 0.f); }      // (NaN != 0)
+    template <int N>
+    __device__ static inline float finite(const float (&v)[N]) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.f);
+        return wave_max(m);
     }
 };
 
 // One wave per (sequence, head, block) that the new rows touch; the waves behind them rotate q.
-//   K: a lane has 16-byte pieces of rows, as memory has them.
+//   K, q: a lane has 16-byte pieces of rows, four to a row, a quarter row apart: the rotary dims are then the same piece of every lane, and
+//         the fp64 work of the others is skipped.
 //   V: a lane has columns 2 x, 2 x + 1 of 16 rows, that is two 16-byte runs of v_codes: rows are read 256 bytes a wave and instruction,
 //      and no transpose is needed.  Rows of the open block come in runs from v_tail, which is transposed already.
-// Bound by memory; K and V are each held in registers between the search for the scale and the codes.
+// Bound by memory; K and V are held in registers between the search for the scale and the codes, V's loads go out before K's work.
 template <typename T, int D, int BL>
 __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
-    constexpr int V = Elem<T>::VEC, RP = D / V;      // pieces of a row
+    constexpr int V = Elem<T>::VEC, RP = D / V, LR = RP / 4;      // pieces of a row, lanes to a row
     const int lane = threadIdx.x & 63;
     const int pos0 = a.pos0_dev ? *a.pos0_dev : a.pos0_host;
     if (pos0 < 0) return;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int e_lane = lane % LR * V;      // piece k of this lane: dims e_lane + k D / 4
     if (item >= a.kv_items) {
-        const int64_t i = (item - a.kv_items) * (64 / RP) + lane / RP;      // row (b, t, h) of q
+        const uint32_t i = (item - a.kv_items) * (64 / LR) + lane / LR;      // row (b, t, h) of q
         if (i >= a.q_rows) return;
-        const int64_t bt = i / a.heads, b = bt / a.q_len;
-        const int h = (int)(i - bt * a.heads), t = (int)(bt - b * a.q_len), e0 = (lane & (RP - 1)) * V;
-        float v[V];
-        rotated_piece<T>(a, (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h, e0, angle_of(a, pos0 + t), v);
+        const uint32_t bt = i / (uint32_t)a.heads, b = bt / (uint32_t)a.q_len;
+        const int h = (int)(i - bt * a.heads), t = (int)(bt - b * a.q_len);
+        const T* src = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
+        T* dst = (T*)a.q_out.p + b * a.q_out.b + t * a.q_out.t + h * a.q_out.h;
+        const int64_t ang = angle_of(a, pos0 + t);
+        float v[4][V];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) rotated_piece<T>(a, src, e_lane + k * (D / 4), ang, v[k]);
         asm volatile("" ::: "memory");      // q_out may be q: every lane of the row has read before one writes
-        store_vec<T>((T*)a.q_out.p + b * a.q_out.b + t * a.q_out.t + h * a.q_out.h + e0, v);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) store_vec<T>(dst + e_lane + k * (D / 4), v[k]);
         return;
     }
-    const int64_t bh = item / a.blocks;
+    const uint32_t bh = item / (uint32_t)a.blocks;
     const int nth = (int)(item - bh * a.blocks);
-    const int64_t b = bh / a.c.kv_heads;
+    const uint32_t b = bh / (uint32_t)a.c.kv_heads;
     const int h = (int)(bh - b * a.c.kv_heads);
     const int64_t end = pos0 + (int64_t)a.q_len < a.c.n_max ? pos0 + (int64_t)a.q_len : a.c.n_max;
     const T* ksrc = (const T*)a.k.p + b * a.k.b + h * a.k.h;
     const T* vsrc = (const T*)a.v.p + b * a.v.b + h * a.v.h;
-    T* kt = (T*)a.c.k_tail + bh * BL * D;
-    T* vt = (T*)a.c.v_tail + bh * BL * D;
+    T* kt = (T*)a.c.k_tail + (int64_t)bh * BL * D;
+    T* vt = (T*)a.c.v_tail + (int64_t)bh * BL * D;
     const int64_t n_blk = a.c.n_max / BL;
     const int first = pos0 / BL, last = (int)(end / BL);      // `last` stays open
     if (nth > 0 && first + nth >= last) return;
-    const int64_t row0 = (int64_t)(first + nth) * BL;
+    const int64_t blk = first + nth, row0 = blk * BL;
     if (row0 >= end) return;
     const int old = nth == 0 ? pos0 - (int)row0 : 0;          // rows of the block that stand in the tail
     if (row0 + BL <= end) {
-        const int64_t blk = first + nth;
-        {
-            constexpr int NP = BL * RP / 64 > 0 ? BL * RP / 64 : 1;
-            float x[NP][V];
-            BlockMax top;
+        constexpr int UNITS = D / 2 * (BL / 16), NU = (UNITS + 63) / 64;      // V: (pair of columns, run of 16 rows)
+        typedef typename std::conditional<sizeof(T) == 2, uint32_t, float2>::type Pair;
+        Pair raw[NU][16];
 #pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int idx = i * 64 + lane, t = idx / RP, e0 = (idx & (RP - 1)) * V;
+        for (int u = 0; u < NU; ++u) {
+            const int idx = u * 64 + lane, d = (idx % (D / 2)) * 2, t0 = idx / (D / 2) * 16;
+            const T* p = vsrc + (row0 - pos0 + t0) * a.v.t + d;
 #pragma unroll
-                for (int e = 0; e < V; ++e) x[i][e] = 0.f;
-                if (t >= BL) continue;
-                if (t < old) load_vec<T>(kt + t * D + e0, x[i]);
-                else {
-                    const int64_t at = row0 + t - pos0;
-                    rotated_piece<T>(a, ksrc + at * a.k.t, e0, a.rot ? angle_of(a, pos0 + (int)at) : 0, x[i]);
-                }
-#pragma unroll
-                for (int e = 0; e < V; ++e) {
-                    x[i][e] = rounded<T>(x[i][e]);
-                    top.see(x[i][e]);
-                }
-            }
-            top.join();
-            const Quantiser q(top.amax);
-            const bool quick = q.direct && !top.odd;
-            if (lane == 0) a.c.k_scale[bh * n_blk + blk] = q.scale;
-            int8_t* out = a.c.k_codes + (bh * a.c.n_max + row0) * D;
-#pragma unroll
-            for (int i = 0; i < NP; ++i) {
-                const int idx = i * 64 + lane;
-                if (idx >= BL * RP) continue;
-                uint32_t w[V / 4];
-#pragma unroll
-                for (int e = 0; e < V; e += 4)
-                    w[e / 4] = quick ? q.pack4(x[i][e], x[i][e + 1], x[i][e + 2], x[i][e + 3])
-                                     : q.pack4_exact(x[i][e], x[i][e + 1], x[i][e + 2], x[i][e + 3]);
-                if constexpr (V == 8) *(uint2*)(out + idx * V) = uint2{w[0], w[1]};
-                else *(uint32_t*)(out + idx * V) = w[0];
+            for (int e = 0; e < 16; ++e) {
+                raw[u][e] = Pair{};
+                if (idx < UNITS && t0 + e >= old) raw[u][e] = *(const Pair*)(p + e * a.v.t);
             }
         }
         {
-            constexpr int UNITS = D / 2 * (BL / 16), NU = (UNITS + 63) / 64;      // (pair of columns, run of 16 rows)
+            constexpr int NR = BL * LR / 64 > 0 ? BL * LR / 64 : 1;      // rows of a lane
+            float x[NR][4][V];
+            BlockMax top;
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const int t = (i * 64 + lane) / LR;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int e0 = e_lane + k * (D / 4);
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[i][k][e] = 0.f;
+                    if (t >= BL) continue;
+                    if (t < old) load_vec<T>(kt + t * D + e0, x[i][k]);
+                    else load_vec<T>(ksrc + (row0 + t - pos0) * a.k.t + e0, x[i][k]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const int t = (i * 64 + lane) / LR;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int e0 = e_lane + k * (D / 4);
+                    if (t < BL && t >= old && e0 < a.rot) {
+                        const int at = (int)(row0 + t - pos0);
+                        rotated_piece<T>(a, ksrc + at * a.k.t, e0, angle_of(a, pos0 + at), x[i][k]);
+                        round_piece<T>(x[i][k]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < V; ++e) top.see(x[i][k][e]);
+                }
+            }
+            const bool odd = top.odd();
+            float amax = wave_max(top.amax);
+            if (odd) {
+                amax = 0.f;
+#pragma unroll
+                for (int i = 0; i < NR; ++i)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) amax = fmaxf(amax, BlockMax::finite(x[i][k]));
+            }
+            const Quantiser q(amax);
+            const bool quick = q.direct && !odd;
+            if (lane == 0) a.c.k_scale[bh * n_blk + blk] = q.scale;
+            int8_t* out = a.c.k_codes + (bh * a.c.n_max + row0) * D;
+#pragma unroll
+            for (int i = 0; i < NR; ++i) {
+                const int t = (i * 64 + lane) / LR;
+                if (t >= BL) continue;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float* y = x[i][k];
+                    uint32_t w[V / 4];
+#pragma unroll
+                    for (int e = 0; e < V; e += 4)
+                        w[e / 4] = quick ? q.pack4(y[e], y[e + 1], y[e + 2], y[e + 3]) : q.pack4_exact(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                    int8_t* o = out + t * D + e_lane + k * (D / 4);
+                    if constexpr (V == 8) *(uint2*)o = uint2{w[0], w[1]};
+                    else *(uint32_t*)o = w[0];
+                }
+            }
+        }
+        {
             float x[NU][2][16];
             BlockMax top;
 #pragma unroll
             for (int u = 0; u < NU; ++u) {
                 const int idx = u * 64 + lane, d = (idx % (D / 2)) * 2, t0 = idx / (D / 2) * 16;
 #pragma unroll
-                for (int e = 0; e < 16; ++e) x[u][0][e] = x[u][1][e] = 0.f;
-                if (idx >= UNITS) continue;
-                if (t0 < old) {
+                for (int e = 0; e < 16; ++e) {
+                    if constexpr (sizeof(T) == 2) {
+                        x[u][0][e] = __uint_as_float(raw[u][e] << 16);
+                        x[u][1][e] = __uint_as_float(raw[u][e] & 0xffff0000u);
+                    } else {
+                        x[u][0][e] = raw[u][e].x;
+                        x[u][1][e] = raw[u][e].y;
+                    }
+                }
+                if (idx < UNITS && t0 < old) {
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -188,30 +247,24 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
                             float v[V];
                             load_vec<T>(vt + (d + c) * BL + t0 + e, v);
 #pragma unroll
-                            for (int k = 0; k < V; ++k) x[u][c][e + k] = v[k];
+                            for (int k = 0; k < V; ++k) x[u][c][e + k] = t0 + e + k < old ? v[k] : x[u][c][e + k];
                         }
                 }
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
-                    if (t0 + e >= old) {
-                        const T* p = vsrc + (row0 + t0 + e - pos0) * a.v.t + d;
-                        if constexpr (sizeof(T) == 2) {
-                            const uint32_t two = *(const uint32_t*)p;
-                            x[u][0][e] = __uint_as_float(two << 16);
-                            x[u][1][e] = __uint_as_float(two & 0xffff0000u);
-                        } else {
-                            const float2 two = *(const float2*)p;
-                            x[u][0][e] = two.x;
-                            x[u][1][e] = two.y;
-                        }
-                    }
                     top.see(x[u][0][e]);
                     top.see(x[u][1][e]);
                 }
             }
-            top.join();
-            const Quantiser q(top.amax);
-            const bool quick = q.direct && !top.odd;
+            const bool odd = top.odd();
+            float amax = wave_max(top.amax);
+            if (odd) {
+                amax = 0.f;
+#pragma unroll
+                for (int u = 0; u < NU; ++u) amax = fmaxf(amax, fmaxf(BlockMax::finite(x[u][0]), BlockMax::finite(x[u][1])));
+            }
+            const Quantiser q(amax);
+            const bool quick = q.direct && !odd;
             if (lane == 0) a.c.v_scale[bh * n_blk + blk] = q.scale;
             int8_t* out = a.c.v_codes + (bh * n_blk + blk) * D * BL;
 #pragma unroll
@@ -237,9 +290,9 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
     const int from = open0 > pos0 ? 0 : (int)(pos0 - open0), to = (int)(end - open0);
     for (int idx = from * RP + lane; idx < to * RP; idx += 64) {
         const int t = idx / RP, e0 = (idx & (RP - 1)) * V;
-        const int64_t at = open0 + t - pos0;
+        const int at = (int)(open0 + t - pos0);
         float v[V];
-        rotated_piece<T>(a, ksrc + at * a.k.t, e0, a.rot ? angle_of(a, pos0 + (int)at) : 0, v);
+        rotated_piece<T>(a, ksrc + at * a.k.t, e0, a.rot ? angle_of(a, pos0 + at) : 0, v);
         store_vec<T>(kt + t * D + e0, v);
     }
     for (int t = from; t < to; ++t)
@@ -892,7 +945,10 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.v = rows_of(v);
     a.blocks = pos0_dev ? (q_len + cache->block - 2) / cache->block + 1
                         : (int)(((int64_t)pos0_host + q_len - 1) / cache->block - pos0_host / cache->block) + 1;
-    a.kv_items = cache->batch * cache->kv_heads * a.blocks;
+    const int64_t kv_items = cache->batch * cache->kv_heads * a.blocks, q_rows = q ? cache->batch * q_len * heads : 0;
+    BT_CHECK_ARG(kv_items < (1ll << 30) && q_rows < (1ll << 30), "bt_kv8_append: too many rows for one call");
+    a.kv_items = (uint32_t)kv_items;
+    a.q_rows = (uint32_t)q_rows;
     a.q_len = q_len;
     a.heads = heads;
     a.rot = rot;
@@ -904,9 +960,7 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.max_pos = max_pos;
     const int V = dtype == BT_BF16 ? 8 : 4;
     a.vec_rope = (rot / 2) % V == 0 && aligned16(cos_tab) && aligned16(sin_tab);
-    a.q_rows = q ? cache->batch * q_len * heads : 0;
-    const int64_t waves = a.kv_items + ceil_div(a.q_rows * cache->head_dim, 64 * V);
-    BT_CHECK_ARG(waves < (1ll << 31), "bt_kv8_append: grid too large");
+    const int64_t waves = kv_items + ceil_div(q_rows * cache->head_dim, 256 * V);
     const dim3 grid((unsigned)ceil_div(waves, 4));
     hipStream_t s = (hipStream_t)stream;
     ProfScope ps(BT_PROF_ROPE, s);
