@@ -24,7 +24,7 @@ BUILD = os.path.join(CSRC, "_build")
 LIB = os.path.join(HERE, "libbt_hip.so")
 LIB_DBG = os.path.join(HERE, "libbt_hip_dbg.so")
 SOURCES = ["core.hip", "gemm.hip", "norm.hip", "misc.hip", "attention.hip", "engine.hip", "quant.hip", "kv8.hip"]
-HEADERS = [os.path.join(CSRC, "bt_common.h"), os.path.join(CSRC, "bt_quant.h"), os.path.join(os.path.dirname(HERE), "include", "bt_hip.h")]
+HEADERS = [os.path.join(CSRC, "bt_common.h"), os.path.join(CSRC, "bt_quant.h"), os.path.join(CSRC, "bt_gelu.h"), os.path.join(os.path.dirname(HERE), "include", "bt_hip.h")]
 EXPORTS = os.path.join(CSRC, "exports.map")   # linker version script: bt_* global, everything else local
 # packed fp32 arithmetic stays off: some forms of v_pk_{add,mul,fma}_f32 have given wrong results now and then (the host pass does not
 # know the feature and says so; that is harmless)

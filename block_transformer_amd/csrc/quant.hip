@@ -1,6 +1,9 @@
 // 8-bit integers for the linear layers: bt_quant_rows (one scale per row) and bt_linear_q8 (the product, with its epilogue).
 #include "bt_common.h"
+#include "bt_gelu.h"
 #include "bt_quant.h"
+
+#include <type_traits>
 
 namespace bt {
 
@@ -215,17 +218,27 @@ struct Q8Args {
     int* slab;          // [slices][M][N]
 };
 
-// act(acc * sx * sw + bias): fp32; the residual joins where the row is written
-__device__ inline float q8_value(int acc, float sa, float sw, float bias, int act) {
-    const float y = fmaf((float)acc, sa * sw, bias);
-    return act == BT_ACT_GELU ? 0.5f * y * (1.0f + erff(y * 0.70710678118654752440f)) : y;
+// act(acc * sx * sw + bias): fp32; the residual joins where the row is written.  GELU: erf for fp32, the polynomial of the other bf16
+// epilogues (8.5e-6 relative) where the result is rounded to 8 bits.
+template <typename T>
+__device__ inline void q8_values(const i32x4& acc, float sa, const float (&sw)[4], const float (&bias)[4], int act, float (&y)[4]) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) y[r] = fmaf((float)acc[r], sa * sw[r], bias[r]);
+    if (act == BT_ACT_GELU) {
+        if constexpr (sizeof(T) == 2) gelu4(y);
+        else
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] = 0.5f * y[r] * (1.0f + erff(y[r] * 0.70710678118654752440f));
+    }
 }
 
 template <typename T>
 __device__ inline void q8_store(const Q8Args& e, int m, int n, int acc) {
-    float y = q8_value(acc, e.a_scale[m], e.w_scale[n], e.bias ? Elem<T>::load((const T*)e.bias + n) : 0.f, e.act);
-    if (e.residual) y += Elem<T>::load((const T*)e.residual + (int64_t)m * e.ldr + n);
-    Elem<T>::store((T*)e.out + (int64_t)m * e.ldo + n, y);
+    const float bias[4] = {e.bias ? Elem<T>::load((const T*)e.bias + n) : 0.f}, sw[4] = {e.w_scale[n]};
+    float y[4];
+    q8_values<T>(i32x4{acc, 0, 0, 0}, e.a_scale[m], sw, bias, e.act, y);
+    if (e.residual) y[0] += Elem<T>::load((const T*)e.residual + (int64_t)m * e.ldr + n);
+    Elem<T>::store((T*)e.out + (int64_t)m * e.ldo + n, y[0]);
 }
 
 // Any K % 16 == 0: 64 x 64 tile per workgroup, 64 bytes of K at a time through LDS, four products per v_dot4.
@@ -281,6 +294,100 @@ __device__ inline void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
+// The tile of this workgroup.  Workgroups of one XCD (ids that are equal mod 8) take neighbouring tiles, in columns of HIGH tile rows: its
+// L2 serves them with each other's panels.
+template <int HIGH>
+__device__ inline void q8_tile(const Q8Args& e, int& tm, int& tn) {
+    const int tiles = e.tiles_m * e.tiles_n, id = blockIdx.x;
+    const int per = tiles >> 3, rest = tiles & 7, xcd = id & 7, local = id >> 3;
+    const int at = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + local;
+    const int group = at / (HIGH * e.tiles_n), first = group * HIGH, high = min(e.tiles_m - first, HIGH), in = at - group * HIGH * e.tiles_n;
+    tm = first + in % high;
+    tn = in / high;
+}
+
+constexpr int q8_pitch(int nb, int size) { return 16 * nb * size + 16; }      // bytes of a row of a wave's patch: its 16 NB columns
+
+// The sums of a wave, NI fragments of 16 rows (row0(i) is the first of fragment i) by 16 NB columns from n_w: lane (c, g) has columns
+// 16 j + 4 g .. + 3 of row c.  Scales, bias, activation and residual there, then one rounding; the rows are put together in `patch` (16
+// rows, the wave's own) and leave as 16-byte pieces.
+template <typename T, int NI, int NB, typename Row0>
+__device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], char* patch, int n_w, Row0 row0) {
+    constexpr int PITCH = q8_pitch(NB, sizeof(T));
+    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+    // every load of scales and bias at once, and the residual's one fragment ahead: a load that is waited for costs a microsecond here
+    float sa[NI], sw[NB][4], bias[NB][4];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) sa[i] = e.a_scale[min(row0(i) + c, e.M - 1)];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) {
+        const int n = n_w + j * 16 + g * 4;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            sw[j][r] = e.w_scale[min(n + r, e.N - 1)];
+            bias[j][r] = e.bias ? Elem<T>::load((const T*)e.bias + min(n + r, e.N - 1)) : 0.f;
+        }
+    }
+    typedef typename std::conditional<sizeof(T) == 2, uint2, float4>::type Four;
+    Four next[NB] = {};
+    auto load_residual = [&](int i) {
+        const int m = row0(i) + c;
+        if (!e.residual || m >= e.M) return;
+        const T* p = (const T*)e.residual + (int64_t)m * e.ldr + n_w + g * 4;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            const int n = n_w + j * 16 + g * 4;
+            if (e.wide && n + 4 <= e.N) next[j] = *(const Four*)(p + j * 16);
+            else {
+                T v[4] = {};
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (n + r < e.N) v[r] = p[j * 16 + r];
+                __builtin_memcpy(&next[j], v, sizeof v);
+            }
+        }
+    };
+    load_residual(0);
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+        Four res[NB];
+#pragma unroll
+        for (int j = 0; j < NB; ++j) res[j] = next[j];
+        if (i + 1 < NI) load_residual(i + 1);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) {
+            float y[4];
+            q8_values<T>(acc[i][j], sa[i], sw[j], bias[j], e.act, y);
+            if (e.residual) {
+                if constexpr (sizeof(T) == 2) {
+                    y[0] += __uint_as_float(res[j].x << 16), y[1] += __uint_as_float(res[j].x & 0xffff0000u);
+                    y[2] += __uint_as_float(res[j].y << 16), y[3] += __uint_as_float(res[j].y & 0xffff0000u);
+                } else {
+                    y[0] += res[j].x, y[1] += res[j].y, y[2] += res[j].z, y[3] += res[j].w;
+                }
+            }
+            if constexpr (sizeof(T) == 2) *(uint2*)(patch + c * PITCH + (j * 16 + g * 4) * 2) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+            else *(float4*)(patch + c * PITCH + (j * 16 + g * 4) * 4) = float4{y[0], y[1], y[2], y[3]};
+        }
+        asm volatile("" ::: "memory");      // the patch is the wave's own, and a wave's LDS accesses stay in order
+        constexpr int V = Elem<T>::VEC, CH = 16 * NB / V;      // 16-byte pieces of a row
+#pragma unroll
+        for (int x = 0; x < 16 * CH; x += 64) {
+            const int r = (x + lane) / CH, d = ((x + lane) - r * CH) * V, mm = row0(i) + r, n = n_w + d;
+            if (mm >= e.M || n >= e.N) continue;
+            float y[V];
+            load_vec<T>((const T*)(patch + r * PITCH) + d, y);
+            T* out = (T*)e.out + (int64_t)mm * e.ldo + n;
+            if (e.wide && n + V <= e.N) store_vec<T>(out, y);
+            else
+#pragma unroll
+                for (int q = 0; q < V; ++q)
+                    if (n + q < e.N) Elem<T>::store(out + q, y[q]);
+        }
+        asm volatile("" ::: "memory");
+    }
+}
+
 // The tile kernel: 32 MI x 32 NB per workgroup of 2 x 2 waves, 64 bytes of K a step, K % 64 == 0.
 //  * Two workgroups to a CU: while one waits at its barrier or writes its tile, the other's waves have the matrix units.  So a K step
 //    needs one barrier and the epilogue no software overlap.
@@ -289,25 +396,21 @@ __device__ inline void wait_loads() {
 //    step t - 1, whose stage takes the loads of step t + NS - 1.
 //  * LDS rows are 64 bytes; the four 16-byte pieces of row r are stored in the order p ^ ((r >> 1) & 3) ^ ((r >> 3) & 1): the 16 rows that
 //    a fragment read touches at once are spread over all banks.
-//  * mfma(W, A): a lane gets four neighbouring columns of one row; rows are put together in LDS and leave as 16-byte pieces.
+//  * mfma(W, A): a lane gets four neighbouring columns of one row (q8_write).
 template <typename T, int MI, int NB, int NS>
 __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
     constexpr int BM = 32 * MI, BN = 32 * NB, STAGE = (BM + BN) * 64;
     constexpr int LA = BM / 64, LW = BN / 64, LOADS = LA + LW;      // 1 KiB loads of a wave and step
-    constexpr int PITCH = 16 * NB * sizeof(T) + 16;                 // a row of the wave's patch: its 16 NB columns
+    constexpr int PITCH = q8_pitch(NB, sizeof(T));
     constexpr int RING = NS * STAGE, PATCH = 4 * 16 * PITCH;
     __shared__ __attribute__((aligned(16))) char smem[RING > PATCH ? RING : PATCH];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1, c = lane & 15, g = lane >> 4;
 
-    // workgroups of one XCD (ids that are equal mod 8) take neighbouring tiles, in columns of 8 tile rows: its L2 serves them with each
-    // other's panels
-    const int tiles = e.tiles_m * e.tiles_n, id = blockIdx.x;
-    const int per = tiles >> 3, rest = tiles & 7, xcd = id & 7, local = id >> 3;
-    const int at = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + local;
-    const int group = at / (8 * e.tiles_n), first = group * 8, high = min(e.tiles_m - first, 8), in = at - group * 8 * e.tiles_n;
-    const int m0 = (first + in % high) * BM, n0 = (in / high) * BN;
-
+    int m0, n0;
+    q8_tile<8>(e, m0, n0);
+    m0 *= BM;
+    n0 *= BN;
     const int k0 = blockIdx.y * e.steps * 64, steps = min(e.steps, (e.K - k0) >> 6);
     const int8_t* A = e.A + (int64_t)m0 * e.lda + k0;
     const int8_t* W = e.W + (int64_t)n0 * e.ldw + k0;
@@ -379,68 +482,143 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
         }
         return;
     }
-    float sw[NB][4], bias[NB][4];
-#pragma unroll
-    for (int j = 0; j < NB; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int n = n_w + j * 16 + g * 4 + r < e.N ? n_w + j * 16 + g * 4 + r : e.N - 1;
-            sw[j][r] = e.w_scale[n];
-            bias[j][r] = e.bias ? Elem<T>::load((const T*)e.bias + n) : 0.f;
-        }
     __syncthreads();      // the ring is the patches' now
-    char* patch = smem + wave * 16 * PITCH;
+    q8_write<T, MI, NB>(e, acc, smem + wave * 16 * PITCH, n_w, [&](int i) { return m_w + i * 16; });
+}
+
+// The kernel for the largest products: 256 x 256 per workgroup of eight waves, 128 bytes of K a step, K % 128 == 0.  What bounds a large
+// product here is the way from L2 into a CU (about 25 bytes a clock measured, and it moves whole 128-byte lines): a 256 x 256 tile asks
+// for a third less than 256 x 128 does, and a step of 128 bytes takes every line once.  That leaves room for one workgroup to a CU, so
+// its waves take turns by themselves:
+//  * The waves are two groups of four, one of each on every SIMD, half a phase apart: while one group's MFMAs run (a phase has 32 of them),
+//    the other reads its fragments and sends loads.  Group 1 begins with one barrier more, so its first barrier of a phase meets group
+//    0's second.
+//  * A step has two phases, one for each half (128 rows) of A; W's fragments are read in the first and kept.  LDS holds two steps of four
+//    half tiles (A0, W0, W1, A1: in the order in which they are wanted).  Phase (t, 0) sends W1 and A1 of step t + 1, phase (t, 1) sends A0
+//    and W0 of step t + 2 into the places that phase (t, 0) has read.
+//  * Before phase (t, 0) a wave has sent 6 + 4 t half tiles and needs the first 4 t + 3 of them, before (t, 1) 8 + 4 t and 4 t + 4: at most 3
+//    and 4 half tiles, of two loads each, may be on their way; in the last step nothing is.  Group 0 waits at the top of a phase, group 1
+//    for the next phase's before its second barrier, which is the one that opens that phase to group 0.
+//  * A wave's reads have returned before its second barrier of a phase; the other group sends the loads that overwrite those places behind
+//    that barrier.
+//  * A row of 128 bytes has its 16-byte pieces in the order p ^ (row & 7).
+template <typename T>
+__global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
+    constexpr int HALF = 128 * 128, STEP = 4 * HALF, PITCH = q8_pitch(4, sizeof(T));
+    static_assert(8 * 16 * PITCH <= 2 * STEP, "the patches take the ring's place");
+    __shared__ __attribute__((aligned(16))) char smem[2 * STEP];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave >> 2, wn = wave & 3, c = lane & 15, g = lane >> 4;
+    const bool second = wm != 0;
+    int m0, n0;
+    q8_tile<4>(e, m0, n0);
+    m0 *= 256;
+    n0 *= 256;
+    const int steps = e.K >> 7;
+    const int8_t* A = e.A + (int64_t)m0 * e.lda;
+    const int8_t* W = e.W + (int64_t)n0 * e.ldw;
+    uint32_t off[4][2];      // [half tile][load]
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        const int m = m_w + i * 16 + c;
-        const float sa = e.a_scale[m < e.M ? m : e.M - 1];
-        float res[NB][4] = {};      // joins before the one rounding
-        if (e.residual && m < e.M) {
-            const T* p = (const T*)e.residual + (int64_t)m * e.ldr + n_w + g * 4;
+    for (int h = 0; h < 4; ++h)
 #pragma unroll
-            for (int j = 0; j < NB; ++j) {
-                const int n = n_w + j * 16 + g * 4;
-                if (e.wide && n + 4 <= e.N) {
-                    if constexpr (sizeof(T) == 2) {
-                        const uint2 u = *(const uint2*)(p + j * 16);
-                        res[j][0] = __uint_as_float(u.x << 16), res[j][1] = __uint_as_float(u.x & 0xffff0000u);
-                        res[j][2] = __uint_as_float(u.y << 16), res[j][3] = __uint_as_float(u.y & 0xffff0000u);
-                    } else {
-                        const float4 u = *(const float4*)(p + j * 16);
-                        res[j][0] = u.x, res[j][1] = u.y, res[j][2] = u.z, res[j][3] = u.w;
-                    }
-                } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (n + r < e.N) res[j][r] = Elem<T>::load(p + j * 16 + r);
-                }
-            }
+        for (int i = 0; i < 2; ++i) {
+            const bool a = h == 0 || h == 3;
+            int row = (h >= 2 ? 128 : 0) + wave * 16 + i * 8 + (lane >> 3);
+            const int last = a ? e.M - 1 - m0 : e.N - 1 - n0;      // rows beyond the matrix repeat its last one
+            row = row < last ? row : last;
+            off[h][i] = (uint32_t)row * (uint32_t)(a ? e.lda : e.ldw) + (uint32_t)((lane & 7) ^ (lane >> 3)) * 16;
         }
-#pragma unroll
-        for (int j = 0; j < NB; ++j) {
-            float y[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] = q8_value(acc[i][j][r], sa, sw[j][r], bias[j][r], e.act) + res[j][r];
-            if constexpr (sizeof(T) == 2) *(uint2*)(patch + c * PITCH + (j * 16 + g * 4) * 2) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-            else *(float4*)(patch + c * PITCH + (j * 16 + g * 4) * 4) = float4{y[0], y[1], y[2], y[3]};
-        }
-        asm volatile("" ::: "memory");      // the patch is the wave's own, and a wave's LDS accesses stay in order
-        constexpr int V = Elem<T>::VEC, CH = 16 * NB / V;      // 16-byte pieces of a row
-#pragma unroll
-        for (int x = 0; x < 16 * CH; x += 64) {
-            const int r = (x + lane) / CH, d = ((x + lane) - r * CH) * V, mm = m_w + i * 16 + r, n = n_w + d;
-            if (mm >= e.M || n >= e.N) continue;
-            float y[V];
-            load_vec<T>((const T*)(patch + r * PITCH) + d, y);
-            T* out = (T*)e.out + (int64_t)mm * e.ldo + n;
-            if (e.wide && n + V <= e.N) store_vec<T>(out, y);
-            else
-#pragma unroll
-                for (int q = 0; q < V; ++q)
-                    if (n + q < e.N) Elem<T>::store(out + q, y[q]);
-        }
+    const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)smem + wave * 2048;
+    auto load = [&](int t, auto half) {      // half tile `half` of step t
+        constexpr int h = decltype(half)::value;
+        if (t >= steps) return;
+        const int8_t* base = (h == 0 || h == 3 ? A : W) + (int64_t)t * 128;
+        dma16(base, off[h][0], ring + (t & 1) * STEP + h * HALF);
+        dma16(base, off[h][1], ring + (t & 1) * STEP + h * HALF + 1024);
+    };
+    using H0 = std::integral_constant<int, 0>;
+    using H1 = std::integral_constant<int, 1>;
+    using H2 = std::integral_constant<int, 2>;
+    using H3 = std::integral_constant<int, 3>;
+    auto barrier = [] {
         asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    load(0, H0{}); load(0, H1{}); load(0, H2{}); load(0, H3{});
+    load(1, H0{}); load(1, H1{});
+    i32x4 acc[8][4];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    auto wait_first = [&](int t) {      // for phase (t, 0)
+        if (t < steps - 1) wait_loads<6>();
+        else wait_loads<0>();
+    };
+    auto wait_second = [&](int t) {     // for phase (t, 1)
+        if (t < steps - 1) wait_loads<8>();
+        else wait_loads<0>();
+    };
+    if (second) {
+        wait_first(0);
+        barrier();
     }
+    const int p0 = (g ^ (c & 7)) * 16, p1 = ((4 + g) ^ (c & 7)) * 16;      // this lane's pieces of a row: the step's first and second 64 bytes
+    i32x4 af[4][2], wf[4][2];
+    for (int t = 0; t < steps; ++t) {
+        const char* step = smem + (t & 1) * STEP;
+        const char* a = step + (wm * 64 + c) * 128;
+        const char* w = step + (wn >> 1 ? 2 : 1) * HALF + ((wn & 1) * 64 + c) * 128;
+        // phase 0
+        if (!second) wait_first(t);
+        barrier();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            wf[j][0] = *(const i32x4*)(w + j * 2048 + p0);
+            af[j][0] = *(const i32x4*)(a + j * 2048 + p0);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            wf[j][1] = *(const i32x4*)(w + j * 2048 + p1);
+            af[j][1] = *(const i32x4*)(a + j * 2048 + p1);
+        }
+        load(t + 1, H2{});
+        load(t + 1, H3{});
+        if (second) wait_second(t);
+        __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
+        barrier();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+        // phase 1
+        if (!second) wait_second(t);
+        barrier();
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) af[i][k] = *(const i32x4*)(a + 3 * HALF + i * 2048 + (k ? p1 : p0));
+        load(t + 2, H0{});
+        load(t + 2, H1{});
+        if (second && t + 1 < steps) wait_first(t + 1);
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+        barrier();
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) acc[4 + i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[4 + i][j], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+    if (!second) barrier();      // group 1 has read its last fragments: the ring is the patches' now
+    q8_write<T, 8, 4>(e, acc, smem + wave * 16 * PITCH, n0 + wn * 64, [&](int i) { return m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16; });
 }
 
 template <typename T, int MI, int NB, int NS>
@@ -457,7 +635,11 @@ static int launch_linear_q8(Q8Args& e, hipStream_t s) {
     ProfScope ps(BT_PROF_LINEAR_MFMA, s);
     if (e.K % 64 == 0 && e.lda < (1 << 23) && e.ldw < (1 << 23)) {
         const int64_t big = ceil_div(e.M, 256) * ceil_div(e.N, 128);
-        if (big >= 512) launch_tile<T, 8, 4, 3>(e, s);
+        if (e.K % 128 == 0 && ceil_div(e.M, 256) * ceil_div(e.N, 256) >= 192) {
+            e.tiles_m = (int)ceil_div(e.M, 256);
+            e.tiles_n = (int)ceil_div(e.N, 256);
+            hipLaunchKernelGGL((linear_q8_big_kernel<T>), dim3((unsigned)(e.tiles_m * e.tiles_n)), dim3(512), 0, s, e);
+        } else if (big >= 512) launch_tile<T, 8, 4, 3>(e, s);
         else if (ceil_div(e.M, 128) * ceil_div(e.N, 128) >= 256) launch_tile<T, 4, 4, 4>(e, s);
         else launch_tile<T, 2, 2, 4>(e, s);
     } else
