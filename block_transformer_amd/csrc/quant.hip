@@ -3,6 +3,7 @@
 #include "bt_gelu.h"
 #include "bt_quant.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace bt {
@@ -232,58 +233,6 @@ __device__ inline void q8_values(const i32x4& acc, float sa, const float (&sw)[4
     }
 }
 
-template <typename T>
-__device__ inline void q8_store(const Q8Args& e, int m, int n, int acc) {
-    const float bias[4] = {e.bias ? Elem<T>::load((const T*)e.bias + n) : 0.f}, sw[4] = {e.w_scale[n]};
-    float y[4];
-    q8_values<T>(i32x4{acc, 0, 0, 0}, e.a_scale[m], sw, bias, e.act, y);
-    if (e.residual) y[0] += Elem<T>::load((const T*)e.residual + (int64_t)m * e.ldr + n);
-    Elem<T>::store((T*)e.out + (int64_t)m * e.ldo + n, y[0]);
-}
-
-// Any K % 16 == 0: 64 x 64 tile per workgroup, 64 bytes of K at a time through LDS, four products per v_dot4.
-template <typename T>
-__global__ __launch_bounds__(256) void linear_q8_dot_kernel(Q8Args e) {
-    __shared__ int4 sa[64][5], sw[64][5];
-    const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64;
-    const int r = threadIdx.x >> 2, c = threadIdx.x & 3;
-    const int tm = (threadIdx.x >> 4) * 4, tn = (threadIdx.x & 15) * 4;
-    int acc[4][4] = {};
-    for (int k0 = 0; k0 < e.K; k0 += 64) {
-        const int k = k0 + c * 16;
-        int4 a{0, 0, 0, 0}, w{0, 0, 0, 0};
-        if (k < e.K && m0 + r < e.M) a = *(const int4*)(e.A + (m0 + r) * e.lda + k);
-        if (k < e.K && n0 + r < e.N) w = *(const int4*)(e.W + (n0 + r) * e.ldw + k);
-        __syncthreads();
-        sa[r][c] = a;
-        sw[r][c] = w;
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            int4 av[4], wv[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                av[i] = sa[tm + i][q];
-                wv[i] = sw[tn + i][q];
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    acc[i][j] = __builtin_amdgcn_sdot4(av[i].x, wv[j].x, acc[i][j], false);
-                    acc[i][j] = __builtin_amdgcn_sdot4(av[i].y, wv[j].y, acc[i][j], false);
-                    acc[i][j] = __builtin_amdgcn_sdot4(av[i].z, wv[j].z, acc[i][j], false);
-                    acc[i][j] = __builtin_amdgcn_sdot4(av[i].w, wv[j].w, acc[i][j], false);
-                }
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (m0 + tm + i < e.M && n0 + tn + j < e.N) q8_store<T>(e, m0 + tm + i, n0 + tn + j, acc[i][j]);
-}
-
 // 16 bytes per lane from base + off (unsigned) straight into LDS at lds + 16 * lane.  The waits cover an M0 write right before the load
 // (1) and a base that a v_readlane may just have brought back from a spill (5): neither is padded inside an asm string.
 __device__ inline void dma16(const int8_t* base, uint32_t off, uint32_t lds) {
@@ -388,7 +337,8 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
     }
 }
 
-// The tile kernel: 32 MI x 32 NB per workgroup of 2 x 2 waves, 64 bytes of K a step, K % 64 == 0.
+// The tile kernel: 32 MI x 32 NB per workgroup of 2 x 2 waves, 64 bytes of K a step; of a last step that is not whole, what lies behind K
+// is replaced by the step's first bytes, and A's operand is zero there.
 //  * Two workgroups to a CU: while one waits at its barrier or writes its tile, the other's waves have the matrix units.  So a K step
 //    needs one barrier and the epilogue no software overlap.
 //  * A and W travel global -> LDS without registers, NS - 1 steps ahead, in a ring of NS stages.  A wave waits for its own loads of step t
@@ -411,7 +361,9 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
     q8_tile<8>(e, m0, n0);
     m0 *= BM;
     n0 *= BN;
-    const int k0 = blockIdx.y * e.steps * 64, steps = min(e.steps, (e.K - k0) >> 6);
+    const int k0 = blockIdx.y * e.steps * 64, steps = min(e.steps, (e.K - k0 + 63) >> 6);
+    const int whole = min(4, (e.K - k0 - (steps - 1) * 64) >> 4);      // 16-byte pieces of the last step
+    const int cut = whole < 4 ? steps - 1 : -1;
     const int8_t* A = e.A + (int64_t)m0 * e.lda + k0;
     const int8_t* W = e.W + (int64_t)n0 * e.ldw + k0;
     uint32_t off[LOADS];
@@ -423,13 +375,15 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
         row = row < last ? row : last;
         off[i] = (uint32_t)row * (uint32_t)(i < LA ? e.lda : e.ldw) + piece * 16;
     }
+    const uint32_t back = piece >= whole ? piece * 16 : 0;
     const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)smem;
     auto load = [&](int t) {
         const uint32_t stage = ring + (t % NS) * STAGE;
+        const uint32_t less = t == cut ? back : 0;
 #pragma unroll
         for (int i = 0; i < LOADS; ++i)
-            if (i < LA) dma16(A + (int64_t)t * 64, off[i], stage + (wave * LA + i) * 1024);
-            else dma16(W + (int64_t)t * 64, off[i], stage + BM * 64 + (wave * LW + i - LA) * 1024);
+            if (i < LA) dma16(A + (int64_t)t * 64, off[i] - less, stage + (wave * LA + i) * 1024);
+            else dma16(W + (int64_t)t * 64, off[i] - less, stage + BM * 64 + (wave * LW + i - LA) * 1024);
     };
     i32x4 acc[MI][NB];
 #pragma unroll
@@ -442,8 +396,9 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
 
     const int frag = c * 64 + (g ^ ((c >> 1) & 3) ^ ((c >> 3) & 1)) * 16;
     int stage = 0;
-    for (int t = 0; t < steps; ++t) {
+    auto step = [&](int t, auto last) {
         if (t + NS - 2 < steps) wait_loads<LOADS * (NS - 2)>();
+        else if (NS > 4 && t + 4 < steps) wait_loads<LOADS * 4>();      // (at most what is still out)
         else if (NS > 3 && t + 1 < steps) wait_loads<LOADS>();
         else wait_loads<0>();
         __builtin_amdgcn_s_barrier();
@@ -456,12 +411,21 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
         for (int j = 0; j < NB; ++j) wf[j] = *(const i32x4*)(w + j * 1024);
 #pragma unroll
         for (int i = 0; i < MI; ++i) af[i] = *(const i32x4*)(a + i * 1024);
+        if constexpr (decltype(last)::value) {
+            if (g >= whole) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i) af[i] = i32x4{0, 0, 0, 0};
+            }
+        }
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
             for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], af[i], acc[i][j], 0, 0, 0);
         stage = stage + 1 == NS ? 0 : stage + 1;
-    }
+    };
+    const int full = steps - (cut >= 0);
+    for (int t = 0; t < full; ++t) step(t, std::false_type{});
+    if (cut >= 0) step(cut, std::true_type{});
 
     const int m_w = m0 + wm * MI * 16, n_w = n0 + wn * NB * 16;
     if (e.slices > 1) {
@@ -621,29 +585,177 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
     q8_write<T, 8, 4>(e, acc, smem + wave * 16 * PITCH, n0 + wn * 64, [&](int i) { return m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16; });
 }
 
+// Few rows: 16 MB rows by 16 NB columns per workgroup, the waves dividing K among themselves.  W is read once, straight into the operand
+// registers of the matrix instruction (a lane holds 16 bytes of a row: nothing to rearrange, no LDS, no barrier in the loop), with
+// every load of four 128-byte units out at once: a problem of this size is a few microseconds of latency, not of bandwidth.  A comes the
+// same way, from the caches.  The partial sums meet in LDS; being integers, they do not depend on the number of waves.
+template <typename T, int MB, int NB, int NW>
+__global__ __launch_bounds__(NW * 64) void linear_q8_rows_kernel(Q8Args e) {
+    __shared__ i32x4 part[NW][MB * NB][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int n0 = blockIdx.x * 16 * NB, m0 = blockIdx.y * 16 * MB;
+    const int8_t* ap[MB];
+    const int8_t* wp[NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i) ap[i] = e.A + (int64_t)min(m0 + 16 * i + c, e.M - 1) * e.lda + 16 * g;
+#pragma unroll
+    for (int j = 0; j < NB; ++j) wp[j] = e.W + (int64_t)min(n0 + 16 * j + c, e.N - 1) * e.ldw + 16 * g;
+    i32x4 acc[MB][NB];
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+    constexpr int U = MB * NB >= 8 ? 1 : MB * NB >= 2 ? 2 : 4;      // units of a round
+    const i32x4 zero{0, 0, 0, 0};
+    for (int k = wave * 128; k < e.K; k += NW * 128 * U) {
+        i32x4 a[U][2][MB], w[U][2][NB];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int at = k + u * NW * 128 + h * 64;
+                const bool in = at + 16 * g < e.K;      // K is a whole number of 16-byte pieces
+#pragma unroll
+                for (int j = 0; j < NB; ++j) w[u][h][j] = in ? *(const i32x4*)(wp[j] + at) : zero;
+#pragma unroll
+                for (int i = 0; i < MB; ++i) a[u][h][i] = in ? *(const i32x4*)(ap[i] + at) : zero;
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int i = 0; i < MB; ++i)
+#pragma unroll
+                    for (int j = 0; j < NB; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][h][j], a[u][h][i], acc[i][j], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < MB; ++i)
+#pragma unroll
+        for (int j = 0; j < NB; ++j) part[wave][i * NB + j][lane] = acc[i][j];
+    __syncthreads();
+    // lane (c, g) of fragment f: row c, columns 4 g .. 4 g + 3
+    for (int x = threadIdx.x; x < MB * NB * 64; x += NW * 64) {
+        const int f = x >> 6, l = x & 63;
+        i32x4 sum = part[0][f][l];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) sum += part[w][f][l];
+        const int m = m0 + f / NB * 16 + (l & 15), n = n0 + f % NB * 16 + (l >> 4) * 4;
+        if (m >= e.M || n >= e.N) continue;
+        float sw[4], bias[4], y[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            sw[r] = e.w_scale[min(n + r, e.N - 1)];
+            bias[r] = e.bias ? Elem<T>::load((const T*)e.bias + min(n + r, e.N - 1)) : 0.f;
+        }
+        q8_values<T>(sum, e.a_scale[m], sw, bias, e.act, y);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            if (n + r >= e.N) continue;
+            if (e.residual) y[r] += Elem<T>::load((const T*)e.residual + (int64_t)m * e.ldr + n + r);
+            Elem<T>::store((T*)e.out + (int64_t)m * e.ldo + n + r, y[r]);
+        }
+    }
+}
+
+// Joins K slices: sums them (integers: in any order) and finishes as the tile kernel does.  Four columns a thread.
+template <typename T>
+__global__ __launch_bounds__(256) void linear_q8_join_kernel(Q8Args e) {
+    const int quads = (e.N + 3) >> 2;
+    const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (x >= (int64_t)e.M * quads) return;
+    const int m = (int)(x / quads), n = (int)(x - (int64_t)m * quads) * 4;
+    const int64_t slice = (int64_t)e.M * e.N;
+    const int* p = e.slab + (int64_t)m * e.N + n;
+    const bool four = n + 4 <= e.N && (e.N & 3) == 0;
+    i32x4 sum{0, 0, 0, 0};
+    for (int s = 0; s < e.slices; ++s, p += slice) {
+        if (four) sum += *(const i32x4*)p;
+        else
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (n + r < e.N) sum[r] += p[r];
+    }
+    float sw[4], bias[4], y[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        sw[r] = e.w_scale[min(n + r, e.N - 1)];
+        bias[r] = e.bias ? Elem<T>::load((const T*)e.bias + min(n + r, e.N - 1)) : 0.f;
+    }
+    q8_values<T>(sum, e.a_scale[m], sw, bias, e.act, y);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if (n + r >= e.N) continue;
+        if (e.residual) y[r] += Elem<T>::load((const T*)e.residual + (int64_t)m * e.ldr + n + r);
+        Elem<T>::store((T*)e.out + (int64_t)m * e.ldo + n + r, y[r]);
+    }
+}
+
+// What runs a product, from its sizes alone: the cheapest by a model of the time in microseconds, fitted to graph-replayed launches of
+// M = 32 .. 8192 by N = 2048, 6144, 8192 by K = 2048, 8192 (within 20 % of them; its choice within 10 % of the best).
+//   64 x 64 tiles    4 + 0.18 a step while there is one to a CU, 0.128 times their number from two on    (256 x 6144 x 2048: 11.7; 128 x 128: 18.2)
+//   128 x 128 tiles  5 + 0.36 a step, times their number to a CU from one on                             (512 x 8192 x 2048: 19.7; 64 x 64: 21.6)
+//   256 x 256 tiles  11 + 1.5 for two steps, times rounds                                                (2048 x 6144 x 2048: 32.7; 128 x 128: 40.8)
+//   K in slices      3 for the second launch, and the sums once out and once in at 4 TB/s                (256 x 2048 x 8192 in 4: 18.8; whole: 27.5)
+// Up to 32 rows the rows kernel, which reads W as fast as it comes (1 x 6144 x 2048: 5.1; from 33 rows on tiles are as fast or faster).
+struct Q8Plan {
+    enum Kind { ROWS, TILE64, TILE128, BIG } kind;
+    int slices;      // of K (TILE64 and TILE128)
+};
+
+static Q8Plan q8_plan(int64_t M, int64_t N, int64_t K) {
+    if (M <= 32) return {Q8Plan::ROWS, 1};
+    const int64_t steps = ceil_div(K, 64);
+    const double t64 = (double)(ceil_div(M, 64) * ceil_div(N, 64)) / 256, t128 = (double)(ceil_div(M, 128) * ceil_div(N, 128)) / 256;
+    Q8Plan best{Q8Plan::TILE64, 1};
+    double least = 1e30;
+    for (int s = 1; s <= 8 && (s == 1 || steps / s >= 4); s *= 2) {
+        const double part = (double)ceil_div(steps, s), join = s == 1 ? 0 : 3 + (double)s * (double)M * (double)N * 8 / 4e6;
+        const double a = 4 + part * std::max(0.18, 0.128 * t64 * s) + join, b = 5 + part * 0.36 * std::max(1.0, t128 * s) + join;
+        if (a < least) least = a, best = {Q8Plan::TILE64, s};
+        if (b < least) least = b, best = {Q8Plan::TILE128, s};
+    }
+    if (K % 128 == 0 && (double)ceil_div(ceil_div(M, 256) * ceil_div(N, 256), 256) * (11 + 0.75 * (double)steps) < least) best = {Q8Plan::BIG, 1};
+    return best;
+}
+
 template <typename T, int MI, int NB, int NS>
-static void launch_tile(Q8Args& e, hipStream_t s) {
+static void launch_tile(Q8Args& e, int slices, hipStream_t s) {
     e.tiles_m = (int)ceil_div(e.M, 32 * MI);
     e.tiles_n = (int)ceil_div(e.N, 32 * NB);
-    e.slices = 1;
-    e.steps = e.K / 64;
-    hipLaunchKernelGGL((linear_q8_tile_kernel<T, MI, NB, NS>), dim3((unsigned)(e.tiles_m * e.tiles_n), 1), dim3(256), 0, s, e);
+    e.steps = (int)ceil_div(ceil_div(e.K, 64), slices);
+    e.slices = (int)ceil_div(ceil_div(e.K, 64), e.steps);
+    hipLaunchKernelGGL((linear_q8_tile_kernel<T, MI, NB, NS>), dim3((unsigned)(e.tiles_m * e.tiles_n), (unsigned)e.slices), dim3(256), 0, s, e);
+    if (e.slices > 1)
+        hipLaunchKernelGGL((linear_q8_join_kernel<T>), dim3((unsigned)ceil_div((int64_t)e.M * ((e.N + 3) / 4), 256)), dim3(256), 0, s, e);
+}
+
+template <typename T, int MB, int NB>
+static void launch_rows(const Q8Args& e, hipStream_t s) {
+    hipLaunchKernelGGL((linear_q8_rows_kernel<T, MB, NB, 8>), dim3((unsigned)ceil_div(e.N, 16 * NB), (unsigned)ceil_div(e.M, 16 * MB)), dim3(512),
+                       0, s, e);
 }
 
 template <typename T>
-static int launch_linear_q8(Q8Args& e, hipStream_t s) {
+static int launch_linear_q8(Q8Args& e, int64_t scratch_bytes, hipStream_t s) {
     ProfScope ps(BT_PROF_LINEAR_MFMA, s);
-    if (e.K % 64 == 0 && e.lda < (1 << 23) && e.ldw < (1 << 23)) {
-        const int64_t big = ceil_div(e.M, 256) * ceil_div(e.N, 128);
-        if (e.K % 128 == 0 && ceil_div(e.M, 256) * ceil_div(e.N, 256) >= 192) {
+    Q8Plan p = q8_plan(e.M, e.N, e.K);
+    if (p.slices > 1 && scratch_bytes < (int64_t)p.slices * e.M * e.N * (int64_t)sizeof(int)) p.slices = 1;
+    if (e.lda >= (1 << 23) || e.ldw >= (1 << 23)) p.kind = Q8Plan::ROWS;      // a tile's rows would not be within 32 bits
+    switch (p.kind) {
+        case Q8Plan::ROWS:
+            if (e.M <= 16) launch_rows<T, 1, 1>(e, s);
+            else launch_rows<T, 2, 1>(e, s);
+            break;
+        case Q8Plan::TILE64: launch_tile<T, 2, 2, 8>(e, p.slices, s); break;
+        case Q8Plan::TILE128: launch_tile<T, 4, 4, 4>(e, p.slices, s); break;
+        case Q8Plan::BIG:
             e.tiles_m = (int)ceil_div(e.M, 256);
             e.tiles_n = (int)ceil_div(e.N, 256);
             hipLaunchKernelGGL((linear_q8_big_kernel<T>), dim3((unsigned)(e.tiles_m * e.tiles_n)), dim3(512), 0, s, e);
-        } else if (big >= 512) launch_tile<T, 8, 4, 3>(e, s);
-        else if (ceil_div(e.M, 128) * ceil_div(e.N, 128) >= 256) launch_tile<T, 4, 4, 4>(e, s);
-        else launch_tile<T, 2, 2, 4>(e, s);
-    } else
-        hipLaunchKernelGGL((linear_q8_dot_kernel<T>), dim3((unsigned)ceil_div(e.N, 64), (unsigned)ceil_div(e.M, 64)), dim3(256), 0, s, e);
+            break;
+    }
     BT_LAUNCH_CHECK("bt_linear_q8 launch");
     return BT_OK;
 }
@@ -668,8 +780,9 @@ extern "C" int bt_quant_rows(int dtype, int64_t M, int64_t K, const void* x, int
 }
 
 extern "C" int64_t bt_linear_q8_scratch_bytes(int64_t M, int64_t N, int64_t K) {
-    (void)M; (void)N; (void)K;
-    return 0;
+    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    const Q8Plan p = q8_plan(M, N, K);
+    return p.slices > 1 ? (int64_t)p.slices * M * N * (int64_t)sizeof(int) : 0;
 }
 
 extern "C" int bt_linear_q8(int dtype, int64_t M, int64_t N, int64_t K, const int8_t* A, int64_t lda, const float* a_scale,
@@ -704,5 +817,8 @@ extern "C" int bt_linear_q8(int dtype, int64_t M, int64_t N, int64_t K, const in
     e.act = act;
     const int V = dtype == BT_BF16 ? 8 : 4;
     e.wide = aligned16(out) && ldo % V == 0 && (!residual || (aligned16(residual) && ldr % V == 0));
-    return dtype == BT_BF16 ? launch_linear_q8<bf16>(e, (hipStream_t)stream) : launch_linear_q8<float>(e, (hipStream_t)stream);
+    e.slab = (int*)scratch;
+    if (!scratch) scratch_bytes = 0;
+    return dtype == BT_BF16 ? launch_linear_q8<bf16>(e, scratch_bytes, (hipStream_t)stream)
+                            : launch_linear_q8<float>(e, scratch_bytes, (hipStream_t)stream);
 }
