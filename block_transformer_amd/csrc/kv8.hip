@@ -477,19 +477,20 @@ struct Attend {
         for (int k = 0; k < NC; ++k) {
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                uint32_t out[ND] = {};
+                uint32_t v[4];      // the number plus 128 for every lower digit: its bytes are the digits, the lower ones with 128 on top
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    int v = bad != 0.f ? 0 : (int)rintf(x[k][4 * w + e] * up * inv);
-#pragma unroll
-                    for (int i = ND - 1; i >= 0; --i) {
-                        const int low = i ? (int)(int8_t)(v & 255) : v;
-                        out[i] |= (uint32_t)(low & 255) << (8 * e);
-                        v = (v - low) >> 8;
-                    }
+                for (int e = 0; e < 4; ++e)
+                    v[e] = bad != 0.f ? (ND == 2 ? 0x80u : 0x8080u) : (uint32_t)((int)rintf(x[k][4 * w + e] * up * inv) + (ND == 2 ? 0x80 : 0x8080));
+                const uint32_t a01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010400), a23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010400);
+                const uint32_t b0 = __builtin_amdgcn_perm(a23, a01, 0x05040100), b1 = __builtin_amdgcn_perm(a23, a01, 0x07060302);
+                if (ND == 2) {
+                    dig[0][k][w] = (int)b1;
+                } else {
+                    const uint32_t c01 = __builtin_amdgcn_perm(v[1], v[0], 0x06020602), c23 = __builtin_amdgcn_perm(v[3], v[2], 0x06020602);
+                    dig[0][k][w] = (int)__builtin_amdgcn_perm(c23, c01, 0x05040100);
+                    dig[1][k][w] = (int)(b1 ^ 0x80808080u);
                 }
-#pragma unroll
-                for (int i = 0; i < ND; ++i) dig[i][k][w] = (int)out[i];
+                dig[ND - 1][k][w] = (int)(b0 ^ 0x80808080u);
             }
         }
     }
@@ -512,15 +513,30 @@ struct Attend {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) v[j] = *(const i32x4*)(p + (int64_t)16 * j * a.c.block);
     }
-    // bit e: this lane's query sees row 16 g + e of the tile (all 16 rows begin at tok0)
+    // bits 0 .. count - 1: the mask of rows tok0 .. (those before `end`)
+    __device__ inline uint32_t masked(int64_t tok0, int count, int64_t end) const {
+        uint32_t on = 0;
+        if (count == 16 && tok0 + 16 <= end) {      // 16 bytes at once, wherever they lie
+            uint4 u;
+            __builtin_memcpy(&u, mask + tok0, 16);
+            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t set = ((((w[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[i]) >> 7) & 0x01010101u;      // bytes that are not 0
+                on |= ((set * 0x10204080u) >> 28) << (4 * i);      // its first byte to bit 28, its last to bit 31
+            }
+        } else {
+            for (int e = 0; e < count; ++e)
+                if (tok0 + e < end && mask[tok0 + e] != 0) on |= 1u << e;
+        }
+        return on;
+    }
+    // bit e: this lane's query sees row tok0 + e, one of `count` rows of which those before `end` are there
     __device__ inline uint32_t visible(int64_t tok0, int count, int64_t end) const {
         const int64_t left = (end < lim ? end : lim) - tok0;
         const int most = left < count ? (left < 0 ? 0 : (int)left) : count;
-        uint32_t on = (1u << most) - 1u;
-        if (mask)
-            for (int e = 0; e < count; ++e)
-                if (tok0 + e < end && mask[tok0 + e] == 0) on &= ~(1u << e);
-        return on;
+        const uint32_t on = (1u << most) - 1u;
+        return mask ? on & masked(tok0, count, end) : on;
     }
 
     // enters a tile with its largest score mt: the factor for what is there already; `gamma` for what comes
@@ -531,7 +547,10 @@ struct Attend {
         return alpha;
     }
 
-    __device__ inline void tile(int64_t at, const i32x4 (&k)[4][NC], const i32x4 (&v)[NJ], bool cut) {
+    // One tile.  `k` and `v` hold it; MORE: the next tile's take their places as soon as they have been used, K under the softmax and
+    // the second product, V under the next tile's first.
+    template <bool MORE>
+    __device__ inline void tile(int64_t at, int64_t then, i32x4 (&k)[4][NC], i32x4 (&v)[NJ], bool cut) {
         const int64_t tok0 = at * 64 + 16 * g, blk = tok0 >> a.shift;
         const float sk = blk < full ? ks[blk] : 0.f, sv = blk < full ? vs[blk] : 0.f;
         const float mul = qs * sk;
@@ -551,6 +570,7 @@ struct Attend {
 #pragma unroll
             for (int r = 0; r < 4; ++r) s[i][r] = (ND == 3 ? fmaf((float)acc[r], 256.f, (float)low[r]) : (float)acc[r]) * mul;
         }
+        if (MORE) load_k(then, k);
         if (cut) {
             const uint32_t on = visible(tok0, 16, n_full);
 #pragma unroll
@@ -597,6 +617,7 @@ struct Attend {
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[j][r] = fmaf((float)acc[r], beta256, fmaf((float)low[r], beta, o[j][r] * alpha));
         }
+        if (MORE) load_v(then, v);
     }
 
     // The open block: rows n_full .. end - 1, row 4 nI g + 4 i + r of it with lane g's (i, r), nI = block / 16.
@@ -633,9 +654,8 @@ struct Attend {
         }
         const int64_t tok0 = n_full + per * g;
         const uint32_t on = visible(tok0, per, end);
-        uint32_t some = 0;      // rows that any query may see
-        for (int e = 0; e < per; ++e)
-            if (tok0 + e < end && !(mask && mask[tok0 + e] == 0)) some |= 1u << e;
+        const int there = end - tok0 < per ? (end > tok0 ? (int)(end - tok0) : 0) : per;
+        const uint32_t some = ((1u << there) - 1u) & (mask ? masked(tok0, per, end) : ~0u);      // rows that any query may see
         float mt = M_FLOOR;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -655,41 +675,49 @@ struct Attend {
                 sum += s[i][r];
             }
         l = fmaf(l, alpha, sum);
-        bool odd = false;
+        // P V.  Rows that nobody may see are taken as zero: they may hold anything.
+        f32x4 before[NJ];
+        uint32_t keep[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) keep[e] = (some >> e) & 1 ? ~0u : 0u;
+        float zero = 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            o[j] *= alpha;
+            before[j] = o[j] *= alpha;
             const T* vr = vt + (16 * j + c) * bl + per * g;
-            float v[16];
+            if constexpr (sizeof(T) == 2) {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                v[e] = e < per ? Elem<T>::load(vr + e) : 0.f;
-                v[e] = (some >> e) & 1 ? v[e] : 0.f;
-                odd |= !(fabsf(v[e]) < INFINITY);
-                v[e] = fabsf(v[e]) < INFINITY ? v[e] : 0.f;
-            }
-#pragma unroll
-            for (int h = 0; h < 16; h += 8) {
-                if (h >= per) continue;
-                if constexpr (sizeof(T) == 2) {
+                for (int h = 0; h < 16; h += 8) {
+                    if (h >= per) continue;
                     union { uint32_t u[4]; bf16x8 f; } vf, hi, lo;
 #pragma unroll
                     for (int e = 0; e < 8; e += 2) {
                         const float p0 = s[(h + e) >> 2][(h + e) & 3], p1 = s[(h + e + 1) >> 2][(h + e + 1) & 3];
-                        vf.u[e >> 1] = pack_bf16x2(v[h + e], v[h + e + 1]);
+                        vf.u[e >> 1] = h + e < per ? *(const uint32_t*)(vr + h + e) : 0u;      // per is 4, 8 or 16
+                        vf.u[e >> 1] &= __builtin_amdgcn_perm(keep[h + e + 1], keep[h + e], 0x05040100);
                         hi.u[e >> 1] = pack_bf16x2(p0, p1);
                         lo.u[e >> 1] = pack_bf16x2(p0 - __uint_as_float(hi.u[e >> 1] << 16), p1 - __uint_as_float(hi.u[e >> 1] & 0xffff0000u));
                     }
                     o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.f, hi.f, o[j], 0, 0, 0);
                     o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.f, lo.f, o[j], 0, 0, 0);
-                } else {
+                }
+            } else {
 #pragma unroll
-                    for (int e = h; e < h + 8; ++e) o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e], s[e >> 2][e & 3], o[j], 0, 0, 0);
+                for (int h = 0; h < 16; h += 4) {
+                    if (h >= per) continue;
+                    const f32x4 v = *(const f32x4*)(vr + h);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        o[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(__float_as_uint(v[e]) & keep[h + e]), s[h >> 2][e], o[j], 0, 0, 0);
                 }
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) zero = fmaf(o[j][r], 0.f, zero);
         }
-        // an infinity or NaN in a row that some queries see and others may not: a matrix product would give it to all of them
-        if (__any(odd)) {
+        // An infinity or NaN in a row that some queries see and others do not: the product has given it to all of them.  Once more, by hand.
+        if (__any(zero != 0.f)) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) o[j] = before[j];
 #pragma unroll 1
             for (int x = 0; x < bl; ++x) {
                 const int gg = x / per, e = x - gg * per;
@@ -703,7 +731,7 @@ struct Attend {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const float y = Elem<T>::load(vt + (16 * j + 4 * g + r) * bl + x);
-                        if (seen && !(fabsf(y) < INFINITY)) o[j][r] = fmaf(p, y, o[j][r]);
+                        o[j][r] = seen ? fmaf(p, y, o[j][r]) : o[j][r];
                     }
             }
         }
@@ -711,7 +739,7 @@ struct Attend {
 };
 
 template <typename T, int D, int NW>
-__global__ __launch_bounds__(NW * 64, NW == 1 ? 2 : 2) void attention_kv8_kernel(AttnArgs a) {
+__global__ __launch_bounds__(NW * 64, 2) void attention_kv8_kernel(AttnArgs a) {
     using A = Attend<T, D>;
     __shared__ float merged[NW > 1 ? NW : 1][NW > 1 ? 16 : 1][D + 4];
     const int wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
@@ -749,21 +777,15 @@ __global__ __launch_bounds__(NW * 64, NW == 1 ? 2 : 2) void attention_kv8_kernel
     const int64_t tiles = (closed + 63) >> 6, all = tiles + (end > w.n_full ? 1 : 0);
     const int64_t per = (all + a.n_split - 1) / a.n_split;
     int64_t at = split * per + wave;
-    const int64_t stop = (split + 1) * per < all ? (split + 1) * per : all;
-    i32x4 k[4][A::NC], v[A::NJ];
-    if (at < stop && at < tiles) w.load_k(at, k);
-    for (; at < stop && at < tiles; at += NW) {
-        i32x4 next[4][A::NC];
+    const int64_t stop = (split + 1) * per < all ? (split + 1) * per : all, closed_stop = stop < tiles ? stop : tiles;
+    if (at < closed_stop) {
+        i32x4 k[4][A::NC], v[A::NJ];
+        w.load_k(at, k);
         w.load_v(at, v);
-        const bool more = at + NW < stop && at + NW < tiles;
-        if (more) w.load_k(at + NW, next);
-        w.tile(at, k, v, w.mask || at * 64 + 64 > w.n_full || at * 64 + 64 > least);
-        if (more) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int x = 0; x < A::NC; ++x) k[i][x] = next[i][x];
-        }
+        auto cut = [&](int64_t t) { return w.mask || t * 64 + 64 > w.n_full || t * 64 + 64 > least; };
+        for (; at + NW < closed_stop; at += NW) w.template tile<true>(at, at + NW, k, v, cut(at));
+        w.template tile<false>(at, 0, k, v, cut(at));
+        at += NW;
     }
     if (at < stop) w.tail(end);
     w.l = sum_over_groups(w.l);
