@@ -505,6 +505,19 @@ struct Attend {
             for (int n = 0; n < NC; ++n) k[i][n] = *(const i32x4*)(p + 64 * n);
         }
     }
+    // the scales and the mask of this lane's 16 rows of a tile
+    struct Side {
+        float sk, sv;
+        uint4 mask;
+    };
+    __device__ inline Side load_side(int64_t tile) const {
+        const int64_t tok = tile * 64 + 16 * g;
+        int64_t blk = tok >> a.shift;
+        blk = blk < full ? blk : full - 1;      // (a tile has a full block; what lies behind the last is hidden)
+        Side x{ks[blk], vs[blk], uint4{0, 0, 0, 0}};
+        if (mask && tok + 16 <= n_full) __builtin_memcpy(&x.mask, mask + tok, 16);      // wherever they lie
+        return x;
+    }
     __device__ inline void load_v(int64_t tile, i32x4 (&v)[NJ]) const {
         const int64_t tok = tile * 64 + 16 * g;
         int64_t blk = tok >> a.shift;
@@ -513,30 +526,22 @@ struct Attend {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) v[j] = *(const i32x4*)(p + (int64_t)16 * j * a.c.block);
     }
-    // bits 0 .. count - 1: the mask of rows tok0 .. (those before `end`)
-    __device__ inline uint32_t masked(int64_t tok0, int count, int64_t end) const {
+    // bit e: byte e is not 0
+    __device__ static inline uint32_t set_bytes(const uint4& u) {
+        const uint32_t w[4] = {u.x, u.y, u.z, u.w};
         uint32_t on = 0;
-        if (count == 16 && tok0 + 16 <= end) {      // 16 bytes at once, wherever they lie
-            uint4 u;
-            __builtin_memcpy(&u, mask + tok0, 16);
-            const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t set = ((((w[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[i]) >> 7) & 0x01010101u;      // bytes that are not 0
-                on |= ((set * 0x10204080u) >> 28) << (4 * i);      // its first byte to bit 28, its last to bit 31
-            }
-        } else {
-            for (int e = 0; e < count; ++e)
-                if (tok0 + e < end && mask[tok0 + e] != 0) on |= 1u << e;
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t set = ((((w[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[i]) >> 7) & 0x01010101u;
+            on |= ((set * 0x10204080u) >> 28) << (4 * i);      // the first byte's to bit 28, the last one's to bit 31
         }
         return on;
     }
-    // bit e: this lane's query sees row tok0 + e, one of `count` rows of which those before `end` are there
-    __device__ inline uint32_t visible(int64_t tok0, int count, int64_t end) const {
+    // bits 0 .. count - 1: rows tok0 .. that are before `end` and before this lane's query's limit
+    __device__ inline uint32_t reached(int64_t tok0, int count, int64_t end) const {
         const int64_t left = (end < lim ? end : lim) - tok0;
         const int most = left < count ? (left < 0 ? 0 : (int)left) : count;
-        const uint32_t on = (1u << most) - 1u;
-        return mask ? on & masked(tok0, count, end) : on;
+        return (1u << most) - 1u;
     }
 
     // enters a tile with its largest score mt: the factor for what is there already; `gamma` for what comes
@@ -550,10 +555,11 @@ struct Attend {
     // One tile.  `k` and `v` hold it; MORE: the next tile's take their places as soon as they have been used, K under the softmax and
     // the second product, V under the next tile's first.
     template <bool MORE>
-    __device__ inline void tile(int64_t at, int64_t then, i32x4 (&k)[4][NC], i32x4 (&v)[NJ], bool cut) {
-        const int64_t tok0 = at * 64 + 16 * g, blk = tok0 >> a.shift;
-        const float sk = blk < full ? ks[blk] : 0.f, sv = blk < full ? vs[blk] : 0.f;
-        const float mul = qs * sk;
+    __device__ inline void tile(int64_t at, int64_t then, i32x4 (&k)[4][NC], i32x4 (&v)[NJ], Side& side, bool cut) {
+        const int64_t tok0 = at * 64 + 16 * g;
+        const Side now = side;
+        if (MORE) side = load_side(then);
+        const float sk = now.sk, sv = now.sv, mul = qs * sk;
         float s[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -572,7 +578,8 @@ struct Attend {
         }
         if (MORE) load_k(then, k);
         if (cut) {
-            const uint32_t on = visible(tok0, 16, n_full);
+            uint32_t on = reached(tok0, 16, n_full);
+            if (mask) on &= set_bytes(now.mask);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -653,9 +660,11 @@ struct Attend {
             for (int r = 0; r < 4; ++r) s[i][r] = acc[r] * a.scale;
         }
         const int64_t tok0 = n_full + per * g;
-        const uint32_t on = visible(tok0, per, end);
         const int there = end - tok0 < per ? (end > tok0 ? (int)(end - tok0) : 0) : per;
-        const uint32_t some = ((1u << there) - 1u) & (mask ? masked(tok0, per, end) : ~0u);      // rows that any query may see
+        uint32_t some = (1u << there) - 1u;      // rows that any query may see
+        if (mask)
+            for (int e = 0; e < there; ++e) some &= mask[tok0 + e] != 0 ? ~0u : ~(1u << e);
+        const uint32_t on = reached(tok0, per, end) & some;
         float mt = M_FLOOR;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -771,8 +780,6 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kv8_kernel(AttnArgs a) {
     w.vs = a.c.v_scale + w.bh * w.n_blk;
     w.mask = a.mask ? a.mask + b * a.mask_ld : nullptr;
     w.q = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
-    w.load_query(real);
-
     const int64_t closed = w.n_full < end ? w.n_full : end;      // rows of full blocks that somebody sees
     const int64_t tiles = (closed + 63) >> 6, all = tiles + (end > w.n_full ? 1 : 0);
     const int64_t per = (all + a.n_split - 1) / a.n_split;
@@ -780,13 +787,16 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kv8_kernel(AttnArgs a) {
     const int64_t stop = (split + 1) * per < all ? (split + 1) * per : all, closed_stop = stop < tiles ? stop : tiles;
     if (at < closed_stop) {
         i32x4 k[4][A::NC], v[A::NJ];
+        typename A::Side side = w.load_side(at);
         w.load_k(at, k);
         w.load_v(at, v);
+        w.load_query(real);      // (its wait covers them too)
         auto cut = [&](int64_t t) { return w.mask || t * 64 + 64 > w.n_full || t * 64 + 64 > least; };
-        for (; at + NW < closed_stop; at += NW) w.template tile<true>(at, at + NW, k, v, cut(at));
-        w.template tile<false>(at, 0, k, v, cut(at));
+        for (; at + NW < closed_stop; at += NW) w.template tile<true>(at, at + NW, k, v, side, cut(at));
+        w.template tile<false>(at, 0, k, v, side, cut(at));
         at += NW;
-    }
+    } else
+        w.load_query(real);
     if (at < stop) w.tail(end);
     w.l = sum_over_groups(w.l);
 
