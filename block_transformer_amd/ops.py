@@ -196,6 +196,20 @@ def _at(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
+def _flat(t: torch.Tensor):
+    """(rows, columns, row stride) of a tensor of rows: 2-D with any row stride, or contiguous."""
+    shape = t.shape
+    if len(shape) == 2:
+        M, K = shape
+        ld, one = t.stride()
+        if one == 1 or K == 1:
+            return M, K, ld if M > 1 else K      # (the stride of a single row says nothing)
+    elif len(shape) > 2 and t.is_contiguous():
+        K = shape[-1]
+        return t.numel() // K if K else 0, K, K
+    raise _lib.BtError("expected rows with unit inner stride: 2-D, or contiguous")
+
+
 def _expect(t: torch.Tensor, what: str, shape, dtype) -> None:
     if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise _lib.BtError(f"{what} must be contiguous {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
@@ -205,10 +219,9 @@ def quantize_rows(x: torch.Tensor, ln_w: Optional[torch.Tensor] = None, ln_b: Op
     """(codes, scales) of the rows of ``x`` [..., K] -- of LayerNorm(x; ln_w, ln_b, eps) if weights are given -- in 8-bit integers with one
     scale per row: codes int8 [..., round_up(K, 16)] (zero behind column K), scales float32 [...].  Activations and weights alike:
     ``quantize_rows(weight)`` has one scale per output channel.  A row with an infinity or NaN in it gets scale NaN."""
-    if x.dim() and x.shape[-1] == 0:
+    M, K, ldx = _flat(x)
+    if K == 0:
         raise _lib.BtError("rows are empty")
-    x2, ldx = _rows(x)
-    M, K = x2.shape
     if (ln_w is None) != (ln_b is None):
         raise _lib.BtError("LayerNorm needs ln_w and ln_b")
     for w in (ln_w, ln_b):
@@ -217,9 +230,10 @@ def quantize_rows(x: torch.Tensor, ln_w: Optional[torch.Tensor] = None, ln_b: Op
     Kp = (K + 15) // 16 * 16
     code, index = dtype_code(x.dtype), x.get_device()
     with _on(index, ln_w, ln_b):
-        codes = torch.empty(x.shape[:-1] + (Kp,), dtype=torch.int8, device=x.device)
-        scales = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        check(lib().bt_quant_rows(code, M, K, x2.data_ptr(), ldx, _at(ln_w), _at(ln_b), eps, codes.data_ptr(), Kp, scales.data_ptr(),
+        lead, device = x.shape[:-1], x.device
+        codes = torch.empty(lead + (Kp,), dtype=torch.int8, device=device)
+        scales = torch.empty(lead, dtype=torch.float32, device=device)
+        check(lib().bt_quant_rows(code, M, K, x.data_ptr(), ldx, _at(ln_w), _at(ln_b), eps, codes.data_ptr(), Kp, scales.data_ptr(),
                                   _raw_stream(index)), "bt_quant_rows")
     return codes, scales
 
@@ -246,14 +260,12 @@ def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight:
     code = dtype_code(dtype)
     if xc.dtype != torch.int8 or wc.dtype != torch.int8 or xs.dtype != torch.float32 or ws.dtype != torch.float32:
         raise _lib.BtError("quantised operands are (int8 codes, float32 scales)")
-    a2, lda = _rows(xc)
-    lda = lda if a2.shape[0] > 1 else a2.shape[1]     # the stride of one row says nothing
-    if wc.dim() != 2 or wc.stride(1) != 1:
-        raise _lib.BtError("weight codes must be [N, K] with unit inner stride")
-    M, K = a2.shape
-    N = wc.shape[0]
-    if wc.shape[1] != K:
-        raise _lib.BtError(f"codes of x have {K} columns, those of the weight {wc.shape[1]}")
+    M, K, lda = _flat(xc)
+    if wc.dim() != 2:
+        raise _lib.BtError("weight codes must be [N, K]")
+    N, Kw, ldw = _flat(wc)
+    if Kw != K:
+        raise _lib.BtError(f"codes of x have {K} columns, those of the weight {Kw}")
     if xs.numel() != M or ws.numel() != N or not xs.is_contiguous() or not ws.is_contiguous():
         raise _lib.BtError("one contiguous scale per row of codes is needed")
     if act not in ("none", "gelu"):
@@ -261,24 +273,26 @@ def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight:
     if bias is not None:
         _expect(bias, "bias", (N,), dtype)
     shape = xc.shape[:-1] + (N,)
-    r2, ldr = None, 0
+    ldr = 0
     if residual is not None:
         if residual.shape != shape or residual.dtype != dtype:
             raise _lib.BtError(f"residual must be {dtype} {tuple(shape)}")
-        r2, ldr = _rows(residual)
+        ldr = _flat(residual)[2]
     index = xc.get_device()
     with _on(index, xs, wc, ws, bias, residual, out, scratch):
         if out is None:
             out = torch.empty(shape, dtype=dtype, device=xc.device)
+            ldo = N
         elif out.shape != shape or out.dtype != dtype:
             raise _lib.BtError(f"out must be {dtype} {tuple(shape)}")
-        o2, ldo = _rows(out)
+        else:
+            ldo = _flat(out)[2]
         if scratch is None:
-            need = int(lib().bt_linear_q8_scratch_bytes(M, N, K))
+            need = lib().bt_linear_q8_scratch_bytes(M, N, K)
             if need:
                 scratch = torch.empty(need, dtype=torch.uint8, device=xc.device)
-        check(lib().bt_linear_q8(code, M, N, K, a2.data_ptr(), lda, xs.data_ptr(), wc.data_ptr(), wc.stride(0) if N > 1 else K,
-                                 ws.data_ptr(), _at(bias), _at(r2), ldr, o2.data_ptr(), ldo,
+        check(lib().bt_linear_q8(code, M, N, K, xc.data_ptr(), lda, xs.data_ptr(), wc.data_ptr(), ldw, ws.data_ptr(), _at(bias),
+                                 _at(residual), ldr, out.data_ptr(), ldo,
                                  _lib.BT_ACT_GELU if act == "gelu" else _lib.BT_ACT_NONE, _at(scratch),
                                  0 if scratch is None else scratch.numel() * scratch.element_size(), _raw_stream(index)), "bt_linear_q8")
     return out
@@ -290,16 +304,18 @@ def _kv8(kv: Sequence[torch.Tensor]):
     if kc.dim() != 4 or kt.dim() != 4:
         raise _lib.BtError("a layer of an 8-bit cache is (k_codes, v_codes, k_scale, v_scale, k_tail, v_tail), see runtime.KV8Cache")
     B, H, n_max, d = kc.shape
-    block = kt.shape[2]
+    block, dtype = kt.shape[2], kt.dtype
     if block == 0 or n_max % block:
         raise _lib.BtError(f"{n_max} rows are not a whole number of blocks of {block}")
-    for t, what, shape, dtype in ((kc, "k_codes", (B, H, n_max, d), torch.int8), (vc, "v_codes", (B, H, n_max // block, d, block), torch.int8),
-                                  (ks, "k_scale", (B, H, n_max // block), torch.float32), (vs, "v_scale", ks.shape, torch.float32),
-                                  (kt, "k_tail", (B, H, block, d), kt.dtype), (vt, "v_tail", (B, H, d, block), kt.dtype)):
-        if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
-            _expect(t, what, shape, dtype)
+    blocks = n_max // block
+    _expect(kc, "k_codes", (B, H, n_max, d), torch.int8)
+    _expect(vc, "v_codes", (B, H, blocks, d, block), torch.int8)
+    _expect(ks, "k_scale", (B, H, blocks), torch.float32)
+    _expect(vs, "v_scale", (B, H, blocks), torch.float32)
+    _expect(kt, "k_tail", (B, H, block, d), dtype)
+    _expect(vt, "v_tail", (B, H, d, block), dtype)
     return (_lib.bt_kv8_cache(block, H, d, B, n_max, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt.data_ptr(),
-                              vt.data_ptr()), dtype_code(kt.dtype))
+                              vt.data_ptr()), dtype_code(dtype))
 
 
 def _kv8_rows(t: torch.Tensor, what: str, batch: int, q_len: int, d: int, dtype):
