@@ -5,6 +5,31 @@
 
 namespace bt {
 
+// Sum and maximum over the four lanes c, c + 16, c + 32, c + 48, in all of them: two lane swaps of gfx950, no LDS.
+__device__ inline float max_over_groups(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ inline float sum_over_groups(float x) {
+    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+// over all 64 lanes, the 16 of a row by DPP: ten instructions instead of six round trips through LDS
+__device__ inline float sum64(float x) { return sum_over_groups(row16_sum_dpp(x)); }
+__device__ inline float max64(float x) {
+#define BT_MAX_DPP(ctrl) x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, 0xf, 0xf, false)))
+    BT_MAX_DPP(0x128);      // row_ror:8, row_ror:4, quad_perm [2,3,0,1], quad_perm [1,0,3,2]
+    BT_MAX_DPP(0x124);
+    BT_MAX_DPP(0x4e);
+    BT_MAX_DPP(0xb1);
+#undef BT_MAX_DPP
+    return max_over_groups(x);
+}
+
 // s = fl32(amax / 127), code(x) = clamp(round_half_even(x / s), -127, 127) with the quotient taken exactly, without a division per
 // value.
 //   exact():  y = x * fl32(1 / s) is within 3 * 2^-24 |y| < 3e-5 of x / s, so with h = floor(y) + 1/2 the quotient lies in (h - 1, h + 1)

@@ -98,7 +98,7 @@ struct BlockMax {
         float m = 0.f;
 #pragma unroll
         for (int i = 0; i < N; ++i) m = fmaxf(m, fabsf(v[i]) < INFINITY ? fabsf(v[i]) : 0.f);
-        return wave_max(m);
+        return max64(m);
     }
 };
 
@@ -194,7 +194,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
                 }
             }
             const bool odd = top.odd();
-            float amax = wave_max(top.amax);
+            float amax = max64(top.amax);
             if (odd) {
                 amax = 0.f;
 #pragma unroll
@@ -257,7 +257,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
                 }
             }
             const bool odd = top.odd();
-            float amax = wave_max(top.amax);
+            float amax = max64(top.amax);
             if (odd) {
                 amax = 0.f;
 #pragma unroll
@@ -410,20 +410,6 @@ struct AttnArgs {
 };
 
 constexpr float M_FLOOR = -1e30f;      // "no score yet": finite, so that differences of two of them are 0
-
-// the largest over the four lanes c, c + 16, c + 32, c + 48, in all of them
-__device__ inline float max_over_groups(float x) {
-    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
-    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
-}
-__device__ inline float sum_over_groups(float x) {
-    auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
-    auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
-}
 
 template <typename T, int D>
 struct Attend {
@@ -873,7 +859,7 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(AttnArgs a) {
     const float* p = a.part + (int64_t)blockIdx.x * a.n_split * (D + 2);
     float m = M_FLOOR;
     for (int s = tid; s < a.n_split; s += 256) m = fmaxf(m, p[(int64_t)s * (D + 2) + D]);
-    m = wave_max(m);
+    m = max64(m);
     if ((tid & 63) == 0) most[tid >> 6] = m;
     __syncthreads();
     m = fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3]));

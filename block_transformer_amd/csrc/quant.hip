@@ -18,7 +18,7 @@ struct RowReduce {      // over the R waves of a row (R = 4: the workgroup)
     float* slot;
     int wave;
     __device__ inline float sum(float v) {
-        v = wave_sum(v);
+        v = sum64(v);
         if (R == 1) return v;
         __syncthreads();
         if ((threadIdx.x & 63) == 0) slot[wave] = v;
@@ -26,7 +26,7 @@ struct RowReduce {      // over the R waves of a row (R = 4: the workgroup)
         return slot[0] + slot[1] + slot[2] + slot[3];
     }
     __device__ inline float max(float v) {
-        v = wave_max(v);
+        v = max64(v);
         if (R == 1) return v;
         __syncthreads();
         if ((threadIdx.x & 63) == 0) slot[wave] = v;
@@ -69,12 +69,21 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
         const float mean = all.sum(sum) / (float)K;
         float sq = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+        for (int i = 0; i < NV; ++i) {
+            const int c = (i * 64 * R + at) * V;
+            float part = 0.f;
 #pragma unroll
             for (int e = 0; e < V; ++e) {
                 v[i][e] -= mean;
-                if ((i * 64 * R + at) * V + e < K) sq = fmaf(v[i][e], v[i][e], sq);
+                part = fmaf(v[i][e], v[i][e], part);
             }
+            if (c + V > K) {      // what lies behind the row does not count
+                part = 0.f;
+#pragma unroll
+                for (int e = 0; e < V; ++e) part = c + e < K ? fmaf(v[i][e], v[i][e], part) : part;
+            }
+            sq += part;
+        }
         const float rstd = rsqrtf(all.sum(sq) / (float)K + eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -86,17 +95,15 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
             for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, wv[e], bv[e]);      // 0 beyond K, as wv and bv are
         }
     }
-    float amax = 0.f;
-    bool odd = false;
+    float amax = 0.f, zero = 0.f;      // (0 * v is 0 unless v is an infinity or NaN)
 #pragma unroll
     for (int i = 0; i < NV; ++i)
 #pragma unroll
         for (int e = 0; e < V; ++e) {
-            if (LN && v[i][e] != v[i][e] && (i * 64 * R + at) * V + e >= K) v[i][e] = 0.f;      // (0 * an infinite rstd)
             amax = fmaxf(amax, fabsf(v[i][e]));
-            odd |= !(fabsf(v[i][e]) < INFINITY);
+            zero = fmaf(v[i][e], 0.f, zero);
         }
-    amax = all.max(odd ? INFINITY : amax);
+    amax = all.max(zero == 0.f ? amax : INFINITY);
     const bool bad = amax == INFINITY;
     const Quantiser q(bad ? 0.f : amax);
     if (at == 0) scales[row] = bad ? __int_as_float(0x7fc00000) : q.scale;
