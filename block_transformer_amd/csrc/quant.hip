@@ -221,6 +221,7 @@ struct Q8Args {
     int64_t ldo;
     int act;
     int wide;           // out (and residual) take 16-byte accesses
+    int fours;          // w_scale and bias give four columns at a time
     int tiles_m, tiles_n;
     int slices, steps;  // K split into `slices` ranges of `steps` 64-byte steps; > 1: sums go to `slab`
     int* slab;          // [slices][M][N]
@@ -250,50 +251,72 @@ __device__ inline void wait_loads() {
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"(N) : "memory");
 }
 
-// The tile of this workgroup.  Workgroups of one XCD (ids that are equal mod 8) take neighbouring tiles, in columns of HIGH tile rows: its
-// L2 serves them with each other's panels.
+// Tile number `round` of this workgroup, of those that `groups` workgroups take a round at a time; false: there is none.  Workgroups of one
+// XCD (ids that are equal mod 8) take neighbouring tiles, in columns of HIGH tile rows: its L2 serves them with each other's panels.
 template <int HIGH>
-__device__ inline void q8_tile(const Q8Args& e, int& tm, int& tn) {
-    const int tiles = e.tiles_m * e.tiles_n, id = blockIdx.x;
+__device__ inline bool q8_tile(const Q8Args& e, int groups, int round, int& tm, int& tn) {
+    const int base = round * groups, tiles = min(e.tiles_m * e.tiles_n - base, groups), id = blockIdx.x;
     const int per = tiles >> 3, rest = tiles & 7, xcd = id & 7, local = id >> 3;
-    const int at = (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + local;
+    if (tiles <= 0 || local >= per + (xcd < rest)) return false;
+    const int at = base + (xcd < rest ? xcd * (per + 1) : rest * (per + 1) + (xcd - rest) * per) + local;
     const int group = at / (HIGH * e.tiles_n), first = group * HIGH, high = min(e.tiles_m - first, HIGH), in = at - group * HIGH * e.tiles_n;
     tm = first + in % high;
     tn = in / high;
+    return true;
 }
 
-constexpr int q8_pitch(int nb, int size) { return 16 * nb * size + 16; }      // bytes of a row of a wave's patch: its 16 NB columns
+constexpr int q8_pitch(int nb) { return 16 * nb * 2 + 16; }      // bytes of a row of a wave's bf16 patch: its 16 NB columns
 
 // The sums of a wave, NI fragments of 16 rows (row0(i) is the first of fragment i) by 16 NB columns from n_w: lane (c, g) has columns
-// 16 j + 4 g .. + 3 of row c.  Scales, bias, activation and residual there, then one rounding; the rows are put together in `patch` (16
-// rows, the wave's own) and leave as 16-byte pieces.
+// 16 j + 4 g .. + 3 of row c.  Scales, bias, activation and residual there, then one rounding.  fp32 leaves from there, 16 bytes a lane;
+// bf16 rows are put together in `patch` (16 rows, the wave's own) first.  A tile that is whole and `wide` takes 2 NI (bf16) or NI NB stores
+// of NB = 4.
 template <typename T, int NI, int NB, typename Row0>
-__device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], char* patch, int n_w, Row0 row0) {
-    constexpr int PITCH = q8_pitch(NB, sizeof(T));
-    const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+__device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], char* patch, int n_w, int lane, Row0 row0) {
+    constexpr int PITCH = q8_pitch(NB);
+    const int c = lane & 15, g = lane >> 4;
     // every load of scales and bias at once, and the residual's one fragment ahead: a load that is waited for costs a microsecond here
     float sa[NI], sw[NB][4], bias[NB][4];
 #pragma unroll
     for (int i = 0; i < NI; ++i) sa[i] = e.a_scale[min(row0(i) + c, e.M - 1)];
+    const bool fours = e.fours && n_w + 16 * NB <= e.N;
 #pragma unroll
     for (int j = 0; j < NB; ++j) {
         const int n = n_w + j * 16 + g * 4;
+        if (fours) {
+            const float4 s4 = *(const float4*)(e.w_scale + n);
+            sw[j][0] = s4.x, sw[j][1] = s4.y, sw[j][2] = s4.z, sw[j][3] = s4.w;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            sw[j][r] = e.w_scale[min(n + r, e.N - 1)];
-            bias[j][r] = e.bias ? Elem<T>::load((const T*)e.bias + min(n + r, e.N - 1)) : 0.f;
-        }
+            for (int r = 0; r < 4; ++r) bias[j][r] = 0.f;
+            if (e.bias) {
+                if constexpr (sizeof(T) == 2) {
+                    const uint2 u = *(const uint2*)((const T*)e.bias + n);
+                    bias[j][0] = __uint_as_float(u.x << 16), bias[j][1] = __uint_as_float(u.x & 0xffff0000u);
+                    bias[j][2] = __uint_as_float(u.y << 16), bias[j][3] = __uint_as_float(u.y & 0xffff0000u);
+                } else {
+                    const float4 u = *(const float4*)((const T*)e.bias + n);
+                    bias[j][0] = u.x, bias[j][1] = u.y, bias[j][2] = u.z, bias[j][3] = u.w;
+                }
+            }
+        } else
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                sw[j][r] = e.w_scale[min(n + r, e.N - 1)];
+                bias[j][r] = e.bias ? Elem<T>::load((const T*)e.bias + min(n + r, e.N - 1)) : 0.f;
+            }
     }
+    // the wave's part of a tile that is whole, in 16-byte pieces: no test a row, and a row's address is a scalar and one lane offset
+    const bool whole = e.wide && row0(NI - 1) + 16 <= e.M && n_w + 16 * NB <= e.N;
     typedef typename std::conditional<sizeof(T) == 2, uint2, float4>::type Four;
     Four next[NB] = {};
     auto load_residual = [&](int i) {
         const int m = row0(i) + c;
         if (!e.residual || m >= e.M) return;
-        const T* p = (const T*)e.residual + (int64_t)m * e.ldr + n_w + g * 4;
+        const T* p = (const T*)e.residual + (int64_t)row0(i) * e.ldr + n_w + (uint32_t)(c * (int)e.ldr + g * 4);
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int n = n_w + j * 16 + g * 4;
-            if (e.wide && n + 4 <= e.N) next[j] = *(const Four*)(p + j * 16);
+            if (whole) next[j] = *(const Four*)(p + j * 16);
             else {
                 T v[4] = {};
 #pragma unroll
@@ -322,23 +345,33 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
                     y[0] += res[j].x, y[1] += res[j].y, y[2] += res[j].z, y[3] += res[j].w;
                 }
             }
-            if constexpr (sizeof(T) == 2) *(uint2*)(patch + c * PITCH + (j * 16 + g * 4) * 2) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
-            else *(float4*)(patch + c * PITCH + (j * 16 + g * 4) * 4) = float4{y[0], y[1], y[2], y[3]};
+            if constexpr (sizeof(T) == 2) {
+                *(uint2*)(patch + c * PITCH + (j * 16 + g * 4) * 2) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
+            } else {
+                T* out = (T*)e.out + (int64_t)row0(i) * e.ldo + n_w + (uint32_t)(c * (int)e.ldo + g * 4) + j * 16;
+                if (whole) *(u32x4_t*)out = u32x4_t{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])};
+                else if (row0(i) + c < e.M)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (n_w + j * 16 + g * 4 + r < e.N) out[r] = y[r];
+            }
         }
+        if constexpr (sizeof(T) == 4) continue;
         asm volatile("" ::: "memory");      // the patch is the wave's own, and a wave's LDS accesses stay in order
         constexpr int V = Elem<T>::VEC, CH = 16 * NB / V;      // 16-byte pieces of a row
 #pragma unroll
         for (int x = 0; x < 16 * CH; x += 64) {
-            const int r = (x + lane) / CH, d = ((x + lane) - r * CH) * V, mm = row0(i) + r, n = n_w + d;
-            if (mm >= e.M || n >= e.N) continue;
-            float y[V];
-            load_vec<T>((const T*)(patch + r * PITCH) + d, y);
-            T* out = (T*)e.out + (int64_t)mm * e.ldo + n;
-            if (e.wide && n + V <= e.N) store_vec<T>(out, y);
-            else
+            const int r0 = x / CH, r = lane / CH, d = (lane - r * CH) * V;      // (64 is a multiple of CH)
+            const u32x4_t v = *(const u32x4_t*)(patch + (r0 + r) * PITCH + d * sizeof(T));
+            T* out = (T*)e.out + (int64_t)(row0(i) + r0) * e.ldo + n_w + (uint32_t)(r * (int)e.ldo + d);
+            if (whole) *(u32x4_t*)out = v;
+            else if (row0(i) + r0 + r < e.M) {
+                T y[V];
+                __builtin_memcpy(y, &v, sizeof v);
 #pragma unroll
                 for (int q = 0; q < V; ++q)
-                    if (n + q < e.N) Elem<T>::store(out + q, y[q]);
+                    if (n_w + d + q < e.N) out[q] = y[q];
+            }
         }
         asm volatile("" ::: "memory");
     }
@@ -358,14 +391,14 @@ template <typename T, int MI, int NB, int NS>
 __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
     constexpr int BM = 32 * MI, BN = 32 * NB, STAGE = (BM + BN) * 64;
     constexpr int LA = BM / 64, LW = BN / 64, LOADS = LA + LW;      // 1 KiB loads of a wave and step
-    constexpr int PITCH = q8_pitch(NB, sizeof(T));
-    constexpr int RING = NS * STAGE, PATCH = 4 * 16 * PITCH;
-    __shared__ __attribute__((aligned(16))) char smem[RING > PATCH ? RING : PATCH];
+    constexpr int PITCH = q8_pitch(NB);
+    static_assert(4 * 16 * PITCH <= NS * STAGE, "the patches take the ring's place");
+    __shared__ __attribute__((aligned(16))) char smem[NS * STAGE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 1, wn = wave & 1, c = lane & 15, g = lane >> 4;
 
     int m0, n0;
-    q8_tile<8>(e, m0, n0);
+    q8_tile<8>(e, gridDim.x, 0, m0, n0);
     m0 *= BM;
     n0 *= BN;
     const int k0 = blockIdx.y * e.steps * 64, steps = min(e.steps, (e.K - k0 + 63) >> 6);
@@ -454,7 +487,7 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
         return;
     }
     __syncthreads();      // the ring is the patches' now
-    q8_write<T, MI, NB>(e, acc, smem + wave * 16 * PITCH, n_w, [&](int i) { return m_w + i * 16; });
+    q8_write<T, MI, NB>(e, acc, smem + wave * 16 * PITCH, n_w, lane, [&](int i) { return m_w + i * 16; });
 }
 
 // The kernel for the largest products: 256 x 256 per workgroup of eight waves, 128 bytes of K a step, K % 128 == 0.  What bounds a large
@@ -467,129 +500,171 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
 //  * A step has two phases, one for each half (128 rows) of A; W's fragments are read in the first and kept.  LDS holds two steps of four
 //    half tiles (A0, W0, W1, A1: in the order in which they are wanted).  Phase (t, 0) sends W1 and A1 of step t + 1, phase (t, 1) sends A0
 //    and W0 of step t + 2 into the places that phase (t, 0) has read.
-//  * Before phase (t, 0) a wave has sent 6 + 4 t half tiles and needs the first 4 t + 3 of them, before (t, 1) 8 + 4 t and 4 t + 4: at most 3
-//    and 4 half tiles, of two loads each, may be on their way; in the last step nothing is.  Group 0 waits at the top of a phase, group 1
-//    for the next phase's before its second barrier, which is the one that opens that phase to group 0.
+//  * A workgroup stays for all its tiles, and the loads run on from one tile into the next: when a tile's sums are finished, the next
+//    one's first two steps are on their way or there, so its products start behind the epilogue without a wait, and the epilogue's stores
+//    drain under them.
+//  * Waits are for all but the youngest loads (they return in order).  In front of phase (t, 0) what may still be out is A1 of the step
+//    and A0, W0 of the next: 6 loads (a half tile is two); in front of (t, 1), the whole next step: 8.  In a tile's first step W1 and A1
+//    of the next are out too (they went ahead of the epilogue): 10 and 8.  In the first two steps of a tile the stores of the one before
+//    are younger than the loads in question and are counted as well, if that tile was whole (else their number varies, and the wait is
+//    for them too).  In the last step of all, for everything.  Group 0 waits at the top of a phase, group 1 for the next phase's before its
+//    second barrier, which is the one that opens that phase to group 0.
 //  * A wave's reads have returned before its second barrier of a phase; the other group sends the loads that overwrite those places behind
 //    that barrier.
+//  * A tile ends with one more barrier for group 0 (group 1 has then read its last) and begins with one more for group 1, so the two
+//    epilogues run side by side.
 //  * A row of 128 bytes has its 16-byte pieces in the order p ^ (row & 7).
 template <typename T>
 __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
-    constexpr int HALF = 128 * 128, STEP = 4 * HALF, PITCH = q8_pitch(4, sizeof(T));
-    static_assert(8 * 16 * PITCH <= 2 * STEP, "the patches take the ring's place");
-    __shared__ __attribute__((aligned(16))) char smem[2 * STEP];
+    constexpr int HALF = 128 * 128, STEP = 4 * HALF, PITCH = q8_pitch(4), PATCH = sizeof(T) == 2 ? 16 * PITCH : 0;
+    constexpr int STORES = sizeof(T) == 2 ? 16 : 32;      // of a wave and whole tile
+    __shared__ __attribute__((aligned(16))) char smem[2 * STEP + 8 * PATCH];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 2, wn = wave & 3, c = lane & 15, g = lane >> 4;
     const bool second = wm != 0;
-    int m0, n0;
-    q8_tile<4>(e, m0, n0);
-    m0 *= 256;
-    n0 *= 256;
     const int steps = e.K >> 7;
-    const int8_t* A = e.A + (int64_t)m0 * e.lda;
-    const int8_t* W = e.W + (int64_t)n0 * e.ldw;
+
+    // the loads: step `lt` of tile number `lround`, the `lx`-th step of all
+    int lm = 0, ln = 0, lt = 0, lround = 0, lx = 0;
+    bool more = true;
+    const int8_t *A = nullptr, *W = nullptr;
     uint32_t off[4][2];      // [half tile][load]
+    auto enter = [&] {
+        more = q8_tile<4>(e, gridDim.x, lround, lm, ln);
+        if (!more) return;
+        A = e.A + (int64_t)lm * 256 * e.lda;
+        W = e.W + (int64_t)ln * 256 * e.ldw;
 #pragma unroll
-    for (int h = 0; h < 4; ++h)
+        for (int h = 0; h < 4; ++h)
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const bool a = h == 0 || h == 3;
-            int row = (h >= 2 ? 128 : 0) + wave * 16 + i * 8 + (lane >> 3);
-            const int last = a ? e.M - 1 - m0 : e.N - 1 - n0;      // rows beyond the matrix repeat its last one
-            row = row < last ? row : last;
-            off[h][i] = (uint32_t)row * (uint32_t)(a ? e.lda : e.ldw) + (uint32_t)((lane & 7) ^ (lane >> 3)) * 16;
-        }
+            for (int i = 0; i < 2; ++i) {
+                const bool a = h == 0 || h == 3;
+                int row = (h >= 2 ? 128 : 0) + wave * 16 + i * 8 + (lane >> 3);
+                const int last = a ? e.M - 1 - lm * 256 : e.N - 1 - ln * 256;      // rows beyond the matrix repeat its last one
+                row = row < last ? row : last;
+                off[h][i] = (uint32_t)row * (uint32_t)(a ? e.lda : e.ldw) + (uint32_t)((lane & 7) ^ (lane >> 3)) * 16;
+            }
+    };
     const uint32_t ring = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)smem + wave * 2048;
-    auto load = [&](int t, auto half) {      // half tile `half` of step t
+    auto load = [&](auto half) {
         constexpr int h = decltype(half)::value;
-        if (t >= steps) return;
-        const int8_t* base = (h == 0 || h == 3 ? A : W) + (int64_t)t * 128;
-        dma16(base, off[h][0], ring + (t & 1) * STEP + h * HALF);
-        dma16(base, off[h][1], ring + (t & 1) * STEP + h * HALF + 1024);
+        if (!more) return;
+        const int8_t* base = h == 0 || h == 3 ? A : W;
+        dma16(base, off[h][0], ring + (lx & 1) * STEP + h * HALF);
+        dma16(base, off[h][1], ring + (lx & 1) * STEP + h * HALF + 1024);
     };
     using H0 = std::integral_constant<int, 0>;
     using H1 = std::integral_constant<int, 1>;
     using H2 = std::integral_constant<int, 2>;
     using H3 = std::integral_constant<int, 3>;
+    auto first_half = [&] { load(H0{}); load(H1{}); };
+    auto second_half = [&] {
+        load(H2{});
+        load(H3{});
+        ++lx;
+        A += 128;
+        W += 128;
+        if (++lt == steps) {
+            lt = 0;
+            ++lround;
+            if (more) enter();
+        }
+    };
     auto barrier = [] {
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
-    load(0, H0{}); load(0, H1{}); load(0, H2{}); load(0, H3{});
-    load(1, H0{}); load(1, H1{});
-    i32x4 acc[8][4];
+    enter();
+    first_half(); second_half();
+    first_half(); second_half();
+
+    int m0, n0, x = 0;      // the tile, and the number of steps of all that are done
+    bool stores = false;    // the tile before has left STORES stores behind the loads of this one's first two steps
+    for (int round = 0; q8_tile<4>(e, gridDim.x, round, m0, n0); ++round) {
+        m0 *= 256;
+        n0 *= 256;
+        i32x4 acc[8][4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < 8; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-    auto wait_first = [&](int t) {      // for phase (t, 0)
-        if (t < steps - 1) wait_loads<6>();
-        else wait_loads<0>();
-    };
-    auto wait_second = [&](int t) {     // for phase (t, 1)
-        if (t < steps - 1) wait_loads<8>();
-        else wait_loads<0>();
-    };
-    if (second) {
-        wait_first(0);
-        barrier();
-    }
-    const int p0 = (g ^ (c & 7)) * 16, p1 = ((4 + g) ^ (c & 7)) * 16;      // this lane's pieces of a row: the step's first and second 64 bytes
-    i32x4 af[4][2], wf[4][2];
-    for (int t = 0; t < steps; ++t) {
-        const char* step = smem + (t & 1) * STEP;
-        const char* a = step + (wm * 64 + c) * 128;
-        const char* w = step + (wn >> 1 ? 2 : 1) * HALF + ((wn & 1) * 64 + c) * 128;
-        // phase 0
-        if (!second) wait_first(t);
-        barrier();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            wf[j][0] = *(const i32x4*)(w + j * 2048 + p0);
-            af[j][0] = *(const i32x4*)(a + j * 2048 + p0);
+            for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+        int nm, nn;
+        const bool last_tile = !q8_tile<4>(e, gridDim.x, round + 1, nm, nn);
+        auto wait_first = [&](int t) {      // for phase (t, 0)
+            if (last_tile && t == steps - 1) wait_loads<0>();
+            else if (t == 0 && stores) wait_loads<10 + STORES>();
+            else if (t == 0) wait_loads<10>();
+            else if (t == 1 && stores) wait_loads<6 + STORES>();
+            else wait_loads<6>();
+        };
+        auto wait_second = [&](int t) {     // for phase (t, 1)
+            if (last_tile && t == steps - 1) wait_loads<0>();
+            else if (t <= 1 && stores) wait_loads<8 + STORES>();
+            else wait_loads<8>();
+        };
+        if (second) {
+            wait_first(0);
+            barrier();
         }
+        const int p0 = (g ^ (c & 7)) * 16, p1 = ((4 + g) ^ (c & 7)) * 16;      // this lane's pieces of a row: the step's first and second 64 bytes
+        i32x4 af[4][2], wf[4][2];
+        for (int t = 0; t < steps; ++t, ++x) {
+            const char* step = smem + (x & 1) * STEP;
+            const char* a = step + (wm * 64 + c) * 128;
+            const char* w = step + (wn >> 1 ? 2 : 1) * HALF + ((wn & 1) * 64 + c) * 128;
+            // phase 0
+            if (!second) wait_first(t);
+            barrier();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            wf[j][1] = *(const i32x4*)(w + j * 2048 + p1);
-            af[j][1] = *(const i32x4*)(a + j * 2048 + p1);
+            for (int j = 0; j < 4; ++j) {
+                wf[j][0] = *(const i32x4*)(w + j * 2048 + p0);
+                af[j][0] = *(const i32x4*)(a + j * 2048 + p0);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                wf[j][1] = *(const i32x4*)(w + j * 2048 + p1);
+                af[j][1] = *(const i32x4*)(a + j * 2048 + p1);
+            }
+            if (t > 0) second_half();
+            if (second) wait_second(t);
+            __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
+            barrier();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            // phase 1
+            if (!second) wait_second(t);
+            barrier();
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) af[i][k] = *(const i32x4*)(a + 3 * HALF + i * 2048 + (k ? p1 : p0));
+            first_half();
+            if (second && t + 1 < steps) wait_first(t + 1);
+            __builtin_amdgcn_s_waitcnt(0xc07f);
+            barrier();
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) acc[4 + i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[4 + i][j], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        load(t + 1, H2{});
-        load(t + 1, H3{});
-        if (second) wait_second(t);
-        __builtin_amdgcn_s_waitcnt(0xc07f);      // lgkmcnt(0)
-        barrier();
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[i][j], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-        // phase 1
-        if (!second) wait_second(t);
-        barrier();
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) af[i][k] = *(const i32x4*)(a + 3 * HALF + i * 2048 + (k ? p1 : p0));
-        load(t + 2, H0{});
-        load(t + 2, H1{});
-        if (second && t + 1 < steps) wait_first(t + 1);
-        __builtin_amdgcn_s_waitcnt(0xc07f);
-        barrier();
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[4 + i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[4 + i][j], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
+        if (!second) barrier();      // group 1 has read its last fragments
+        second_half();
+        int hide = lane;
+        asm volatile("" : "+v"(hide));      // the epilogue's addresses are not to be kept in registers through the products
+        q8_write<T, 8, 4>(e, acc, smem + 2 * STEP + wave * PATCH, n0 + wn * 64, hide, [&](int i) { return m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16; });
+        stores = e.wide && m0 + 256 <= e.M && n0 + 256 <= e.N;
     }
-    if (!second) barrier();      // group 1 has read its last fragments: the ring is the patches' now
-    q8_write<T, 8, 4>(e, acc, smem + wave * 16 * PITCH, n0 + wn * 64, [&](int i) { return m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16; });
 }
 
 // Few rows: 16 MB rows by 16 NB columns per workgroup, the waves dividing K among themselves.  W is read once, straight into the operand
@@ -760,7 +835,7 @@ static int launch_linear_q8(Q8Args& e, int64_t scratch_bytes, hipStream_t s) {
         case Q8Plan::BIG:
             e.tiles_m = (int)ceil_div(e.M, 256);
             e.tiles_n = (int)ceil_div(e.N, 256);
-            hipLaunchKernelGGL((linear_q8_big_kernel<T>), dim3((unsigned)(e.tiles_m * e.tiles_n)), dim3(512), 0, s, e);
+            hipLaunchKernelGGL((linear_q8_big_kernel<T>), dim3((unsigned)std::min(e.tiles_m * e.tiles_n, 256)), dim3(512), 0, s, e);
             break;
     }
     BT_LAUNCH_CHECK("bt_linear_q8 launch");
@@ -804,6 +879,7 @@ extern "C" int bt_linear_q8(int dtype, int64_t M, int64_t N, int64_t K, const in
     BT_CHECK_ARG(lda >= K && ldw >= K && lda % 16 == 0 && ldw % 16 == 0 && aligned16(A) && aligned16(W),
                  "bt_linear_q8: rows of codes must be 16-byte granular");
     BT_CHECK_ARG(ldo >= N && (!residual || ldr >= N), "bt_linear_q8: row stride smaller than row");
+    BT_CHECK_ARG(ldo < (1 << 26) && ldr < (1 << 26), "bt_linear_q8: row stride too large");      // (16 rows within 32 bits)
     BT_CHECK_ARG(act == BT_ACT_NONE || act == BT_ACT_GELU, "bt_linear_q8: bad act %d", act);
     BT_CHECK_ARG(!scratch || (scratch_bytes >= 0 && aligned16(scratch)), "bt_linear_q8: scratch must be 16-byte aligned");
     Q8Args e{};
@@ -824,6 +900,7 @@ extern "C" int bt_linear_q8(int dtype, int64_t M, int64_t N, int64_t K, const in
     e.act = act;
     const int V = dtype == BT_BF16 ? 8 : 4;
     e.wide = aligned16(out) && ldo % V == 0 && (!residual || (aligned16(residual) && ldr % V == 0));
+    e.fours = aligned16(w_scale) && aligned16(bias);
     e.slab = (int*)scratch;
     if (!scratch) scratch_bytes = 0;
     return dtype == BT_BF16 ? launch_linear_q8<bf16>(e, scratch_bytes, (hipStream_t)stream)

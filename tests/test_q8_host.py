@@ -56,6 +56,7 @@ def test_linear_q8_refusals():
     refused(call(A=P + 4), "16-byte granular")
     refused(call(ldo=7), "row stride")
     refused(call(residual=P, ldr=7), "row stride")
+    refused(call(ldo=1 << 26), "too large")
     refused(call(act=2), "act")
     refused(call(scratch=P + 8, scratch_bytes=64), "scratch")
     assert call(M=0) == 0
