@@ -108,8 +108,10 @@ struct BlockMax {
 //   V: a lane has columns 2 x, 2 x + 1 of 16 rows, that is two 16-byte runs of v_codes: rows are read 256 bytes a wave and instruction,
 //      and no transpose is needed.  Rows of the open block come in runs from v_tail, which is transposed already.
 // Bound by memory; K and V are held in registers between the search for the scale and the codes, V's loads go out before K's work.
+constexpr int QU = 2;
+
 template <typename T, int D, int BL>
-__global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(256, D * BL <= 2048 ? 4 : D * BL <= 4096 ? 3 : 1) void kv8_append_kernel(AppendArgs a) {
     constexpr int V = Elem<T>::VEC, RP = D / V, LR = RP / 4;      // pieces of a row, lanes to a row
     const int lane = threadIdx.x & 63;
     const int pos0 = a.pos0_dev ? *a.pos0_dev : a.pos0_host;
@@ -117,25 +119,44 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(AppendArgs a) {
     const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int e_lane = lane % LR * V;      // piece k of this lane: dims e_lane + k D / 4
     if (item >= a.kv_items) {
-        const uint32_t i = (item - a.kv_items) * (64 / LR) + lane / LR;      // row (b, t, h) of q
-        if (i >= a.q_rows) return;
-        const uint32_t bt = i / (uint32_t)a.heads, b = bt / (uint32_t)a.q_len;
-        const int h = (int)(i - bt * a.heads), t = (int)(bt - b * a.q_len);
-        const T* src = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
-        T* dst = (T*)a.q_out.p + b * a.q_out.b + t * a.q_out.t + h * a.q_out.h;
-        const int64_t ang = angle_of(a, pos0 + t);
-        float v[4][V];
+        // QU rows (b, t, h) of q a lane, their loads out together.  The last workgroup has waves too many, without q all of these are.
+        const uint32_t i0 = (item - a.kv_items) * (QU * 64 / LR);
+        if (i0 >= a.q_rows) return;
+        const T* src[QU];
+        T* dst[QU];
+        int pos[QU];
+        bool there[QU];
+        float v[QU][4][V];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) rotated_piece<T>(a, src, e_lane + k * (D / 4), ang, v[k]);
+        for (int u = 0; u < QU; ++u) {
+            uint32_t i = i0 + u * (64 / LR) + lane / LR;
+            there[u] = i < a.q_rows;
+            i = there[u] ? i : a.q_rows - 1;
+            const uint32_t bt = i / (uint32_t)a.heads, b = bt / (uint32_t)a.q_len;
+            const int h = (int)(i - bt * a.heads), t = (int)(bt - b * a.q_len);
+            src[u] = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
+            dst[u] = (T*)a.q_out.p + b * a.q_out.b + t * a.q_out.t + h * a.q_out.h;
+            pos[u] = pos0 + t;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) load_vec<T>(src[u] + e_lane + k * (D / 4), v[u][k]);
+        }
+#pragma unroll
+        for (int u = 0; u < QU; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (e_lane + k * (D / 4) < a.rot) rotated_piece<T>(a, src[u], e_lane + k * (D / 4), angle_of(a, pos[u]), v[u][k]);
         asm volatile("" ::: "memory");      // q_out may be q: every lane of the row has read before one writes
 #pragma unroll
-        for (int k = 0; k < 4; ++k) store_vec<T>(dst + e_lane + k * (D / 4), v[k]);
+        for (int u = 0; u < QU; ++u)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+                if (there[u]) store_vec<T>(dst[u] + e_lane + k * (D / 4), v[u][k]);
         return;
     }
-    const uint32_t bh = item / (uint32_t)a.blocks;
-    const int nth = (int)(item - bh * a.blocks);
-    const uint32_t b = bh / (uint32_t)a.c.kv_heads;
-    const int h = (int)(bh - b * a.c.kv_heads);
+    // neighbouring waves take neighbouring heads: of a fused projection's rows they read one piece of memory
+    const uint32_t bn = item / (uint32_t)a.c.kv_heads, b = bn / (uint32_t)a.blocks;
+    const int h = (int)(item - bn * a.c.kv_heads), nth = (int)(bn - b * a.blocks);
+    const uint32_t bh = b * a.c.kv_heads + h;
     const int64_t end = pos0 + (int64_t)a.q_len < a.c.n_max ? pos0 + (int64_t)a.q_len : a.c.n_max;
     const T* ksrc = (const T*)a.k.p + b * a.k.b + h * a.k.h;
     const T* vsrc = (const T*)a.v.p + b * a.v.b + h * a.v.h;
@@ -978,7 +999,7 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.max_pos = max_pos;
     const int V = dtype == BT_BF16 ? 8 : 4;
     a.vec_rope = (rot / 2) % V == 0 && aligned16(cos_tab) && aligned16(sin_tab);
-    const int64_t waves = kv_items + ceil_div(q_rows * cache->head_dim, 256 * V);
+    const int64_t waves = kv_items + ceil_div(q_rows * cache->head_dim, 256 * V * QU);
     const dim3 grid((unsigned)ceil_div(waves, 4));
     hipStream_t s = (hipStream_t)stream;
     ProfScope ps(BT_PROF_ROPE, s);
