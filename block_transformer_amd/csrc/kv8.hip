@@ -29,7 +29,8 @@ struct AppendArgs {
 };
 
 __device__ inline int64_t angle_of(const AppendArgs& a, int pos) {
-    int64_t r = a.pos_table ? a.pos_table[pos] : pos;
+    // (rows behind the cache's end are dropped, but their queries are rotated all the same: not by what lies behind the table)
+    int64_t r = a.pos_table ? a.pos_table[pos < a.c.n_max ? pos : a.c.n_max - 1] : pos;
     r = r < 0 ? 0 : r;
     return r < a.max_pos ? r : a.max_pos - 1;
 }

@@ -253,7 +253,8 @@ int bt_quant_rows(int dtype, int64_t M, int64_t K, const void* x, int64_t ldx, c
 
 /* out[m, n] = act(sum_k A[m, k] W[n, k] * a_scale[m] * w_scale[n] + bias[n]) + residual[m, n]: bt_linear in 8-bit integers.  The sum is
  * an exact int32; the rest is fp32, rounded once to `dtype` (of bias, residual and out).  K % 16 == 0, K <= 131056 (the sum cannot
- * leave int32), lda / ldw % 16 == 0, A / W 16-byte aligned; out, bias and residual may have any alignment and row stride.
+ * leave int32), lda / ldw % 16 == 0, A / W 16-byte aligned; out, bias and residual may have any alignment and a row stride below 2^26;
+ * residual may be out.
  * `scratch` (16-byte aligned, >= bt_linear_q8_scratch_bytes(M, N, K), which may be 0) lets short problems split K over workgroups;
  * without it they run unsplit, with the same bits (integer sums do not depend on their order). */
 int64_t bt_linear_q8_scratch_bytes(int64_t M, int64_t N, int64_t K);

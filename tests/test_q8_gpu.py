@@ -183,6 +183,22 @@ def test_linear_q8_strides_and_untouched_memory(M, N, K, dtype):
     assert (out == 7.0).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(5, 40, 32), (33, 70, 16), (100, 130, 48), (200, 72, 80), (257, 264, 336)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_q8_short_and_cut_steps_of_k(M, N, K, dtype):
+    x, w, b, _, y, tol = linear_case(M, N, K, dtype, seed=K)
+    assert ((ops.linear_q8(cuda(x), cuda(w), cuda(b)).cpu().double() - y).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(3, 264, 128), (200, 512, 256), (300, 2048, 4096), (3500, 3650, 128)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_linear_q8_onto_its_own_residual(M, N, K, dtype):
+    x, w, b, r, y, tol = linear_case(M, N, K, dtype, seed=12, residual=True)
+    stream = cuda(r)
+    assert ops.linear_q8(cuda(x), cuda(w), cuda(b), stream, out=stream) is stream
+    assert ((stream.cpu().double() - y).abs() <= tol).all()
+
+
 def test_linear_q8_of_float_rows_and_a_row_that_is_not_finite():
     x, w = rnd(6, 200, seed=9), rnd(50, 200, seed=10)
     x[2, 7] = float("nan")
@@ -328,6 +344,10 @@ def test_append_beyond_the_end_with_a_device_position():
     for p in (32, 1000, -1):
         ops.kv8_append(kv, None, x.to(DEV)[:, :, 0], x.to(DEV)[:, :, 1], pos.fill_(p))
     assert all(same(a, b) for a, b in zip(kv, before))
+    # the queries of rows that are dropped take the position table's last entry
+    t, at = table(16), (torch.arange(32) * 5 % 31).int()
+    q = ops.kv8_append(kv, x.to(DEV)[:, :, 0], x.to(DEV)[:, :, 0], x.to(DEV)[:, :, 1], pos.fill_(30), rope=t.to(DEV), pos_table=at.to(DEV))
+    assert torch.equal(q.cpu(), ref.rope(x[:, :, 0], at[torch.arange(30, 38).clamp(max=31)].long(), t).to(BF16))
 
 
 @pytest.mark.parametrize("B,heads,H,d,block,rot,dtype", CACHES)
@@ -375,6 +395,29 @@ def test_attention(B, heads, H, d, block, dtype, n, q_len):
     kv, k, v, q = attention_case(B, heads, H, d, block, dtype, n, q_len, seed=n + d)
     y = ref.attention(q, k, v, n - q_len)
     check_attention(ops.attention_kv8(q.to(DEV), kv, n - q_len), y, q, k, v, dtype)
+
+
+@pytest.mark.parametrize("B,heads,H,d,block,dtype", SHAPES[1:6])
+def test_attention_of_every_row(B, heads, H, d, block, dtype):
+    """As many queries as rows: the first sees one row, the last all."""
+    n = 139
+    kv, k, v, q = attention_case(B, heads, H, d, block, dtype, n, n, seed=d)
+    check_attention(ops.attention_kv8(q.to(DEV), kv, 0), ref.attention(q, k, v, 0), q, k, v, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attention_with_a_device_position(dtype):
+    """The position read on the device, behind the cache's end and before its start too."""
+    kv, k, v, q = attention_case(2, 4, 2, 64, 16, dtype, 90, 3, seed=41)
+    pos = torch.zeros(1, dtype=torch.int32, device=DEV)
+    for p in (87, 40, 0, 63, 64):
+        y = ref.attention(q, k[:, :, :p + 3], v[:, :, :p + 3], p)
+        if p == 87:      # (rows behind p + 3 stand in codes: a smaller p would take some of them for the open block's)
+            check_attention(ops.attention_kv8(q.to(DEV), kv, pos.fill_(p)), y, q, k, v, dtype)
+        assert torch.equal(ops.attention_kv8(q.to(DEV), kv, pos.fill_(p), n_split=1).nan_to_num(7),
+                           ops.attention_kv8(q.to(DEV), kv, p, n_split=1).nan_to_num(7))
+    assert (ops.attention_kv8(q.to(DEV), kv, pos.fill_(-50)) == 0).all()
+    assert ops.attention_kv8(q.to(DEV), kv, pos.fill_(1 << 30)).shape == (2, 3, 4, 64)
 
 
 @pytest.mark.parametrize("B,heads,H,d,block,dtype", SHAPES[:6])
