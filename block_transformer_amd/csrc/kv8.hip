@@ -3,6 +3,7 @@
 #include "bt_common.h"
 #include "bt_quant.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace bt {
@@ -567,7 +568,8 @@ struct Attend {
         const int64_t tok0 = at * 64 + 16 * g;
         const Side now = side;
         if (MORE) side = load_side(then);
-        const float sk = now.sk, sv = now.sv, mul = qs * sk;
+        const float mul = qs * now.sk;
+        float sv = now.sv;
         float s[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -588,6 +590,7 @@ struct Attend {
         if (cut) {
             uint32_t on = reached(tok0, 16, n_full);
             if (mask) on &= set_bytes(now.mask);
+            sv = on ? sv : 0.f;      // of a block that nobody sees not even the scale counts: it may be anything
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -911,8 +914,9 @@ __global__ __launch_bounds__(256) void attention_kv8_join_kernel(AttnArgs a) {
 template <typename T, int D>
 static void launch_attention(const AttnArgs& a, int64_t groups, hipStream_t s) {
     const int64_t grid = groups * a.n_split;
-    // four waves to a head's rows where heads are few, one where they fill the card by themselves
-    if (grid >= 4096)
+    // Four waves to a head's rows where heads are few, one where there would be more workgroups of four than the card holds at a time
+    // (two to a CU): 512 heads x 543 rows 19.0 against 22.5 us, 768 heads 31.6 against 25.9, 2048 heads 70.9 against 54.7.
+    if (grid > 512)
         hipLaunchKernelGGL((attention_kv8_kernel<T, D, 1>), dim3((unsigned)grid), dim3(64), 0, s, a);
     else
         hipLaunchKernelGGL((attention_kv8_kernel<T, D, 4>), dim3((unsigned)grid), dim3(256), 0, s, a);
@@ -1031,12 +1035,14 @@ extern "C" int bt_kv8_read(int dtype, const bt_kv8_cache* cache, int64_t n, int6
     return BT_OK;
 }
 
-// Enough workgroups of four waves for the card (256 CUs, two of them to a CU), no split shorter than eight 64-row tiles: two a wave.
+// One workgroup to a CU, none with less than two 64-row tiles, 64 splits at most; fewer than three are not worth the second launch of 4 us.
+// Measured at 16 heads of one sequence: 543 rows 10.7 us whole, 9.2 in 4; 2000 rows 15.9 and 9.2 in 16; 32768 rows 163 and 27.6 in 16 (32: 27.7);
+// at 128 heads 543 rows 11.0 whole, 11.8 in 2.
 extern "C" int32_t bt_attention_kv8_split_count(int64_t batch, int32_t kv_heads, int32_t group, int32_t q_len, int64_t n) {
     const int64_t groups = batch * kv_heads * ceil_div((int64_t)group * q_len, 16), tiles = ceil_div(n, 64);
     if (groups <= 0) return 1;
-    const int64_t want = ceil_div(512, groups), most = tiles / 8;
-    return (int32_t)(want < most ? want : most > 1 ? most : 1);
+    const int64_t s = std::min<int64_t>(std::min(256 / groups, tiles / 2), 64);
+    return s < 3 ? 1 : (int32_t)s;
 }
 
 extern "C" int64_t bt_attention_kv8_workspace_bytes(int64_t batch, int32_t q_len, int32_t heads, int32_t head_dim, int32_t n_split) {

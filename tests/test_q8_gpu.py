@@ -464,6 +464,22 @@ def test_attention_masked_infinities_of_a_full_block(dtype):
     check_attention(ops.attention_kv8(q.to(DEV), kv, n - 1, mask=mask.to(DEV)), y, q, k, v, dtype)
 
 
+@pytest.mark.parametrize("B,heads,H,d,block,dtype", SHAPES[1:6])
+def test_attention_masked_blocks_that_were_never_written(B, heads, H, d, block, dtype):
+    """Blocks that the mask hides as a whole may hold any codes and scales."""
+    n = 5 * block + 70
+    kv, k, v, q = attention_case(B, heads, H, d, block, dtype, n, 2, seed=43)
+    mask = torch.ones(B, n, dtype=torch.uint8)
+    for j, bad in ((0, "nan"), (2, "inf"), (3, "-inf"), (4, "nan")):
+        mask[:, j * block:(j + 1) * block] = 0
+        kv[2][:, :, j], kv[3][:, :, j] = float(bad), float(bad)
+        kv[0][:, :, j * block:(j + 1) * block], kv[1][:, :, j] = -128, -128
+    mask[0, :] = 0
+    out = ops.attention_kv8(q.to(DEV), kv, n - 2, mask=mask.to(DEV))
+    check_attention(out, ref.attention(q, k, v, n - 2, mask), q, k, v, dtype)
+    assert (out[0] == 0).all()
+
+
 @pytest.mark.parametrize("dtype", [F32, BF16])
 def test_attention_queries_and_open_rows_that_are_not_finite(dtype):
     """NaN where a NaN or infinity takes part, and in those rows alone."""
