@@ -381,9 +381,10 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
 // is replaced by the step's first bytes, and A's operand is zero there.
 //  * Two workgroups to a CU: while one waits at its barrier or writes its tile, the other's waves have the matrix units.  So a K step
 //    needs one barrier and the epilogue no software overlap.
-//  * A and W travel global -> LDS without registers, NS - 1 steps ahead, in a ring of NS stages.  A wave waits for its own loads of step t
-//    (in order: at most those of the younger steps stay out), then for the others at the barrier; behind it everybody has also consumed
-//    step t - 1, whose stage takes the loads of step t + NS - 1.
+//  * A and W travel global -> LDS without registers, NS - 1 steps ahead, in a ring of NS stages, and LDS -> registers one step ahead: the
+//    fragments of step t + 1 are read under the products of step t.  In step t a wave waits for its own loads of step t + 1 (in order: at
+//    most those of the younger steps stay out), then for the others at the barrier; behind it everybody has also multiplied step t - 1,
+//    whose stage takes the loads of step t + NS - 1.
 //  * LDS rows are 64 bytes; the four 16-byte pieces of row r are stored in the order p ^ ((r >> 1) & 3) ^ ((r >> 3) & 1): the 16 rows that
 //    a fragment read touches at once are spread over all banks.
 //  * mfma(W, A): a lane gets four neighbouring columns of one row (q8_write).
@@ -435,37 +436,55 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
         if (t < steps) load(t);
 
     const int frag = c * 64 + (g ^ ((c >> 1) & 3) ^ ((c >> 3) & 1)) * 16;
-    int stage = 0;
-    auto step = [&](int t, auto last) {
-        if (t + NS - 2 < steps) wait_loads<LOADS * (NS - 2)>();
-        else if (NS > 4 && t + 4 < steps) wait_loads<LOADS * 4>();      // (at most what is still out)
-        else if (NS > 3 && t + 1 < steps) wait_loads<LOADS>();
-        else wait_loads<0>();
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (t + NS - 1 < steps) load(t + NS - 1);
-        const char* a = smem + stage * STAGE + wm * MI * 1024 + frag;
-        const char* w = smem + stage * STAGE + BM * 64 + wn * NB * 1024 + frag;
-        i32x4 af[MI], wf[NB];
+    struct Step {
+        i32x4 a[MI], w[NB];
+    } f[2];
+    auto read = [&](int t, Step& x) {
+        const char* a = smem + (t % NS) * STAGE + wm * MI * 1024 + frag;
+        const char* w = smem + (t % NS) * STAGE + BM * 64 + wn * NB * 1024 + frag;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) wf[j] = *(const i32x4*)(w + j * 1024);
+        for (int j = 0; j < NB; ++j) x.w[j] = *(const i32x4*)(w + j * 1024);
 #pragma unroll
-        for (int i = 0; i < MI; ++i) af[i] = *(const i32x4*)(a + i * 1024);
-        if constexpr (decltype(last)::value) {
-            if (g >= whole) {
-#pragma unroll
-                for (int i = 0; i < MI; ++i) af[i] = i32x4{0, 0, 0, 0};
-            }
-        }
+        for (int i = 0; i < MI; ++i) x.a[i] = *(const i32x4*)(a + i * 1024);
+    };
+    auto multiply = [&](const Step& x) {
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j], af[i], acc[i][j], 0, 0, 0);
-        stage = stage + 1 == NS ? 0 : stage + 1;
+            for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x.w[j], x.a[i], acc[i][j], 0, 0, 0);
     };
-    const int full = steps - (cut >= 0);
-    for (int t = 0; t < full; ++t) step(t, std::false_type{});
-    if (cut >= 0) step(cut, std::true_type{});
+    auto barrier = [] {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    auto step = [&](int t, const Step& now, Step& next) {      // step t of two or more, not the last
+        if (t + NS - 2 < steps) wait_loads<LOADS * (NS - 3)>();
+        else if (NS > 5 && t + 4 < steps) wait_loads<LOADS * 2>();      // (at most what is still out)
+        else wait_loads<0>();
+        barrier();
+        if (t + NS - 1 < steps) load(t + NS - 1);
+        read(t + 1, next);
+        multiply(now);
+    };
+    if (steps >= NS - 1) wait_loads<LOADS * (NS - 2)>();
+    else wait_loads<0>();
+    barrier();
+    read(0, f[0]);
+    int t = 0;
+    for (; t + 2 < steps; t += 2) {
+        step(t, f[0], f[1]);
+        step(t + 1, f[1], f[0]);
+    }
+    if (t + 1 < steps) {
+        step(t, f[0], f[1]);
+        f[0] = f[1];
+    }
+    if (whole < 4 && g >= whole) {
+#pragma unroll
+        for (int i = 0; i < MI; ++i) f[0].a[i] = i32x4{0, 0, 0, 0};
+    }
+    multiply(f[0]);
 
     const int m_w = m0 + wm * MI * 16, n_w = n0 + wn * NB * 16;
     if (e.slices > 1) {
