@@ -794,12 +794,12 @@ __global__ __launch_bounds__(256) void linear_q8_join_kernel(Q8Args e) {
 }
 
 // What runs a product, from its sizes alone: the cheapest by a model of the time in microseconds, fitted to graph-replayed launches of
-// M = 32 .. 8192 by N = 2048, 6144, 8192 by K = 2048, 8192 (within 20 % of them; its choice within 10 % of the best).
-//   64 x 64 tiles    4 + 0.18 a step while there is one to a CU, 0.128 times their number from two on    (256 x 6144 x 2048: 11.7; 128 x 128: 18.2)
-//   128 x 128 tiles  5 + 0.36 a step, times their number to a CU from one on                             (512 x 8192 x 2048: 19.7; 64 x 64: 21.6)
-//   256 x 256 tiles  11 + 1.5 for two steps, times rounds                                                (2048 x 6144 x 2048: 32.7; 128 x 128: 40.8)
-//   K in slices      3 for the second launch, and the sums once out and once in at 4 TB/s                (256 x 2048 x 8192 in 4: 18.8; whole: 27.5)
-// Up to 32 rows the rows kernel, which reads W as fast as it comes (1 x 6144 x 2048: 5.1; from 33 rows on tiles are as fast or faster).
+// M = 64 .. 8192 by N = 2048, 6144, 8192 by K = 2048, 8192 (most within 10 % of it; its choice within 10 % of the best of them).
+//   64 x 64 tiles    3.5 + 0.15 a step, or 0.128 times their number to a CU     (256 x 6144 x 2048: 10.6; 128 x 128 tiles 14.0)
+//   128 x 128 tiles  4.5 + 0.28 a step, or 0.325 times their number to a CU     (512 x 8192 x 2048: 15.8; 64 x 64 tiles 19.9)
+//   256 x 256 tiles  11 + 0.72 a step, times rounds                             (8192 x 2048 x 2048: 34.2; 128 x 128 tiles 47.4)
+//   K in slices      3 for the second launch, and the sums once out and in at 4 TB/s     (128 x 2048 x 8192 in 4: 13.9; whole 22.1)
+// Up to 32 rows the rows kernel, which reads W as fast as it comes (32 x 6144 x 2048: 8.2; 64 rows by tiles 7.9, by rows 9.5).
 struct Q8Plan {
     enum Kind { ROWS, TILE64, TILE128, BIG } kind;
     int slices;      // of K (TILE64 and TILE128)
@@ -813,11 +813,11 @@ static Q8Plan q8_plan(int64_t M, int64_t N, int64_t K) {
     double least = 1e30;
     for (int s = 1; s <= 8 && (s == 1 || steps / s >= 4); s *= 2) {
         const double part = (double)ceil_div(steps, s), join = s == 1 ? 0 : 3 + (double)s * (double)M * (double)N * 8 / 4e6;
-        const double a = 4 + part * std::max(0.18, 0.128 * t64 * s) + join, b = 5 + part * 0.36 * std::max(1.0, t128 * s) + join;
+        const double a = 3.5 + part * std::max(0.15, 0.128 * t64 * s) + join, b = 4.5 + part * std::max(0.28, 0.325 * t128 * s) + join;
         if (a < least) least = a, best = {Q8Plan::TILE64, s};
         if (b < least) least = b, best = {Q8Plan::TILE128, s};
     }
-    if (K % 128 == 0 && (double)ceil_div(ceil_div(M, 256) * ceil_div(N, 256), 256) * (11 + 0.75 * (double)steps) < least) best = {Q8Plan::BIG, 1};
+    if (K % 128 == 0 && (double)ceil_div(ceil_div(M, 256) * ceil_div(N, 256), 256) * (11 + 0.72 * (double)steps) < least) best = {Q8Plan::BIG, 1};
     return best;
 }
 
