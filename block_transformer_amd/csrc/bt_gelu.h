@@ -11,17 +11,15 @@ namespace bt {
 //     gelu(x) = x * Phi(-a)          (x < 0)        = x * (1 - Phi(-a))   (x >= 0)
 // which keeps RELATIVE accuracy in the negative tail (no 1 + erf cancellation).  In fp32 arithmetic the result is within
 // 8.5e-6 relative of the exact erf GELU for x > -6 (|gelu| < 6e-9 beyond, absolute error < 8e-9): 1/230 of a bf16
-// half-ulp (round 6: degree 12 -> 11, polynomial error 2.2e-6 -> 7.7e-6 against ~3e-6 of fp32 evaluation noise -- on every bf16
-// input in [-9, 9] both round to the correctly rounded bf16 value; a degree-10 fit, 2.7e-5, would flip 0.03 % of them, degree 9 0.5 %).
-// The fp32 parity path (gemm_generic_kernel) keeps erff.  Two values per call so the polynomial runs on the packed-fp32 pipe
-// (v_pk_fma_f32): 28 instruction slots per PAIR of values (13 v_pk_fma + 3 v_pk_mul + 2 v_min + 2 v_max + 2 quarter-rate v_exp),
-// round 5: 35.
+// half-ulp (a degree-12 fit has a polynomial error of 2.2e-6 instead of 7.7e-6, both beside ~3e-6 of fp32 evaluation noise -- on every
+// bf16 input in [-9, 9] both round to the correctly rounded bf16 value; a degree-10 fit, 2.7e-5, would flip 0.03 % of them, degree 9 0.5 %).
+// The fp32 parity path (gemm_generic_kernel) keeps erff.  Two values per call: two independent chains of FMAs, so neither waits for
+// its own last step.
 typedef float v2f __attribute__((ext_vector_type(2)));
 
 // min(|x|, 6) and max(x, 0) as single instructions: the builtins (fminf / fmaxf / fabsf) make hipcc quiet a possible signalling NaN
-// first -- a v_max_f32 x, x in front of every min / max -- and materialise |x| with a v_and: 8 of the 35 VALU slots a pair of values
-// cost (ISA of the round-5 epilogue: 14 v_pk_fma + 3 v_pk_mul + 6 v_max + 2 v_min + 2 v_and + 2 quarter-rate v_exp).  Plain asm (not
-// volatile: the scheduler may move it); 6.0 is not an inline constant of the VOP3 encoding -> one SGPR for the whole kernel.
+// first -- a v_max_f32 x, x in front of every min / max -- and materialise |x| with a v_and.  Plain asm (not volatile: the scheduler
+// may move it); 6.0 is not an inline constant of the VOP3 encoding -> one SGPR for the whole kernel.
 __device__ inline float min_abs_f32(float x, float hi) {
     float r;
     asm("v_min_f32_e64 %0, |%1|, %2" : "=v"(r) : "v"(x), "s"(hi));
@@ -51,7 +49,7 @@ __device__ inline v2f gelu_tail2(v2f x) {
     const v2f e = {__builtin_amdgcn_exp2f(t.x), __builtin_amdgcn_exp2f(t.y)};
     const v2f q = e * r;                                 // Phi(-|x|)
     // x * Phi(x) = relu(x) - |x| * Phi(-|x|): the same value as selecting q or 1 - q by sign and multiplying (identical for x < 0,
-    // x - x q for x >= 0), in one packed FMA instead of two compares, two selects, a subtraction and a multiply.  The clamped |x| is
+    // x - x q for x >= 0), in one FMA instead of two compares, two selects, a subtraction and a multiply.  The clamped |x| is
     // used for the product: identical bits for |x| <= 6, and beyond that the term is < 1e-8 either way (q < 2e-9)
     const v2f relu = {relu_f32(x.x), relu_f32(x.y)};
     return relu - a * q;
