@@ -270,8 +270,8 @@ constexpr int q8_pitch(int nb) { return 16 * nb * 2 + 16; }      // bytes of a r
 
 // The sums of a wave, NI fragments of 16 rows (row0(i) is the first of fragment i) by 16 NB columns from n_w: lane (c, g) has columns
 // 16 j + 4 g .. + 3 of row c.  Scales, bias, activation and residual there, then one rounding.  fp32 leaves from there, 16 bytes a lane;
-// bf16 rows are put together in `patch` (16 rows, the wave's own) first.  A tile that is whole and `wide` takes 2 NI (bf16) or NI NB stores
-// of NB = 4.
+// bf16 rows are put together in `patch` (16 rows, the wave's own) first.  A wave's part that is whole and `wide` takes NI NB / 2 (bf16)
+// or NI NB stores.
 template <typename T, int NI, int NB, typename Row0>
 __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], char* patch, int n_w, int lane, Row0 row0) {
     constexpr int PITCH = q8_pitch(NB);
@@ -306,8 +306,8 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
                 bias[j][r] = e.bias ? Elem<T>::load((const T*)e.bias + min(n + r, e.N - 1)) : 0.f;
             }
     }
-    // the wave's part of a tile that is whole, in 16-byte pieces: no test a row, and a row's address is a scalar and one lane offset
-    const bool whole = e.wide && row0(NI - 1) + 16 <= e.M && n_w + 16 * NB <= e.N;
+    // whole columns go in 16-byte pieces, whole rows with no test a row; a row's address is a scalar and one lane offset
+    const bool cols = e.wide && n_w + 16 * NB <= e.N, whole = cols && row0(NI - 1) + 16 <= e.M;
     typedef typename std::conditional<sizeof(T) == 2, uint2, float4>::type Four;
     Four next[NB] = {};
     auto load_residual = [&](int i) {
@@ -317,7 +317,7 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
 #pragma unroll
         for (int j = 0; j < NB; ++j) {
             const int n = n_w + j * 16 + g * 4;
-            if (whole) next[j] = *(const Four*)(p + j * 16);
+            if (cols) next[j] = *(const Four*)(p + j * 16);
             else {
                 T v[4] = {};
 #pragma unroll
@@ -350,8 +350,9 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
                 *(uint2*)(patch + c * PITCH + (j * 16 + g * 4) * 2) = uint2{pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3])};
             } else {
                 T* out = (T*)e.out + (int64_t)row0(i) * e.ldo + n_w + (uint32_t)(c * (int)e.ldo + g * 4) + j * 16;
-                if (whole) *(u32x4_t*)out = u32x4_t{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])};
-                else if (row0(i) + c < e.M)
+                if (whole || (cols && row0(i) + c < e.M))
+                    *(u32x4_t*)out = u32x4_t{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])};
+                else if (!cols && row0(i) + c < e.M)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         if (n_w + j * 16 + g * 4 + r < e.N) out[r] = y[r];
@@ -365,8 +366,8 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
             const int r0 = x / CH, r = lane / CH, d = (lane - r * CH) * V;      // (64 is a multiple of CH)
             const u32x4_t v = *(const u32x4_t*)(patch + (r0 + r) * PITCH + d * sizeof(T));
             T* out = (T*)e.out + (int64_t)(row0(i) + r0) * e.ldo + n_w + (uint32_t)(r * (int)e.ldo + d);
-            if (whole) *(u32x4_t*)out = v;
-            else if (row0(i) + r0 + r < e.M) {
+            if (whole || (cols && row0(i) + r0 + r < e.M)) *(u32x4_t*)out = v;
+            else if (!cols && row0(i) + r0 + r < e.M) {
                 T y[V];
                 __builtin_memcpy(y, &v, sizeof v);
 #pragma unroll
@@ -389,7 +390,7 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
 //  * LDS rows are 64 bytes; the four 16-byte pieces of row r are stored in the order p ^ ((r >> 1) & 3) ^ ((r >> 3) & 1): the 16 rows that
 //    a fragment read touches at once are spread over all banks.
 //  * mfma(W, A): a lane gets four neighbouring columns of one row (q8_write).
-// 256 x 6144 x 2048 10.1 us by 64 x 64 tiles, 1024 x 8192 x 2048 29 us (1.2 POPS) and 4096 x 2048 x 8192 85 us (1.6 POPS) by 128 x 128: bound by
+// 256 x 6144 x 2048 10.1 us by 64 x 64 tiles, 2048 x 2048 x 8192 44 us (1.6 POPS) by 128 x 128: bound by
 // the way from L2 into a CU, as the largest kernel is, with more bytes to an operation.
 template <typename T, int MI, int NB, int NS>
 __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
@@ -512,59 +513,62 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
     q8_write<T, MI, NB>(e, acc, smem + wave * 16 * PITCH, n_w, lane, [&](int i) { return m_w + i * 16; });
 }
 
-// The kernel for the largest products: 256 x 256 per workgroup of eight waves, 128 bytes of K a step, K % 128 == 0.  What bounds a large
-// product here is the way from L2 into a CU (about 25 bytes a clock measured, and it moves whole 128-byte lines): a 256 x 256 tile asks
-// for a third less than 256 x 128 does, and a step of 128 bytes takes every line once.  That leaves room for one workgroup to a CU, so
-// its waves take turns by themselves:
-//  * The waves are two groups of four, one of each on every SIMD, half a phase apart: while one group's MFMAs run (a phase has 32 of them),
+// The kernel for large products: 256 x 64 NB (256 or 128) per workgroup of eight waves, 128 bytes of K a step, K % 128 == 0.  What bounds a
+// large product here is the way from L2 into a CU (about 25 bytes a clock measured, and it moves whole 128-byte lines): a 256 x 256 tile
+// asks for a third less than 256 x 128 does, that for a quarter less than 128 x 128, and a step of 128 bytes takes every line once.  256 x 128
+// is for products that have about 256 of them.  There is room for one workgroup to a CU, so its waves take turns by themselves:
+//  * The waves are two groups of four, one of each on every SIMD, half a phase apart: while one group's MFMAs run (a phase has 8 NB of them),
 //    the other reads its fragments and sends loads.  Group 1 begins with one barrier more, so its first barrier of a phase meets group
 //    0's second.
-//  * A step has two phases, one for each half (128 rows) of A; W's fragments are read in the first and kept.  LDS holds two steps of four
-//    half tiles (A0, W0, W1, A1: in the order in which they are wanted).  Phase (t, 0) sends W1 and A1 of step t + 1, phase (t, 1) sends A0
-//    and W0 of step t + 2 into the places that phase (t, 0) has read.
+//  * A step has two phases, one for each half (128 rows) of A; W's fragments are read in the first and kept.  LDS holds RING steps of half
+//    tiles (A0, W0, W1, A1, or A0, W, A1: in the order in which they are wanted).  Phase (t, 0) sends what follows W0 of step t + RING - 1,
+//    phase (t, 1) sends A0 and W0 of step t + RING into the places that phase (t, 0) has read.
 //  * A workgroup stays for all its tiles, and the loads run on from one tile into the next: when a tile's sums are finished, the next
-//    one's first two steps are on their way or there, so its products start behind the epilogue without a wait, and the epilogue's stores
+//    one's first RING steps are on their way or there, so its products start behind the epilogue without a wait, and the epilogue's stores
 //    drain under them.
-//  * Waits are for all but the youngest loads (they return in order).  In front of phase (t, 0) what may still be out is A1 of the step
-//    and A0, W0 of the next: 6 loads (a half tile is two); in front of (t, 1), the whole next step: 8.  In a tile's first step W1 and A1
-//    of the next are out too (they went ahead of the epilogue): 10 and 8.  In the first two steps of a tile the stores of the one before
-//    are younger than the loads in question and are counted as well, if that tile was whole (else their number varies, and the wait is
-//    for them too).  In the last step of all, for everything.  Group 0 waits at the top of a phase, group 1 for the next phase's before its
-//    second barrier, which is the one that opens that phase to group 0.
+//  * Waits are for all but the youngest loads (they return in order; a half tile is two).  In front of phase (t, 0) what may still be out is
+//    A1 of the step, the next RING - 2 steps, and A0, W0 of the one after; in front of (t, 1), the next RING - 1 steps.  In a tile's
+//    first step all of the next RING - 1 are out (they went ahead of the epilogue).  In the first RING steps of a tile the stores
+//    of the one before are younger than the loads in question and are counted as well, if that tile was whole (else their number varies,
+//    and the wait is for them too).  In the last RING - 1 steps of all, for everything.  Group 0 waits at the top of a phase, group 1 for the
+//    next phase's before its second barrier, which is the one that opens that phase to group 0.
 //  * A wave's reads have returned before its second barrier of a phase; the other group sends the loads that overwrite those places behind
 //    that barrier.
 //  * A tile ends with one more barrier for group 0 (group 1 has then read its last) and begins with one more for group 1, so the two
 //    epilogues run side by side.
 //  * A row of 128 bytes has its 16-byte pieces in the order p ^ (row & 7).
 // 8192 x 8192 x 2048 131 us (2.1 POPS), with GELU 141 us, 8192 x 8192 x 8192 398 us (2.8 POPS, matrix units busy two thirds of the time at the
-// 1.8 GHz that the card then holds).  Of the 131 us, 107 are the products, 10 the stores and 14 the rest of the epilogue.
-template <typename T>
+// 1.8 GHz that the card then holds).  Of the 131 us, 107 are the products, 10 the stores and 14 the rest of the epilogue.  4096 x 2048 x 8192
+// by 256 x 128 65 us (2.1 POPS; by 128 x 128 77, by 256 x 256 on half the CUs 80).
+template <typename T, int NB>
 __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
-    constexpr int HALF = 128 * 128, STEP = 4 * HALF, PITCH = q8_pitch(4), PATCH = sizeof(T) == 2 ? 16 * PITCH : 0;
-    constexpr int STORES = sizeof(T) == 2 ? 16 : 32;      // of a wave and whole tile
-    __shared__ __attribute__((aligned(16))) char smem[2 * STEP + 8 * PATCH];
+    constexpr int HALVES = NB == 4 ? 4 : 3, RING = NB == 4 ? 2 : 3, COLS = 64 * NB;      // A0, W0, (W1,) A1
+    constexpr int HALF = 128 * 128, STEP = HALVES * HALF, PITCH = q8_pitch(NB), PATCH = sizeof(T) == 2 ? 16 * PITCH : 0;
+    constexpr int STORES = sizeof(T) == 2 ? 4 * NB : 8 * NB;      // of a wave and whole tile
+    constexpr int LOADS = 2 * HALVES;                             // of a wave and step
+    __shared__ __attribute__((aligned(16))) char smem[RING * STEP + 8 * PATCH];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wm = wave >> 2, wn = wave & 3, c = lane & 15, g = lane >> 4;
     const bool second = wm != 0;
     const int steps = e.K >> 7;
 
-    // the loads: step `lt` of tile number `lround`, the `lx`-th step of all
+    // the loads: step `lt` of tile number `lround`, into place `lx` of the ring
     int lm = 0, ln = 0, lt = 0, lround = 0, lx = 0;
     bool more = true;
     const int8_t *A = nullptr, *W = nullptr;
-    uint32_t off[4][2];      // [half tile][load]
+    uint32_t off[HALVES][2];      // [half tile][load]
     auto enter = [&] {
         more = q8_tile<4>(e, gridDim.x, lround, lm, ln);
         if (!more) return;
         A = e.A + (int64_t)lm * 256 * e.lda;
-        W = e.W + (int64_t)ln * 256 * e.ldw;
+        W = e.W + (int64_t)ln * COLS * e.ldw;
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
+        for (int h = 0; h < HALVES; ++h)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const bool a = h == 0 || h == 3;
+                const bool a = h == 0 || h == HALVES - 1;
                 int row = (h >= 2 ? 128 : 0) + wave * 16 + i * 8 + (lane >> 3);
-                const int last = a ? e.M - 1 - lm * 256 : e.N - 1 - ln * 256;      // rows beyond the matrix repeat its last one
+                const int last = a ? e.M - 1 - lm * 256 : e.N - 1 - ln * COLS;      // rows beyond the matrix repeat its last one
                 row = row < last ? row : last;
                 off[h][i] = (uint32_t)row * (uint32_t)(a ? e.lda : e.ldw) + (uint32_t)((lane & 7) ^ (lane >> 3)) * 16;
             }
@@ -573,9 +577,9 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
     auto load = [&](auto half) {
         constexpr int h = decltype(half)::value;
         if (!more) return;
-        const int8_t* base = h == 0 || h == 3 ? A : W;
-        dma16(base, off[h][0], ring + (lx & 1) * STEP + h * HALF);
-        dma16(base, off[h][1], ring + (lx & 1) * STEP + h * HALF + 1024);
+        const int8_t* base = h == 0 || h == HALVES - 1 ? A : W;
+        dma16(base, off[h][0], ring + lx * STEP + h * HALF);
+        dma16(base, off[h][1], ring + lx * STEP + h * HALF + 1024);
     };
     using H0 = std::integral_constant<int, 0>;
     using H1 = std::integral_constant<int, 1>;
@@ -584,8 +588,8 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
     auto first_half = [&] { load(H0{}); load(H1{}); };
     auto second_half = [&] {
         load(H2{});
-        load(H3{});
-        ++lx;
+        if constexpr (HALVES == 4) load(H3{});
+        lx = lx + 1 == RING ? 0 : lx + 1;
         A += 128;
         W += 128;
         if (++lt == steps) {
@@ -600,54 +604,58 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
         asm volatile("" ::: "memory");
     };
     enter();
-    first_half(); second_half();
-    first_half(); second_half();
+#pragma unroll
+    for (int i = 0; i < RING; ++i) {
+        first_half();
+        second_half();
+    }
 
-    int m0, n0, x = 0;      // the tile, and the number of steps of all that are done
-    bool stores = false;    // the tile before has left STORES stores behind the loads of this one's first two steps
+    int m0, n0, at = 0;     // the tile, and the step's place in the ring
+    const int rounds = e.tiles_m * e.tiles_n / (int)gridDim.x;      // that every workgroup has a tile in; one more is some workgroups'
+    int left = (rounds + q8_tile<4>(e, gridDim.x, rounds, m0, n0)) * steps;      // steps of all that are still to be done
+    bool stores = false;    // the tile before has left STORES stores behind the loads of this one's first RING steps
     for (int round = 0; q8_tile<4>(e, gridDim.x, round, m0, n0); ++round) {
         m0 *= 256;
-        n0 *= 256;
-        i32x4 acc[8][4];
+        n0 *= COLS;
+        i32x4 acc[8][NB];
 #pragma unroll
         for (int i = 0; i < 8; ++i)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-        int nm, nn;
-        const bool last_tile = !q8_tile<4>(e, gridDim.x, round + 1, nm, nn);
-        auto wait_first = [&](int t) {      // for phase (t, 0)
-            if (last_tile && t == steps - 1) wait_loads<0>();
-            else if (t == 0 && stores) wait_loads<10 + STORES>();
-            else if (t == 0) wait_loads<10>();
-            else if (t == 1 && stores) wait_loads<6 + STORES>();
-            else wait_loads<6>();
+            for (int j = 0; j < NB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
+        constexpr int FIRST = 2 + (RING - 2) * LOADS + 4, WHOLE = 2 + (RING - 1) * LOADS, SECOND = (RING - 1) * LOADS;
+        auto wait_first = [&](int t, int left) {      // for phase (t, 0)
+            if (left < RING) wait_loads<0>();
+            else if (t == 0 && stores) wait_loads<WHOLE + STORES>();
+            else if (t == 0) wait_loads<WHOLE>();
+            else if (t < RING && stores) wait_loads<FIRST + STORES>();
+            else wait_loads<FIRST>();
         };
         auto wait_second = [&](int t) {     // for phase (t, 1)
-            if (last_tile && t == steps - 1) wait_loads<0>();
-            else if (t <= 1 && stores) wait_loads<8 + STORES>();
-            else wait_loads<8>();
+            if (left < RING) wait_loads<0>();
+            else if (t < RING && stores) wait_loads<SECOND + STORES>();
+            else wait_loads<SECOND>();
         };
         if (second) {
-            wait_first(0);
+            wait_first(0, left);
             barrier();
         }
         const int p0 = (g ^ (c & 7)) * 16, p1 = ((4 + g) ^ (c & 7)) * 16;      // this lane's pieces of a row: the step's first and second 64 bytes
-        i32x4 af[4][2], wf[4][2];
-        for (int t = 0; t < steps; ++t, ++x) {
-            const char* step = smem + (x & 1) * STEP;
+        i32x4 af[4][2], wf[NB][2];
+        for (int t = 0; t < steps; ++t, --left, at = at + 1 == RING ? 0 : at + 1) {
+            const char* step = smem + at * STEP;
             const char* a = step + (wm * 64 + c) * 128;
-            const char* w = step + (wn >> 1 ? 2 : 1) * HALF + ((wn & 1) * 64 + c) * 128;
+            const char* w = step + HALF + (wn * 16 * NB + c) * 128;
             // phase 0
-            if (!second) wait_first(t);
+            if (!second) wait_first(t, left);
             barrier();
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                wf[j][0] = *(const i32x4*)(w + j * 2048 + p0);
+                if (j < NB) wf[j][0] = *(const i32x4*)(w + j * 2048 + p0);
                 af[j][0] = *(const i32x4*)(a + j * 2048 + p0);
             }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                wf[j][1] = *(const i32x4*)(w + j * 2048 + p1);
+                if (j < NB) wf[j][1] = *(const i32x4*)(w + j * 2048 + p1);
                 af[j][1] = *(const i32x4*)(a + j * 2048 + p1);
             }
             if (t > 0) second_half();
@@ -660,7 +668,7 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NB; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[i][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
             // phase 1
             if (!second) wait_second(t);
@@ -668,9 +676,9 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) af[i][k] = *(const i32x4*)(a + 3 * HALF + i * 2048 + (k ? p1 : p0));
+                for (int i = 0; i < 4; ++i) af[i][k] = *(const i32x4*)(a + (HALVES - 1) * HALF + i * 2048 + (k ? p1 : p0));
             first_half();
-            if (second && t + 1 < steps) wait_first(t + 1);
+            if (second && t + 1 < steps) wait_first(t + 1, left - 1);
             __builtin_amdgcn_s_waitcnt(0xc07f);
             barrier();
             __builtin_amdgcn_sched_barrier(0);
@@ -679,15 +687,15 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[4 + i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[4 + i][j], 0, 0, 0);
+                    for (int j = 0; j < NB; ++j) acc[4 + i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j][k], af[i][k], acc[4 + i][j], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
         }
         if (!second) barrier();      // group 1 has read its last fragments
         second_half();
         int hide = lane;
         asm volatile("" : "+v"(hide));      // the epilogue's addresses are not to be kept in registers through the products
-        q8_write<T, 8, 4>(e, acc, smem + 2 * STEP + wave * PATCH, n0 + wn * 64, hide, [&](int i) { return m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16; });
-        stores = e.wide && m0 + 256 <= e.M && n0 + 256 <= e.N;
+        q8_write<T, 8, NB>(e, acc, smem + RING * STEP + wave * PATCH, n0 + wn * 16 * NB, hide, [&](int i) { return m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16; });
+        stores = e.wide && m0 + 256 <= e.M && n0 + COLS <= e.N;
     }
 }
 
@@ -800,14 +808,16 @@ __global__ __launch_bounds__(256) void linear_q8_join_kernel(Q8Args e) {
 }
 
 // What runs a product, from its sizes alone: the cheapest by a model of the time in microseconds, fitted to graph-replayed launches of
-// M = 64 .. 8192 by N = 2048, 6144, 8192 by K = 2048, 8192 (most within 10 % of it; its choice within 10 % of the best of them).
+// M = 64 .. 8192 by N = 2048 .. 8192 by K = 1024 .. 8192 (most within 10 % of it; its choice within 10 % of the best of them).
 //   64 x 64 tiles    3.5 + 0.15 a step, or 0.128 times their number to a CU     (256 x 6144 x 2048: 10.6; 128 x 128 tiles 14.0)
-//   128 x 128 tiles  4.5 + 0.28 a step, or 0.325 times their number to a CU     (512 x 8192 x 2048: 15.8; 64 x 64 tiles 19.9)
-//   256 x 256 tiles  11 + 0.72 a step, times rounds                             (8192 x 2048 x 2048: 34.2; 128 x 128 tiles 47.4)
-//   K in slices      3 for the second launch, and the sums once out and in at 4 TB/s     (128 x 2048 x 8192 in 4: 13.9; whole 22.1)
+//   128 x 128 tiles  4.5 + 1.5 times their number t to a CU + 0.28 a step, or 0.3 t     (2048 x 2048 x 2048: 15.1; 256 x 128 tiles 20.5)
+//   256 x 128 tiles  5.5 + 3 a round + 0.44 a step, 0.38 where few CUs have one         (4096 x 2048 x 8192: 64.7; 128 x 128 tiles 77,
+//                                                                                        256 x 256 80)
+//   256 x 256 tiles  5 + 5 a round + 0.73 a step, 0.53 up to half the CUs               (8192 x 2048 x 2048: 33.5; 256 x 128 tiles 44)
+//   K in slices      3 for the second launch, and the sums once out and in at 4 TB/s    (128 x 2048 x 8192 in 4: 13.9; whole 22.1)
 // Up to 32 rows the rows kernel, which reads W as fast as it comes (32 x 6144 x 2048: 8.2; 64 rows by tiles 7.9, by rows 9.5).
 struct Q8Plan {
-    enum Kind { ROWS, TILE64, TILE128, BIG } kind;
+    enum Kind { ROWS, TILE64, TILE128, TALL, BIG } kind;
     int slices;      // of K (TILE64 and TILE128)
 };
 
@@ -819,11 +829,19 @@ static Q8Plan q8_plan(int64_t M, int64_t N, int64_t K) {
     double least = 1e30;
     for (int s = 1; s <= 8 && (s == 1 || steps / s >= 4); s *= 2) {
         const double part = (double)ceil_div(steps, s), join = s == 1 ? 0 : 3 + (double)s * (double)M * (double)N * 8 / 4e6;
-        const double a = 3.5 + part * std::max(0.15, 0.128 * t64 * s) + join, b = 4.5 + part * std::max(0.28, 0.325 * t128 * s) + join;
+        const double a = 3.5 + part * std::max(0.15, 0.128 * t64 * s) + join, b = 4.5 + 1.5 * t128 + part * std::max(0.28, 0.3 * t128 * s) + join;
         if (a < least) least = a, best = {Q8Plan::TILE64, s};
         if (b < least) least = b, best = {Q8Plan::TILE128, s};
     }
-    if (K % 128 == 0 && (double)ceil_div(ceil_div(M, 256) * ceil_div(N, 256), 256) * (11 + 0.72 * (double)steps) < least) best = {Q8Plan::BIG, 1};
+    if (K % 128) return best;
+    auto rounds = [&](int64_t tiles, double each, auto last) {      // of 256 tiles; the last may be for some of the CUs
+        const double rest = (double)(tiles % 256) / 256;
+        return each * (double)ceil_div(tiles, 256) + (double)steps * (last(1.0) * (double)(tiles / 256) + (rest > 0 ? last(rest) : 0));
+    };
+    const double tall = 5.5 + rounds(ceil_div(M, 256) * ceil_div(N, 128), 3, [](double part) { return 0.38 + 0.06 * part; });
+    const double big = 5 + rounds(ceil_div(M, 256) * ceil_div(N, 256), 5, [](double part) { return 0.53 + 0.4 * std::max(0.0, part - 0.5); });
+    if (tall < least) least = tall, best = {Q8Plan::TALL, 1};
+    if (big < least) best = {Q8Plan::BIG, 1};
     return best;
 }
 
@@ -860,7 +878,12 @@ static int launch_linear_q8(Q8Args& e, int64_t scratch_bytes, hipStream_t s) {
         case Q8Plan::BIG:
             e.tiles_m = (int)ceil_div(e.M, 256);
             e.tiles_n = (int)ceil_div(e.N, 256);
-            hipLaunchKernelGGL((linear_q8_big_kernel<T>), dim3((unsigned)std::min(e.tiles_m * e.tiles_n, 256)), dim3(512), 0, s, e);
+            hipLaunchKernelGGL((linear_q8_big_kernel<T, 4>), dim3((unsigned)std::min(e.tiles_m * e.tiles_n, 256)), dim3(512), 0, s, e);
+            break;
+        case Q8Plan::TALL:
+            e.tiles_m = (int)ceil_div(e.M, 256);
+            e.tiles_n = (int)ceil_div(e.N, 128);
+            hipLaunchKernelGGL((linear_q8_big_kernel<T, 2>), dim3((unsigned)std::min(e.tiles_m * e.tiles_n, 256)), dim3(512), 0, s, e);
             break;
     }
     BT_LAUNCH_CHECK("bt_linear_q8 launch");

@@ -151,6 +151,23 @@ def test_linear_q8_many_tiles(M, N, K, dtype, variant):
     assert ((out.cpu().double() - y).abs() <= tol).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(3900, 2040, 1024), (4000, 2048, 640), (5567, 2850, 640), (4100, 3144, 1024)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("variant", ["bias_gelu", "bias_res"])
+def test_linear_q8_tall_tiles_and_cut_rows(M, N, K, dtype, variant):
+    """Products of about as many 256 x 128 tiles as the card has CUs and twice that, whose last rows are no whole tile; once and onto
+    itself."""
+    x, w, b, r, y, tol = linear_case(M, N, K, dtype, seed=M, residual="res" in variant, act="gelu" if "gelu" in variant else "none")
+    act = "gelu" if "gelu" in variant else "none"
+    x, w, b, r = cuda(x), cuda(w), cuda(b), cuda(r)
+    out = ops.linear_q8(x, w, b, r, act=act, dtype=dtype)
+    assert ((out.cpu().double() - y).abs() <= tol).all()
+    for _ in range(3):
+        again = torch.empty(M + 1, N, dtype=dtype, device=DEV).fill_(7)
+        ops.linear_q8(x, w, b, r, act=act, dtype=dtype, out=again[:M])
+        assert torch.equal(again[:M], out) and (again[M] == 7).all()
+
+
 @pytest.mark.parametrize("M", [1, 3, 40, 200])
 def test_linear_q8_largest_sums(M):
     """Every product 127 * 127 (or -127 * 127): the sum is exact to the last bit right up to the K that is refused."""
