@@ -208,6 +208,19 @@ static int launch_quant_rows(int64_t M, int64_t K, const void* x, int64_t ldx, c
 // ---- bt_linear_q8 ----------------------------------------------------------------------------------------------------------
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
+// Vectors at any element's address: rows of an odd length put every row but the first there.  The card takes such accesses whole
+// (5751 bf16 columns, 7707 rows, K = 2560: 163 us by single elements, 107 so).
+typedef i32x4 i32x4_any __attribute__((aligned(4)));
+template <typename T> struct AnyVec;
+template <> struct AnyVec<bf16> {
+    typedef u32x4_t full __attribute__((aligned(2)));                                    // 8 elements
+    typedef uint32_t four __attribute__((ext_vector_type(2), aligned(2)));               // 4
+};
+template <> struct AnyVec<float> {
+    typedef u32x4_t full __attribute__((aligned(4)));
+    typedef float four __attribute__((ext_vector_type(4), aligned(4)));
+};
+
 struct Q8Args {
     const int8_t* A;
     const int8_t* W;
@@ -221,7 +234,6 @@ struct Q8Args {
     void* out;
     int64_t ldo;
     int act;
-    int wide;           // out (and residual) take 16-byte accesses
     int fours;          // w_scale and bias give four columns at a time
     int tiles_m, tiles_n;
     int slices, steps;  // K split into `slices` ranges of `steps` 64-byte steps; > 1: sums go to `slab`
@@ -270,7 +282,7 @@ constexpr int q8_pitch(int nb) { return 16 * nb * 2 + 16; }      // bytes of a r
 
 // The sums of a wave, NI fragments of 16 rows (row0(i) is the first of fragment i) by 16 NB columns from n_w: lane (c, g) has columns
 // 16 j + 4 g .. + 3 of row c.  Scales, bias, activation and residual there, then one rounding.  fp32 leaves from there, 16 bytes a lane;
-// bf16 rows are put together in `patch` (16 rows, the wave's own) first.  A wave's part that is whole and `wide` takes NI NB / 2 (bf16)
+// bf16 rows are put together in `patch` (16 rows, the wave's own) first.  A wave's part that is whole takes NI NB / 2 (bf16)
 // or NI NB stores.
 template <typename T, int NI, int NB, typename Row0>
 __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], char* patch, int n_w, int lane, Row0 row0) {
@@ -307,8 +319,9 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
             }
     }
     // whole columns go in 16-byte pieces, whole rows with no test a row; a row's address is a scalar and one lane offset
-    const bool cols = e.wide && n_w + 16 * NB <= e.N, whole = cols && row0(NI - 1) + 16 <= e.M;
-    typedef typename std::conditional<sizeof(T) == 2, uint2, float4>::type Four;
+    const bool cols = n_w + 16 * NB <= e.N, whole = cols && row0(NI - 1) + 16 <= e.M;
+    typedef typename AnyVec<T>::four Four;
+    typedef typename AnyVec<T>::full Full;
     Four next[NB] = {};
     auto load_residual = [&](int i) {
         const int m = row0(i) + c;
@@ -351,7 +364,7 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
             } else {
                 T* out = (T*)e.out + (int64_t)row0(i) * e.ldo + n_w + (uint32_t)(c * (int)e.ldo + g * 4) + j * 16;
                 if (whole || (cols && row0(i) + c < e.M))
-                    *(u32x4_t*)out = u32x4_t{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])};
+                    *(Full*)out = u32x4_t{__float_as_uint(y[0]), __float_as_uint(y[1]), __float_as_uint(y[2]), __float_as_uint(y[3])};
                 else if (!cols && row0(i) + c < e.M)
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -366,7 +379,7 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
             const int r0 = x / CH, r = lane / CH, d = (lane - r * CH) * V;      // (64 is a multiple of CH)
             const u32x4_t v = *(const u32x4_t*)(patch + (r0 + r) * PITCH + d * sizeof(T));
             T* out = (T*)e.out + (int64_t)(row0(i) + r0) * e.ldo + n_w + (uint32_t)(r * (int)e.ldo + d);
-            if (whole || (cols && row0(i) + r0 + r < e.M)) *(u32x4_t*)out = v;
+            if (whole || (cols && row0(i) + r0 + r < e.M)) *(Full*)out = v;
             else if (!cols && row0(i) + r0 + r < e.M) {
                 T y[V];
                 __builtin_memcpy(y, &v, sizeof v);
@@ -500,7 +513,7 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
 #pragma unroll
             for (int j = 0; j < NB; ++j) {
                 const int n = n_w + j * 16 + g * 4;
-                if (n + 4 <= e.N && (e.N & 3) == 0) *(i32x4*)(slab + (int64_t)m * e.N + n) = acc[i][j];
+                if (n + 4 <= e.N) *(i32x4_any*)(slab + (int64_t)m * e.N + n) = acc[i][j];
                 else
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
@@ -695,7 +708,7 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
         int hide = lane;
         asm volatile("" : "+v"(hide));      // the epilogue's addresses are not to be kept in registers through the products
         q8_write<T, 8, NB>(e, acc, smem + RING * STEP + wave * PATCH, n0 + wn * 16 * NB, hide, [&](int i) { return m0 + (i >> 2) * 128 + wm * 64 + (i & 3) * 16; });
-        stores = e.wide && m0 + 256 <= e.M && n0 + COLS <= e.N;
+        stores = m0 + 256 <= e.M && n0 + COLS <= e.N;
     }
 }
 
@@ -783,10 +796,10 @@ __global__ __launch_bounds__(256) void linear_q8_join_kernel(Q8Args e) {
     const int m = (int)(x / quads), n = (int)(x - (int64_t)m * quads) * 4;
     const int64_t slice = (int64_t)e.M * e.N;
     const int* p = e.slab + (int64_t)m * e.N + n;
-    const bool four = n + 4 <= e.N && (e.N & 3) == 0;
+    const bool four = n + 4 <= e.N;
     i32x4 sum{0, 0, 0, 0};
     for (int s = 0; s < e.slices; ++s, p += slice) {
-        if (four) sum += *(const i32x4*)p;
+        if (four) sum += *(const i32x4_any*)p;
         else
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -808,9 +821,10 @@ __global__ __launch_bounds__(256) void linear_q8_join_kernel(Q8Args e) {
 }
 
 // What runs a product, from its sizes alone: the cheapest by a model of the time in microseconds, fitted to graph-replayed launches of
-// M = 64 .. 8192 by N = 2048 .. 8192 by K = 1024 .. 8192 (most within 10 % of it; its choice within 10 % of the best of them).
-//   64 x 64 tiles    3.5 + 0.15 a step, or 0.128 times their number to a CU     (256 x 6144 x 2048: 10.6; 128 x 128 tiles 14.0)
-//   128 x 128 tiles  4.5 + 1.5 times their number t to a CU + 0.28 a step, or 0.3 t     (2048 x 2048 x 2048: 15.1; 256 x 128 tiles 20.5)
+// M = 64 .. 8192 by N = 512 .. 8192 by K = 256 .. 8192, odd ones among them (half of them within 8 % of it, nine in ten within 22 %; its
+// choice is 1.4 % above the best of them on average, 29 % at most).
+//   64 x 64 tiles    3.5 + 0.8 times their number t to a CU + 0.15 a step, or 0.12 t    (256 x 6144 x 2048: 10.6; 128 x 128 tiles 14.0)
+//   128 x 128 tiles  4.5 + 1.5 t + 0.28 a step, 0.5 where some CUs have two, or 0.3 t   (2048 x 2048 x 2048: 15.1; 256 x 128 tiles 20.5)
 //   256 x 128 tiles  5.5 + 3 a round + 0.44 a step, 0.38 where few CUs have one         (4096 x 2048 x 8192: 64.7; 128 x 128 tiles 77,
 //                                                                                        256 x 256 80)
 //   256 x 256 tiles  5 + 5 a round + 0.73 a step, 0.53 up to half the CUs               (8192 x 2048 x 2048: 33.5; 256 x 128 tiles 44)
@@ -829,7 +843,8 @@ static Q8Plan q8_plan(int64_t M, int64_t N, int64_t K) {
     double least = 1e30;
     for (int s = 1; s <= 8 && (s == 1 || steps / s >= 4); s *= 2) {
         const double part = (double)ceil_div(steps, s), join = s == 1 ? 0 : 3 + (double)s * (double)M * (double)N * 8 / 4e6;
-        const double a = 3.5 + part * std::max(0.15, 0.128 * t64 * s) + join, b = 4.5 + 1.5 * t128 + part * std::max(0.28, 0.3 * t128 * s) + join;
+        const double a = 3.5 + 0.8 * t64 + part * std::max(0.15, 0.12 * t64 * s) + join;
+        const double b = 4.5 + 1.5 * t128 + part * std::max(t128 * s > 1 ? 0.5 : 0.28, 0.3 * t128 * s) + join;
         if (a < least) least = a, best = {Q8Plan::TILE64, s};
         if (b < least) least = b, best = {Q8Plan::TILE128, s};
     }
@@ -946,8 +961,6 @@ extern "C" int bt_linear_q8(int dtype, int64_t M, int64_t N, int64_t K, const in
     e.out = out;
     e.ldo = ldo;
     e.act = act;
-    const int V = dtype == BT_BF16 ? 8 : 4;
-    e.wide = aligned16(out) && ldo % V == 0 && (!residual || (aligned16(residual) && ldr % V == 0));
     e.fours = aligned16(w_scale) && aligned16(bias);
     e.slab = (int*)scratch;
     if (!scratch) scratch_bytes = 0;
