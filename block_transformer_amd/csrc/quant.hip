@@ -8,6 +8,27 @@
 
 namespace bt {
 
+// Vectors at any element's address: rows of an odd length put every row but the first there.  The card takes such accesses whole
+// (linear_q8 with 7707 rows of 5751 bf16 columns, K = 2560: 163 us by single elements, 107 so).
+template <typename T> struct AnyVec;
+template <> struct AnyVec<bf16> {
+    typedef u32x4_t full __attribute__((aligned(2)));                                    // 8 elements
+    typedef uint32_t four __attribute__((ext_vector_type(2), aligned(2)));               // 4
+};
+template <> struct AnyVec<float> {
+    typedef u32x4_t full __attribute__((aligned(4)));
+    typedef float four __attribute__((ext_vector_type(4), aligned(4)));
+};
+
+template <typename T>
+__device__ inline void load_any(const T* p, float (&v)[Elem<T>::VEC]) {
+    const u32x4_t u = *(const typename AnyVec<T>::full*)p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if constexpr (sizeof(T) == 2) v[2 * i] = __uint_as_float(u[i] << 16), v[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        else v[i] = __uint_as_float(u[i]);
+}
+
 // ---- bt_quant_rows ---------------------------------------------------------------------------------------------------------
 // A row is read once into registers -- NV 16-byte pieces a lane, all loads in flight together -- and everything else happens there:
 // LayerNorm statistics (two-pass, fp32), the largest magnitude, the codes.  R waves to a row: one where there are rows enough for
@@ -36,17 +57,17 @@ struct RowReduce {      // over the R waves of a row (R = 4: the workgroup)
     }
 };
 
-// values c .. c + V - 1 of a row of K (zero beyond); VEC: the row is 16-byte aligned
-template <typename T, bool VEC>
+// values c .. c + V - 1 of a row of K (zero beyond)
+template <typename T>
 __device__ inline void load_piece(const T* row, int c, int K, float (&v)[Elem<T>::VEC]) {
     constexpr int V = Elem<T>::VEC;
-    if (VEC && c + V <= K) load_vec<T>(row + c, v);
+    if (c + V <= K) load_any<T>(row + c, v);
     else
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = c + i < K ? Elem<T>::load(row + c + i) : 0.f;
 }
 
-template <typename T, bool LN, bool VEC, int NV, int R>
+template <typename T, bool LN, int NV, int R>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
                                                         const T* __restrict__ b, float eps, int8_t* __restrict__ codes, int64_t ldc,
                                                         float* __restrict__ scales, int64_t M, int K) {
@@ -60,7 +81,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
     const T* xr = x + row * ldx;
     float v[NV][V];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) load_piece<T, VEC>(xr, (i * 64 * R + at) * V, K, v[i]);
+    for (int i = 0; i < NV; ++i) load_piece<T>(xr, (i * 64 * R + at) * V, K, v[i]);
     if (LN) {
         float sum = 0.f;
 #pragma unroll
@@ -90,8 +111,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
         for (int i = 0; i < NV; ++i) {
             const int c = (i * 64 * R + at) * V;
             float wv[V], bv[V];
-            load_piece<T, VEC>(w, c, K, wv);
-            load_piece<T, VEC>(b, c, K, bv);
+            load_piece<T>(w, c, K, wv);
+            load_piece<T>(b, c, K, bv);
 #pragma unroll
             for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, wv[e], bv[e]);      // 0 beyond K, as wv and bv are
         }
@@ -167,38 +188,31 @@ static int launch_quant_rows(int64_t M, int64_t K, const void* x, int64_t ldx, c
                              int64_t ldc, float* scales, hipStream_t s) {
     constexpr int V = Elem<T>::VEC;
     ProfScope ps(BT_PROF_LAYERNORM, s);
-    const bool vec = aligned16(x) && (ldx % V == 0 || M == 1) && (!w || (aligned16(w) && aligned16(b)));
     const int64_t wave_pieces = ceil_div(K, 64 * V), group_pieces = ceil_div(K, 256 * V);
     // one wave to a row from 2048 rows (8 waves to a CU) while it has at most 8 pieces a lane
     const bool one = wave_pieces <= 8 && M >= 2048;
     const int64_t pieces = one ? wave_pieces : group_pieces;
     const dim3 grid((unsigned)(one ? ceil_div(M, 4) : M));
-#define BT_QR(LN_, VEC_, NV_, R_)                                                                                                    \
-    hipLaunchKernelGGL((quant_rows_kernel<T, LN_, VEC_, NV_, R_>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, \
+#define BT_QR(LN_, NV_, R_)                                                                                                          \
+    hipLaunchKernelGGL((quant_rows_kernel<T, LN_, NV_, R_>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, \
                        codes, ldc, scales, M, (int)K)
-#define BT_QR_PIECES(LN_, VEC_, R_)              \
-    do {                                         \
-        if (pieces <= 1) BT_QR(LN_, VEC_, 1, R_); \
-        else if (pieces <= 2) BT_QR(LN_, VEC_, 2, R_); \
-        else if (pieces <= 4) BT_QR(LN_, VEC_, 4, R_); \
-        else BT_QR(LN_, VEC_, 8, R_);            \
-    } while (0)
-#define BT_QR_ROW(LN_, VEC_)                     \
-    do {                                         \
-        if (one) BT_QR_PIECES(LN_, VEC_, 1);     \
-        else BT_QR_PIECES(LN_, VEC_, 4);         \
+#define BT_QR_PIECES(LN_, R_)              \
+    do {                                   \
+        if (pieces <= 1) BT_QR(LN_, 1, R_); \
+        else if (pieces <= 2) BT_QR(LN_, 2, R_); \
+        else if (pieces <= 4) BT_QR(LN_, 4, R_); \
+        else BT_QR(LN_, 8, R_);            \
     } while (0)
     if (pieces > 8) {
         if (w) hipLaunchKernelGGL((quant_long_rows_kernel<T, true>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, codes, ldc, scales, K);
         else hipLaunchKernelGGL((quant_long_rows_kernel<T, false>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, codes, ldc, scales, K);
     } else if (w) {
-        if (vec) BT_QR_ROW(true, true);
-        else BT_QR_ROW(true, false);
+        if (one) BT_QR_PIECES(true, 1);
+        else BT_QR_PIECES(true, 4);
     } else {
-        if (vec) BT_QR_ROW(false, true);
-        else BT_QR_ROW(false, false);
+        if (one) BT_QR_PIECES(false, 1);
+        else BT_QR_PIECES(false, 4);
     }
-#undef BT_QR_ROW
 #undef BT_QR_PIECES
 #undef BT_QR
     BT_LAUNCH_CHECK("bt_quant_rows launch");
@@ -208,18 +222,7 @@ static int launch_quant_rows(int64_t M, int64_t K, const void* x, int64_t ldx, c
 // ---- bt_linear_q8 ----------------------------------------------------------------------------------------------------------
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 
-// Vectors at any element's address: rows of an odd length put every row but the first there.  The card takes such accesses whole
-// (5751 bf16 columns, 7707 rows, K = 2560: 163 us by single elements, 107 so).
 typedef i32x4 i32x4_any __attribute__((aligned(4)));
-template <typename T> struct AnyVec;
-template <> struct AnyVec<bf16> {
-    typedef u32x4_t full __attribute__((aligned(2)));                                    // 8 elements
-    typedef uint32_t four __attribute__((ext_vector_type(2), aligned(2)));               // 4
-};
-template <> struct AnyVec<float> {
-    typedef u32x4_t full __attribute__((aligned(4)));
-    typedef float four __attribute__((ext_vector_type(4), aligned(4)));
-};
 
 struct Q8Args {
     const int8_t* A;
