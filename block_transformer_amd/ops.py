@@ -5,6 +5,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import struct
 from typing import Optional, Sequence, Tuple, Union
 
 import torch
@@ -179,6 +180,10 @@ def rope_tables(max_pos: int, rot: int, base: float, device) -> torch.Tensor:
 _HERE = contextlib.nullcontext()
 # the current stream's handle and the current device without the Python objects around them: together 5 us of a call that takes 10
 _raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+# bt_kv8_cache as bytes: a third of the time that its fields take one by one
+_cache_bytes = struct.Struct("=I3i2q6Q").pack
+_CACHE_SIZE = ctypes.sizeof(_lib.bt_kv8_cache)
+_CONTIGUOUS = torch.contiguous_format
 
 
 def _on(index: int, *tensors):
@@ -230,9 +235,9 @@ def quantize_rows(x: torch.Tensor, ln_w: Optional[torch.Tensor] = None, ln_b: Op
     Kp = (K + 15) // 16 * 16
     code, index = dtype_code(x.dtype), x.get_device()
     with _on(index, ln_w, ln_b):
-        lead, device = x.shape[:-1], x.device
-        codes = torch.empty(lead + (Kp,), dtype=torch.int8, device=device)
-        scales = torch.empty(lead, dtype=torch.float32, device=device)
+        lead = x.shape[:-1]
+        codes = x.new_empty(lead + (Kp,), dtype=torch.int8)
+        scales = x.new_empty(lead, dtype=torch.float32)
         check(lib().bt_quant_rows(code, M, K, x.data_ptr(), ldx, _at(ln_w), _at(ln_b), eps, codes.data_ptr(), Kp, scales.data_ptr(),
                                   _raw_stream(index)), "bt_quant_rows")
     return codes, scales
@@ -281,7 +286,7 @@ def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight:
     index = xc.get_device()
     with _on(index, xs, wc, ws, bias, residual, out, scratch):
         if out is None:
-            out = torch.empty(shape, dtype=dtype, device=xc.device)
+            out = xc.new_empty(shape, dtype=dtype)
             ldo = N
         elif out.shape != shape or out.dtype != dtype:
             raise _lib.BtError(f"out must be {dtype} {tuple(shape)}")
@@ -299,34 +304,44 @@ def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight:
 
 
 def _kv8(kv: Sequence[torch.Tensor]):
-    """(bt_kv8_cache, dtype code) of one layer of an 8-bit cache: (k_codes, v_codes, k_scale, v_scale, k_tail, v_tail)."""
+    """(bt_kv8_cache, dtype code, B, H, n_max, d, dtype) of one layer of an 8-bit cache: (k_codes, v_codes, k_scale, v_scale, k_tail,
+    v_tail)."""
     kc, vc, ks, vs, kt, vt = kv
-    if kc.dim() != 4 or kt.dim() != 4:
+    codes, tail, dtype = kc.shape, kt.shape, kt.dtype
+    if len(codes) != 4 or len(tail) != 4:
         raise _lib.BtError("a layer of an 8-bit cache is (k_codes, v_codes, k_scale, v_scale, k_tail, v_tail), see runtime.KV8Cache")
-    B, H, n_max, d = kc.shape
-    block, dtype = kt.shape[2], kt.dtype
+    B, H, n_max, d = codes
+    block = tail[2]
     if block == 0 or n_max % block:
         raise _lib.BtError(f"{n_max} rows are not a whole number of blocks of {block}")
     blocks = n_max // block
-    _expect(kc, "k_codes", (B, H, n_max, d), torch.int8)
-    _expect(vc, "v_codes", (B, H, blocks, d, block), torch.int8)
-    _expect(ks, "k_scale", (B, H, blocks), torch.float32)
-    _expect(vs, "v_scale", (B, H, blocks), torch.float32)
-    _expect(kt, "k_tail", (B, H, block, d), dtype)
-    _expect(vt, "v_tail", (B, H, d, block), dtype)
-    return (_lib.bt_kv8_cache(block, H, d, B, n_max, kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), kt.data_ptr(),
-                              vt.data_ptr()), dtype_code(dtype))
+    scales = (B, H, blocks)
+    if not (kc.dtype is vc.dtype is torch.int8 and ks.dtype is vs.dtype is torch.float32 and vt.dtype is dtype and
+            ks.shape == scales and vs.shape == scales and vc.shape == (B, H, blocks, d, block) and tail == (B, H, block, d) and
+            vt.shape == (B, H, d, block) and kc.is_contiguous() and vc.is_contiguous() and ks.is_contiguous() and vs.is_contiguous() and
+            kt.is_contiguous() and vt.is_contiguous()):      # (all at once: 3 us less than one by one, which then says what is wrong)
+        _expect(kc, "k_codes", (B, H, n_max, d), torch.int8)
+        _expect(vc, "v_codes", (B, H, blocks, d, block), torch.int8)
+        _expect(ks, "k_scale", scales, torch.float32)
+        _expect(vs, "v_scale", scales, torch.float32)
+        _expect(kt, "k_tail", (B, H, block, d), dtype)
+        _expect(vt, "v_tail", (B, H, d, block), dtype)
+    cache = _lib.bt_kv8_cache.from_buffer_copy(_cache_bytes(_CACHE_SIZE, block, H, d, B, n_max, kc.data_ptr(), vc.data_ptr(),
+                                                            ks.data_ptr(), vs.data_ptr(), kt.data_ptr(), vt.data_ptr()))
+    return cache, dtype_code(dtype), B, H, n_max, d, dtype
 
 
 def _kv8_rows(t: torch.Tensor, what: str, batch: int, q_len: int, d: int, dtype):
+    """(bt_kv8_rows, heads) of rows [batch, q_len, heads, d] with any outer strides."""
     shape = t.shape
-    if len(shape) != 4 or shape[0] != batch or shape[1] != q_len or shape[3] != d or t.dtype != dtype:
+    if len(shape) != 4 or shape[0] != batch or shape[1] != q_len or shape[3] != d or t.dtype is not dtype:
         raise _lib.BtError(f"{what} must be {dtype} [{batch}, {q_len}, heads, {d}], got {t.dtype} {tuple(shape)}")
     sb, st, sh, one = t.stride()
     if one != 1:
         raise _lib.BtError(f"{what} must have unit inner stride")
+    heads = shape[2]
     # (the stride of a single row says nothing)
-    return _lib.bt_kv8_rows(t.data_ptr(), sb if batch > 1 else 0, st if q_len > 1 else 0, sh if shape[2] > 1 else 0)
+    return _lib.bt_kv8_rows(t.data_ptr(), sb if batch > 1 else 0, st if q_len > 1 else 0, sh if heads > 1 else 0), heads
 
 
 def _pos0(pos0):
@@ -343,11 +358,11 @@ def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.T
     int32 on the device) of one layer of an 8-bit cache (``runtime.KV8Cache``), rotating ``k`` and ``q`` [B, q_len, heads, d] by ``rope``
     (``rope_tables``) at positions pos0 + t or ``pos_table[pos0 + t]``.  Returns the rotated q -- in ``q_out`` (which may be q), new
     memory otherwise; q itself without ``rope``.  Blocks that fill up are quantised in the same call."""
-    cache, code = _kv8(kv)
-    dtype = kv[4].dtype
-    B, q_len, H, d = cache.batch, k.shape[1] if k.dim() == 4 else 0, cache.kv_heads, cache.head_dim
-    kr, vr = (_kv8_rows(t, name, B, q_len, d, dtype) for t, name in ((k, "k"), (v, "v")))
-    if k.shape[2] != H or v.shape[2] != H:
+    cache, code, B, H, n_max, d, dtype = _kv8(kv)
+    q_len = k.shape[1] if k.dim() == 4 else 0
+    kr, k_heads = _kv8_rows(k, "k", B, q_len, d, dtype)
+    vr, v_heads = _kv8_rows(v, "v", B, q_len, d, dtype)
+    if k_heads != H or v_heads != H:
         raise _lib.BtError(f"k and v must have the cache's {H} heads")
     if q_len == 0:
         raise _lib.BtError("no rows to append")
@@ -355,26 +370,27 @@ def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.T
     heads = rot = max_pos = 0
     cos = sin = None
     if q is not None:
-        qr, heads = _kv8_rows(q, "q", B, q_len, d, dtype), q.shape[2]
+        qr, heads = _kv8_rows(q, "q", B, q_len, d, dtype)
     pos_dev, pos_host = _pos0(pos0)
     index = k.get_device()
     with _on(index, *kv, q, v, rope, pos_table, q_out, pos0 if pos_dev else None):
         if rope is not None:
-            if rope.dim() != 3 or rope.shape[0] != 2 or rope.dtype != torch.float32 or not rope.is_contiguous():
+            table = rope.shape
+            if len(table) != 3 or table[0] != 2 or rope.dtype != torch.float32 or not rope.is_contiguous():
                 raise _lib.BtError("rope must be contiguous float32 [2, max_pos, rot / 2] (rope_tables)")
-            max_pos, rot = rope.shape[1], 2 * rope.shape[2]
+            max_pos, rot = table[1], 2 * table[2]
             cos = rope.data_ptr()
-            sin = cos + rope.stride(0) * 4
+            sin = cos + max_pos * table[2] * 4
             if q is not None:
                 if q_out is None:
-                    q_out = torch.empty(q.shape, dtype=dtype, device=q.device)
+                    q_out = torch.empty_like(q, memory_format=_CONTIGUOUS)
                 elif q_out.shape != q.shape:
                     raise _lib.BtError("q_out must have q's shape")
-                qor = _kv8_rows(q_out, "q_out", B, q_len, d, dtype)
+                qor = _kv8_rows(q_out, "q_out", B, q_len, d, dtype)[0]
         elif q_out is not None:
             raise _lib.BtError("q_out without rope: there is nothing to rotate q by")
         if pos_table is not None and (pos_table.dtype != torch.int32 or pos_table.dim() != 1 or not pos_table.is_contiguous() or
-                                      pos_table.numel() < (cache.n_max if pos_dev else pos_host + q_len)):
+                                      pos_table.numel() < (n_max if pos_dev else pos_host + q_len)):
             raise _lib.BtError("pos_table must be contiguous int32 and hold an entry for every row")
         check(lib().bt_kv8_append(code, ctypes.byref(cache), q_len, heads if rot else 0, qr if rot else None, qor, kr, vr, pos_dev, pos_host,
                                   _at(pos_table), rot, cos, sin, max_pos, _raw_stream(index)), "bt_kv8_append")
@@ -384,13 +400,13 @@ def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.T
 def kv8_read(kv: Sequence[torch.Tensor], n: int, first: int = 0, count: Optional[int] = None):
     """(k, v) [B, kv_heads, count, d]: rows [first, first + count) (default: to the end) of a layer of an 8-bit cache that holds ``n``
     rows, in the cache's dtype."""
-    cache, code = _kv8(kv)
+    cache, code, B, H, n_max, d, _ = _kv8(kv)
     count = n - first if count is None else count
-    if not 0 <= first <= first + count <= n <= cache.n_max:
-        raise _lib.BtError(f"rows [{first}, {first + count}) of {n} in a cache of {cache.n_max}")
+    if not 0 <= first <= first + count <= n <= n_max:
+        raise _lib.BtError(f"rows [{first}, {first + count}) of {n} in a cache of {n_max}")
     index = kv[0].get_device()
     with _on(index, *kv):
-        k = torch.empty(cache.batch, cache.kv_heads, count, cache.head_dim, dtype=kv[4].dtype, device=kv[0].device)
+        k = kv[4].new_empty(B, H, count, d)
         v = torch.empty_like(k)
         check(lib().bt_kv8_read(code, ctypes.byref(cache), n, first, count, k.data_ptr(), v.data_ptr(), _raw_stream(index)), "bt_kv8_read")
     return k, v
@@ -402,10 +418,9 @@ def attention_kv8(q: torch.Tensor, kv: Sequence[torch.Tensor], pos0, mask: Optio
     multiple of the cache's) sees the rows j <= pos0 + t with mask[b, j] != 0 (uint8 or bool [B, >= n]); zeros where none is left.  The
     rows pos0 .. pos0 + q_len - 1 are in the cache already.  ``n_split``: workgroups that share a head's rows (0: chosen from the sizes;
     with a device-side pos0 from the cache's size); ``ws``: >= bt_attention_kv8_workspace_bytes, allocated when needed and not given."""
-    cache, code = _kv8(kv)
-    B, q_len, H, d, dtype = cache.batch, q.shape[1] if q.dim() == 4 else 0, cache.kv_heads, cache.head_dim, kv[4].dtype
-    qr = _kv8_rows(q, "q", B, q_len, d, dtype)
-    heads = q.shape[2]
+    cache, code, B, H, n_max, d, dtype = _kv8(kv)
+    q_len = q.shape[1] if q.dim() == 4 else 0
+    qr, heads = _kv8_rows(q, "q", B, q_len, d, dtype)
     if q_len == 0 or heads == 0 or heads % H:
         raise _lib.BtError(f"{heads} query heads cannot share {H} key/value heads ({q_len} rows)")
     pos_dev, pos_host = _pos0(pos0)
@@ -414,16 +429,16 @@ def attention_kv8(q: torch.Tensor, kv: Sequence[torch.Tensor], pos0, mask: Optio
         if mask.dim() != 2 or mask.shape[0] != B or mask.dtype not in (torch.uint8, torch.bool) or mask.stride(1) != 1:
             raise _lib.BtError(f"mask must be uint8 or bool [{B}, rows] with unit inner stride")
         mask_ld = mask.stride(0) if B > 1 else mask.shape[1]
-        if mask.shape[1] < (cache.n_max if pos_dev else pos_host + q_len):
+        if mask.shape[1] < (n_max if pos_dev else pos_host + q_len):
             raise _lib.BtError("mask row too short")
     index = q.get_device()
     with _on(index, *kv, mask, out, ws, pos0 if pos_dev else None):
         if out is None:
-            out = torch.empty(B, q_len, heads, d, dtype=dtype, device=q.device)
+            out = torch.empty_like(q, memory_format=_CONTIGUOUS)
         elif out.shape != (B, q_len, heads, d) or out.dtype != dtype or not out.is_contiguous():
             raise _lib.BtError(f"out must be contiguous {dtype} [{B}, {q_len}, {heads}, {d}]")
         if n_split <= 0:
-            n_split = lib().bt_attention_kv8_split_count(B, H, heads // H, q_len, cache.n_max if pos_dev else pos_host + q_len)
+            n_split = lib().bt_attention_kv8_split_count(B, H, heads // H, q_len, n_max if pos_dev else pos_host + q_len)
         if ws is None and n_split > 1:
             need = int(lib().bt_attention_kv8_workspace_bytes(B, q_len, heads, d, n_split))
             ws = torch.empty(need, dtype=torch.uint8, device=q.device)
