@@ -235,7 +235,7 @@ def quantize_rows(x: torch.Tensor, ln_w: Optional[torch.Tensor] = None, ln_b: Op
     Kp = (K + 15) // 16 * 16
     code, index = dtype_code(x.dtype), x.get_device()
     with _on(index, ln_w, ln_b):
-        lead = x.shape[:-1]
+        lead = (M,) if x.dim() == 2 else x.shape[:-1]      # (a plain tuple makes the cheaper call)
         codes = x.new_empty(lead + (Kp,), dtype=torch.int8)
         scales = x.new_empty(lead, dtype=torch.float32)
         check(lib().bt_quant_rows(code, M, K, x.data_ptr(), ldx, _at(ln_w), _at(ln_b), eps, codes.data_ptr(), Kp, scales.data_ptr(),
@@ -277,7 +277,7 @@ def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight:
         raise _lib.BtError(f"unknown activation {act!r}")
     if bias is not None:
         _expect(bias, "bias", (N,), dtype)
-    shape = xc.shape[:-1] + (N,)
+    shape = (M, N) if xc.dim() == 2 else xc.shape[:-1] + (N,)
     ldr = 0
     if residual is not None:
         if residual.shape != shape or residual.dtype != dtype:
