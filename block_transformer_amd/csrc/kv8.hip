@@ -17,9 +17,10 @@ struct Rows {      // bt_kv8_rows on the device
 struct AppendArgs {
     bt_kv8_cache c;
     Rows q, q_out, k, v;
-    uint32_t kv_items;     // waves for keys and values: batch * kv_heads * blocks
+    uint32_t kv_items;     // waves for keys and values: batch * kv_heads * blocks << split
     uint32_t q_rows;       // batch * q_len * heads
     int blocks;            // blocks that q_len rows can touch
+    int split;             // keys and values of a block by a wave each (1), by one (0)
     int q_len, heads, rot, pos0_host;
     bool vec_rope;
     const int32_t* pos0_dev;
@@ -104,18 +105,18 @@ struct BlockMax {
     }
 };
 
-// One wave per (sequence, head, block) that the new rows touch; the waves behind them rotate q.
+// One wave per (sequence, head, block) that the new rows touch, or one for its K and one for its V (`split`); the waves behind them rotate q.
 //   K, q: a lane has 16-byte pieces of rows, four to a row, a quarter row apart: the rotary dims are then the same piece of every lane, and
 //         the fp64 work of the others is skipped.
 //   V: a lane has columns 2 x, 2 x + 1 of 16 rows, that is two 16-byte runs of v_codes: rows are read 256 bytes a wave and instruction,
 //      and no transpose is needed.  Rows of the open block come in runs from v_tail, which is transposed already.
-// Bound by memory; K and V are held in registers between the search for the scale and the codes, V's loads go out before K's work.
-// 32 sequences x 509 rows x 16 heads of 128 (333 MB) 97 us, 62 without q; a step that fills 4096 blocks of 16 rows 15 us, one that fills
-// none 8.4 us.
-constexpr int QU = 2;
+// K and V are held in registers between the search for the scale and the codes; five waves to a SIMD where that fits.  Bound by memory
+// and the chain load -> scale -> codes: 32 sequences x 509 rows x 16 heads of 128 (333 MB) 88 us (3.8 TB/s), the same in blocks of 32
+// 166 us (four waves to a SIMD); a step that fills 4096 blocks of 16 rows 15.5 us, one that fills none 7.5 us.
+constexpr int QU = 1;
 
 template <typename T, int D, int BL>
-__global__ __launch_bounds__(256, D * BL <= 2048 ? 4 : D * BL <= 4096 ? 3 : 1) void kv8_append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(256, D * BL <= 2048 ? 5 : D * BL <= 4096 ? 4 : 2) void kv8_append_kernel(AppendArgs a) {
     constexpr int V = Elem<T>::VEC, RP = D / V, LR = RP / 4;      // pieces of a row, lanes to a row
     const int lane = threadIdx.x & 63;
     const int pos0 = a.pos0_dev ? *a.pos0_dev : a.pos0_host;
@@ -123,7 +124,7 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 4 : D * BL <= 4096 ? 3 : 1) v
     const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int e_lane = lane % LR * V;      // piece k of this lane: dims e_lane + k D / 4
     if (item >= a.kv_items) {
-        // QU rows (b, t, h) of q a lane, their loads out together.  The last workgroup has waves too many, without q all of these are.
+        // QU rows (b, t, h) of q a lane.  The last workgroup has waves too many, without q all of these are.
         const uint32_t i0 = (item - a.kv_items) * (QU * 64 / LR);
         if (i0 >= a.q_rows) return;
         const T* src[QU];
@@ -158,8 +159,9 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 4 : D * BL <= 4096 ? 3 : 1) v
         return;
     }
     // neighbouring waves take neighbouring heads: of a fused projection's rows they read one piece of memory
-    const uint32_t bn = item / (uint32_t)a.c.kv_heads, b = bn / (uint32_t)a.blocks;
-    const int h = (int)(item - bn * a.c.kv_heads), nth = (int)(bn - b * a.blocks);
+    const uint32_t row = item / (uint32_t)a.c.kv_heads, bn = row >> a.split, b = bn / (uint32_t)a.blocks;
+    const bool values = !a.split || (row & 1), keys = !a.split || !(row & 1);
+    const int h = (int)(item - row * a.c.kv_heads), nth = (int)(bn - b * a.blocks);
     const uint32_t bh = b * a.c.kv_heads + h;
     const int64_t end = pos0 + (int64_t)a.q_len < a.c.n_max ? pos0 + (int64_t)a.q_len : a.c.n_max;
     const T* ksrc = (const T*)a.k.p + b * a.k.b + h * a.k.h;
@@ -173,20 +175,7 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 4 : D * BL <= 4096 ? 3 : 1) v
     if (row0 >= end) return;
     const int old = nth == 0 ? pos0 - (int)row0 : 0;          // rows of the block that stand in the tail
     if (row0 + BL <= end) {
-        constexpr int UNITS = D / 2 * (BL / 16), NU = (UNITS + 63) / 64;      // V: (pair of columns, run of 16 rows)
-        typedef typename std::conditional<sizeof(T) == 2, uint32_t, float2>::type Pair;
-        Pair raw[NU][16];
-#pragma unroll
-        for (int u = 0; u < NU; ++u) {
-            const int idx = u * 64 + lane, d = (idx % (D / 2)) * 2, t0 = idx / (D / 2) * 16;
-            const T* p = vsrc + (row0 - pos0 + t0) * a.v.t + d;
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                raw[u][e] = Pair{};
-                if (idx < UNITS && t0 + e >= old) raw[u][e] = *(const Pair*)(p + e * a.v.t);
-            }
-        }
-        {
+        if (keys) {
             constexpr int NR = BL * LR / 64 > 0 ? BL * LR / 64 : 1;      // rows of a lane
             float x[NR][4][V];
             BlockMax top;
@@ -248,7 +237,20 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 4 : D * BL <= 4096 ? 3 : 1) v
                 }
             }
         }
-        {
+        if (values) {
+            constexpr int UNITS = D / 2 * (BL / 16), NU = (UNITS + 63) / 64;      // V: (pair of columns, run of 16 rows)
+            typedef typename std::conditional<sizeof(T) == 2, uint32_t, float2>::type Pair;
+            Pair raw[NU][16];
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+                const int idx = u * 64 + lane, d = (idx % (D / 2)) * 2, t0 = idx / (D / 2) * 16;
+                const T* p = vsrc + (row0 - pos0 + t0) * a.v.t + d;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    raw[u][e] = Pair{};
+                    if (idx < UNITS && t0 + e >= old) raw[u][e] = *(const Pair*)(p + e * a.v.t);
+                }
+            }
             float x[NU][2][16];
             BlockMax top;
 #pragma unroll
@@ -313,15 +315,36 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 4 : D * BL <= 4096 ? 3 : 1) v
     if (nth != 0) return;
     const int64_t open0 = (int64_t)last * BL;
     const int from = open0 > pos0 ? 0 : (int)(pos0 - open0), to = (int)(end - open0);
-    for (int idx = from * RP + lane; idx < to * RP; idx += 64) {
+    for (int idx = from * RP + lane; keys && idx < to * RP; idx += 64) {
         const int t = idx / RP, e0 = (idx & (RP - 1)) * V;
         const int at = (int)(open0 + t - pos0);
         float v[V];
         rotated_piece<T>(a, ksrc + at * a.k.t, e0, a.rot ? angle_of(a, pos0 + at) : 0, v);
         store_vec<T>(kt + t * D + e0, v);
     }
-    for (int t = from; t < to; ++t)
-        for (int d = lane; d < D; d += 64) vt[d * BL + t] = vsrc[(open0 + t - pos0) * a.v.t + d];
+    if (values && to - from == 1) {
+        const T* p = vsrc + (open0 + from - pos0) * a.v.t;
+        for (int d = lane; d < D; d += 64) vt[d * BL + from] = p[d];
+    } else if (values && lane * 2 < D) {
+        // 16 rows in flight together
+        typedef typename std::conditional<sizeof(T) == 2, uint32_t, float2>::type Pair;
+        const int d = lane * 2;
+        for (int t0 = from & ~15; t0 < to; t0 += 16) {
+            const T* p = vsrc + (open0 + t0 - pos0) * a.v.t + d;
+            Pair raw[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (t0 + e >= from && t0 + e < to) raw[e] = *(const Pair*)(p + e * a.v.t);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (t0 + e >= from && t0 + e < to) {
+                    T two[2];
+                    __builtin_memcpy(two, &raw[e], sizeof two);
+                    vt[d * BL + t0 + e] = two[0];
+                    vt[(d + 1) * BL + t0 + e] = two[1];
+                }
+        }
+    }
 }
 
 // ---- bt_kv8_read -----------------------------------------------------------------------------------------------------------
@@ -995,7 +1018,10 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.v = rows_of(v);
     a.blocks = pos0_dev ? (q_len + cache->block - 2) / cache->block + 1
                         : (int)(((int64_t)pos0_host + q_len - 1) / cache->block - pos0_host / cache->block) + 1;
-    const int64_t kv_items = cache->batch * cache->kv_heads * a.blocks, q_rows = q ? cache->batch * q_len * heads : 0;
+    // Blocks that fill up have a wave for K and one for V, steps that fill none (or may: the device knows) one for both: 32 x 509 rows 88 us and 97,
+    // 8 x 100 9.8 and 14.9; a step of 256 sequences that fills no block 9.8 and 7.5.
+    a.split = pos0_dev ? q_len > 1 : ((int64_t)pos0_host + q_len) / cache->block > pos0_host / cache->block;
+    const int64_t kv_items = (cache->batch * cache->kv_heads * a.blocks) << a.split, q_rows = q ? cache->batch * q_len * heads : 0;
     BT_CHECK_ARG(kv_items < (1ll << 30) && q_rows < (1ll << 30), "bt_kv8_append: too many rows for one call");
     a.kv_items = (uint32_t)kv_items;
     a.q_rows = (uint32_t)q_rows;
