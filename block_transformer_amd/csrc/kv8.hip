@@ -30,9 +30,15 @@ struct AppendArgs {
     int64_t max_pos;
 };
 
-__device__ inline int64_t angle_of(const AppendArgs& a, int pos) {
-    // (rows behind the cache's end are dropped, but their queries are rotated all the same: not by what lies behind the table)
-    int64_t r = a.pos_table ? a.pos_table[pos < a.c.n_max ? pos : a.c.n_max - 1] : pos;
+// The entry of the position table for row t of a call at `pos0`, which the device may have read from anywhere: rows behind the cache's end
+// are dropped, but their queries are rotated all the same, by the table's last entry and not by what lies behind it.  (64 bits: pos0 + t
+// leaves an int.)
+__host__ __device__ constexpr int64_t table_entry(int64_t pos, int64_t n_max) { return pos < 0 ? 0 : pos < n_max ? pos : n_max - 1; }
+static_assert(table_entry((int64_t)INT32_MAX + 1, 64) == 63 && table_entry((int64_t)INT32_MAX + (1 << 30), 64) == 63);
+static_assert(table_entry(63, 64) == 63 && table_entry(64, 64) == 63 && table_entry(0, 64) == 0 && table_entry(INT32_MIN, 64) == 0);
+
+__device__ inline int64_t angle_of(const AppendArgs& a, int64_t pos) {
+    int64_t r = a.pos_table ? a.pos_table[table_entry(pos, a.c.n_max)] : pos;
     r = r < 0 ? 0 : r;
     return r < a.max_pos ? r : a.max_pos - 1;
 }
@@ -129,7 +135,7 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 5 : D * BL <= 4096 ? 4 : 2) v
         if (i0 >= a.q_rows) return;
         const T* src[QU];
         T* dst[QU];
-        int pos[QU];
+        int64_t pos[QU];
         bool there[QU];
         float v[QU][4][V];
 #pragma unroll
@@ -141,7 +147,7 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 5 : D * BL <= 4096 ? 4 : 2) v
             const int h = (int)(i - bt * a.heads), t = (int)(bt - b * a.q_len);
             src[u] = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
             dst[u] = (T*)a.q_out.p + b * a.q_out.b + t * a.q_out.t + h * a.q_out.h;
-            pos[u] = pos0 + t;
+            pos[u] = (int64_t)pos0 + t;
 #pragma unroll
             for (int k = 0; k < 4; ++k) load_vec<T>(src[u] + e_lane + k * (D / 4), v[u][k]);
         }
@@ -200,7 +206,7 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 5 : D * BL <= 4096 ? 4 : 2) v
                     const int e0 = e_lane + k * (D / 4);
                     if (t < BL && t >= old && e0 < a.rot) {
                         const int at = (int)(row0 + t - pos0);
-                        rotated_piece<T>(a, ksrc + at * a.k.t, e0, angle_of(a, pos0 + at), x[i][k]);
+                        rotated_piece<T>(a, ksrc + at * a.k.t, e0, angle_of(a, (int64_t)pos0 + at), x[i][k]);
                         round_piece<T>(x[i][k]);
                     }
 #pragma unroll
@@ -319,7 +325,7 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 5 : D * BL <= 4096 ? 4 : 2) v
         const int t = idx / RP, e0 = (idx & (RP - 1)) * V;
         const int at = (int)(open0 + t - pos0);
         float v[V];
-        rotated_piece<T>(a, ksrc + at * a.k.t, e0, a.rot ? angle_of(a, pos0 + at) : 0, v);
+        rotated_piece<T>(a, ksrc + at * a.k.t, e0, a.rot ? angle_of(a, (int64_t)pos0 + at) : 0, v);
         store_vec<T>(kt + t * D + e0, v);
     }
     if (values && to - from == 1) {
