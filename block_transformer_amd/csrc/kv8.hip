@@ -467,7 +467,8 @@ struct AttnArgs {
     float scale;      // log2(e) / sqrt(head_dim)
 };
 
-constexpr float M_FLOOR = -1e30f;      // "no score yet": finite, so that differences of two of them are 0
+// "no score yet": the lowest finite number, so that a difference of two of them is 0 and no score of a row that is seen lies below
+constexpr float M_FLOOR = -3.402823466e38f;
 
 template <typename T, int D>
 struct Attend {
