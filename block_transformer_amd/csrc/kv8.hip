@@ -432,24 +432,25 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(bt_kv8_cache c, int64_t n
 }
 
 // ---- bt_attention_kv8 ------------------------------------------------------------------------------------------------------
-// The cache's codes are multiplied as they are, by v_mfma_i32_16x16x64_i8: q is written as 8-bit digits, q = (amax / Q) sum_i 256^(ND-1-i)
-// dig_i with Q = 127 * 256^(ND-1) -- two digits for bf16 (an error of 2^-16 of the row's largest, bf16 itself has 2^-9), three for fp32 --
-// and so are the probabilities (three digits).  No code is converted, so a byte of the cache costs one load and 1/64 of a matrix
-// instruction per 16 query rows, and the kernel is bound by reading the cache.
+// The arithmetic of an fp32 attention on the bf16 matrix instructions.  A code is an exact bf16, q and the probabilities (times their rows' V
+// scales) enter as the one or three bf16 whose sum they are, so products are exact and sums fp32: small probabilities beside a large one,
+// blocks of different scales and queries with outliers keep all their bits.  (Digits of a fixed point for a tile do not: a row of
+// e^-17 of the largest weight was lost.)
 //
 // A wave works on 16 query rows (rows x heads that share a KV head) and 64 cached rows at a time:
-//   S^T = K Q^T   A = K: lane (m = lane & 15, g = lane >> 4) holds 16 bytes of row tok(i, m) = 16 (m >> 2) + 4 i + (m & 3), i = 0 .. 3.
+//   S^T = K Q^T   A = K: lane (m = lane & 15, g = lane >> 4) holds 16 bytes (8 of 32 dims) of row tok(i, m) = 16 (m >> 2) + 4 i + (m & 3),
+//                 i = 0 .. 3; 8 of them are one operand of v_mfma_f32_16x16x32_bf16 (its k-range 8 g .. 8 g + 7: the dims that q has there).
 //                 In the result lane (query c = lane & 15, g) holds rows 16 g + 4 i + r, r = 0 .. 3: 16 consecutive rows, one block's
 //                 scale, one 16-byte piece of the mask.
-//   O^T = V^T P^T B = P: the lane's own 16 rows are exactly the k-range 16 g .. 16 g + 15 it has to supply: nothing moves between lanes.
-//                 A = V^T: lane m holds 16 consecutive rows of dim 16 j + m, one 16-byte load from v_codes.
-// Softmax: every 64-row tile has its own largest score as the base of its digits (a far larger score elsewhere costs them nothing), and
-// enters a running (max, sum, output) in fp32.  The rows' V scales go into the probabilities, relative to the tile's largest.
-// The open block is one more tile: bf16 or fp32 matrix instructions on its rows as they stand, probabilities as two bf16 (16 bits) or
-// one fp32.
-// Bound by reading the cache where there is enough of it: 1024 sequences x 16 heads of 128 x 543 rows 402 us (5.86 TB/s; the card reads 6.0),
-// 256 sequences 112 us (5.25), 4 sequences x 32773 rows, 8 heads to a KV head, 30 us (4.5).  A tile costs about 430 vector and 40 matrix
-// instructions for its 16 KB, a quarter of what would bound it.  One sequence of 21 rows: 6.7 us, three round trips to memory.
+//   O^T = V^T P^T B = P: the lane's own 16 rows are two operands: nothing moves between lanes.
+//                 A = V^T: lane m holds the same 16 consecutive rows of dim 16 j + m, one 16-byte load from v_codes.
+// Softmax: a running (max, sum, output) in fp32.  The open block is one more tile, its rows as they stand (fp32: v_mfma_f32_16x16x4_f32).
+// Bound by reading the cache where there is enough of it: 1024 sequences x 16 heads of 128 x 543 rows 407 .. 421 us (5.6 .. 5.8 TB/s; the
+// card reads 6.0), 256 sequences 113 .. 119 us (5.2), 4 sequences x 32773 rows, 8 heads to a KV head, 30 us with the join (4.5).  A tile
+// costs about 710 vector instructions (over half of them turn codes into bf16) and 64 matrix instructions for its 16 KB, under half of
+// what would bound it; with one wave to a SIMD that shows: 8 sequences x 24608 rows x 2 heads of 64, 20 query rows each, 24 us, where the
+// fixed-point form took 20.5.  One sequence of 21 rows: 6.2 us, three round trips to memory.
+typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -470,12 +471,40 @@ struct AttnArgs {
 // "no score yet": the lowest finite number, so that a difference of two of them is 0 and no score of a row that is seen lies below
 constexpr float M_FLOOR = -3.402823466e38f;
 
+// The numbers of a pair of floats as NP bf16 each, largest first: what the first has cut off goes to the next, so three are exact.
+template <int NP>
+__device__ inline void cut_bf16x2(float x0, float x1, uint32_t (&out)[NP]) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+        out[p] = __builtin_amdgcn_perm(__float_as_uint(x1), __float_as_uint(x0), 0x07060302);
+        x0 -= __uint_as_float(__float_as_uint(x0) & 0xffff0000u);
+        x1 -= __uint_as_float(__float_as_uint(x1) & 0xffff0000u);
+    }
+}
+
+// eight codes as bf16
+__device__ inline bf16x8 codes_bf16(int w0, int w1) {
+    union { uint32_t u[4]; bf16x8 f; } r;
+    const int w[2] = {w0, w1};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int x = w[i >> 1], at = 16 * (i & 1);
+        r.u[i] = __builtin_amdgcn_perm(__float_as_uint((float)(int8_t)(x >> (at + 8))), __float_as_uint((float)(int8_t)(x >> at)), 0x07060302);
+    }
+    return r.f;
+}
+
 template <typename T, int D>
 struct Attend {
-    static constexpr int ND = sizeof(T) == 2 ? 2 : 3;       // digits of q
+    static constexpr int NQ = sizeof(T) == 2 ? 1 : 3;       // bf16 numbers to an element of q
     static constexpr int NC = (D + 63) / 64;                // 64-dim pieces of a row of K
+    static constexpr int NH = D >= 64 ? 2 : 1;              // operands of a lane's part of a piece, 8 dims each
     static constexpr int NJ = D / 16;                       // 16-dim pieces of the output
-    static constexpr int PD = 127 * 65536;                  // full scale of a probability's three digits
+    typedef typename std::conditional<D >= 64, i32x4, i32x2>::type KPart;
+    union Operand {
+        uint32_t u[4];
+        bf16x8 f;
+    };
 
     const AttnArgs& a;
     const int lane, c, g;
@@ -485,8 +514,9 @@ struct Attend {
     const uint8_t* mask;
     const T* q;
     int64_t lim;              // rows that this lane's query sees
-    float qs = 0.f;           // what one unit of its integer scores stands for, times a.scale
-    i32x4 dig[ND][NC];
+    int up = 0;               // q is held times 2^-up, so that its products with codes stay in fp32
+    float poison = 0.f;       // NaN where q has an infinity or NaN, else 0
+    Operand qf[NQ][NC][NH];
     float m = M_FLOOR, l = 0.f;
     f32x4 o[NJ];
 
@@ -495,15 +525,14 @@ struct Attend {
     __device__ inline void load_query(bool real) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) o[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-        float x[NC][16];
+        float x[NC][8 * NH];
         float amax = 0.f, bad = 0.f;
-        const bool mine = real && (D >= 64 || g < 2);
 #pragma unroll
         for (int k = 0; k < NC; ++k) {
 #pragma unroll
-            for (int e = 0; e < 16; e += Elem<T>::VEC) {
+            for (int e = 0; e < 8 * NH; e += Elem<T>::VEC) {
                 float v[Elem<T>::VEC] = {};
-                if (mine) load_vec<T>(q + 64 * k + 16 * g + e, v);
+                if (real) load_vec<T>(q + 64 * k + 8 * NH * g + e, v);
 #pragma unroll
                 for (int i = 0; i < Elem<T>::VEC; ++i) {
                     x[k][e + i] = v[i];
@@ -514,40 +543,27 @@ struct Attend {
         }
         amax = max_over_groups(amax);
         bad = max_over_groups(bad);
-        const float up = amax < 1e-30f ? 0x1p64f : 1.0f;     // keeps Q / amax finite
-        constexpr float Q = ND == 2 ? 127.f * 256.f : 127.f * 65536.f;
-        const float inv = amax > 0.f ? Q / (amax * up) : 0.f;
-        qs = bad != 0.f ? __int_as_float(0x7fc00000) : amax / Q * a.scale;
+        poison = bad != 0.f ? __int_as_float(0x7fc00000) : 0.f;
+        up = bad != 0.f ? 0 : __builtin_amdgcn_frexp_expf(amax);
 #pragma unroll
-        for (int k = 0; k < NC; ++k) {
+        for (int k = 0; k < NC; ++k)
 #pragma unroll
-            for (int w = 0; w < 4; ++w) {
-                uint32_t v[4];      // the number plus 128 for every lower digit: its bytes are the digits, the lower ones with 128 on top
+            for (int e = 0; e < 8 * NH; e += 2) {
+                uint32_t two[NQ];
+                cut_bf16x2<NQ>(bad != 0.f ? poison : ldexpf(x[k][e], -up), bad != 0.f ? poison : ldexpf(x[k][e + 1], -up), two);
 #pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    v[e] = bad != 0.f ? (ND == 2 ? 0x80u : 0x8080u) : (uint32_t)((int)rintf(x[k][4 * w + e] * up * inv) + (ND == 2 ? 0x80 : 0x8080));
-                const uint32_t a01 = __builtin_amdgcn_perm(v[1], v[0], 0x05010400), a23 = __builtin_amdgcn_perm(v[3], v[2], 0x05010400);
-                const uint32_t b0 = __builtin_amdgcn_perm(a23, a01, 0x05040100), b1 = __builtin_amdgcn_perm(a23, a01, 0x07060302);
-                if (ND == 2) {
-                    dig[0][k][w] = (int)b1;
-                } else {
-                    const uint32_t c01 = __builtin_amdgcn_perm(v[1], v[0], 0x06020602), c23 = __builtin_amdgcn_perm(v[3], v[2], 0x06020602);
-                    dig[0][k][w] = (int)__builtin_amdgcn_perm(c23, c01, 0x05040100);
-                    dig[1][k][w] = (int)(b1 ^ 0x80808080u);
-                }
-                dig[ND - 1][k][w] = (int)(b0 ^ 0x80808080u);
+                for (int p = 0; p < NQ; ++p) qf[p][k][e >> 3].u[(e & 7) >> 1] = two[p];
             }
-        }
     }
 
-    __device__ inline void load_k(int64_t tile, i32x4 (&k)[4][NC]) const {
+    __device__ inline void load_k(int64_t tile, KPart (&k)[4][NC]) const {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             int64_t tok = tile * 64 + 16 * (c >> 2) + 4 * i + (c & 3);
             tok = tok < a.c.n_max ? tok : a.c.n_max - 1;
-            const int8_t* p = kc + tok * D + 16 * (D >= 64 ? g : g & 1);      // D = 32: the upper lanes' digits are zero
+            const int8_t* p = kc + tok * D + 8 * NH * g;
 #pragma unroll
-            for (int n = 0; n < NC; ++n) k[i][n] = *(const i32x4*)(p + 64 * n);
+            for (int n = 0; n < NC; ++n) k[i][n] = *(const KPart*)(p + 64 * n);
         }
     }
     // the scales and the mask of this lane's 16 rows of a tile
@@ -589,10 +605,9 @@ struct Attend {
         return (1u << most) - 1u;
     }
 
-    // enters a tile with its largest score mt: the factor for what is there already; `gamma` for what comes
-    __device__ inline float enter(float mt, float& gamma) {
+    // enters a tile with its largest score: the factor for what is there already
+    __device__ inline float enter(float mt) {
         const float mn = fmaxf(m, mt), alpha = __builtin_amdgcn_exp2f(m - mn);
-        gamma = __builtin_amdgcn_exp2f(mt - mn);
         m = mn;
         return alpha;
     }
@@ -600,27 +615,26 @@ struct Attend {
     // One tile.  `k` and `v` hold it; MORE: the next tile's take their places as soon as they have been used, K under the softmax and
     // the second product, V under the next tile's first.
     template <bool MORE>
-    __device__ inline void tile(int64_t at, int64_t then, i32x4 (&k)[4][NC], i32x4 (&v)[NJ], Side& side, bool cut) {
+    __device__ inline void tile(int64_t at, int64_t then, KPart (&k)[4][NC], i32x4 (&v)[NJ], Side& side, bool cut) {
         const int64_t tok0 = at * 64 + 16 * g;
         const Side now = side;
         if (MORE) side = load_side(then);
-        const float mul = qs * now.sk;
+        const float mul = ldexpf(a.scale * now.sk, up);
         float sv = now.sv;
         float s[4][4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            i32x4 acc{0, 0, 0, 0}, low{0, 0, 0, 0};
+            f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int n = 0; n < NC; ++n) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i][n], dig[0][n], acc, 0, 0, 0);
-            acc <<= 8;
+            for (int n = 0; n < NC; ++n)
 #pragma unroll
-            for (int n = 0; n < NC; ++n) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i][n], dig[1][n], acc, 0, 0, 0);
-            if (ND == 3) {
+                for (int h = 0; h < NH; ++h) {
+                    const bf16x8 kf = codes_bf16(k[i][n][2 * h], k[i][n][2 * h + 1]);
 #pragma unroll
-                for (int n = 0; n < NC; ++n) low = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[i][n], dig[ND - 1][n], low, 0, 0, 0);
-            }
+                    for (int p = NQ - 1; p >= 0; --p) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[p][n][h].f, acc, 0, 0, 0);
+                }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[i][r] = (ND == 3 ? fmaf((float)acc[r], 256.f, (float)low[r]) : (float)acc[r]) * mul;
+            for (int r = 0; r < 4; ++r) s[i][r] = acc[r] * mul;
         }
         if (MORE) load_k(then, k);
         if (cut) {
@@ -637,39 +651,31 @@ struct Attend {
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) mt = fmaxf(mt, s[i][r]);
-        mt = max_over_groups(mt);
-        const float top = max_over_groups(sv);
-        const float rel = top > 0.f ? sv / top : 0.f;
-        float gamma, sum = 0.f;
-        const float alpha = enter(mt, gamma);
-        i32x4 p[3];
+        const float alpha = enter(max_over_groups(mt));
+        float sum = 0.f;
+        Operand p[3][2];      // rows 8 h .. 8 h + 7 of the lane's 16
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t f[4];
+        for (int e = 0; e < 16; e += 2) {
+            const float e0 = __builtin_amdgcn_exp2f(s[e >> 2][e & 3] - m), e1 = __builtin_amdgcn_exp2f(s[e >> 2][(e & 3) + 1] - m);
+            sum += e0;
+            sum += e1;
+            uint32_t two[3];
+            cut_bf16x2<3>(e0 * sv, e1 * sv, two);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float e = __builtin_amdgcn_exp2f(s[i][r] - mt);
-                sum += e;
-                // the three digits as the bytes of a float's mantissa: 2^23 + N, N = P + 0x8080, P = round(p PD)
-                f[r] = __float_as_uint(fmaf(e * rel, (float)PD, 8388608.f + 32896.f));
-            }
-            const uint32_t a01 = __builtin_amdgcn_perm(f[1], f[0], 0x05010400), a23 = __builtin_amdgcn_perm(f[3], f[2], 0x05010400);
-            const uint32_t b01 = __builtin_amdgcn_perm(f[1], f[0], 0x06020602), b23 = __builtin_amdgcn_perm(f[3], f[2], 0x06020602);
-            p[0][i] = (int)__builtin_amdgcn_perm(b23, b01, 0x05040100);
-            p[1][i] = (int)(__builtin_amdgcn_perm(a23, a01, 0x07060302) ^ 0x80808080u);
-            p[2][i] = (int)(__builtin_amdgcn_perm(a23, a01, 0x05040100) ^ 0x80808080u);
+            for (int x = 0; x < 3; ++x) p[x][e >> 3].u[(e & 7) >> 1] = two[x];
         }
-        l = fmaf(l, alpha, sum * gamma);
-        const float beta = top * gamma * (1.0f / (float)PD), beta256 = beta * 256.f;
+        l = fmaf(l, alpha, sum);
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            i32x4 acc{0, 0, 0, 0}, low{0, 0, 0, 0};
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[j], p[0], acc, 0, 0, 0);
-            low = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[j], p[2], low, 0, 0, 0);
-            acc <<= 8;
-            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(v[j], p[1], acc, 0, 0, 0);
+            f32x4 acc{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[j][r] = fmaf((float)acc[r], beta256, fmaf((float)low[r], beta, o[j][r] * alpha));
+            for (int h = 0; h < 2; ++h) {
+                const bf16x8 vf = codes_bf16(v[j][2 * h], v[j][2 * h + 1]);
+#pragma unroll
+                for (int x = 2; x >= 0; --x) acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, p[x][h].f, acc, 0, 0, 0);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[j][r] = fmaf(o[j][r], alpha, acc[r]);
         }
         if (MORE) load_v(then, v);
     }
@@ -704,7 +710,7 @@ struct Attend {
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s[i][r] = acc[r] * a.scale;
+            for (int r = 0; r < 4; ++r) s[i][r] = fmaf(acc[r], a.scale, poison);
         }
         const int64_t tok0 = n_full + per * g;
         const int there = end - tok0 < per ? (end > tok0 ? (int)(end - tok0) : 0) : per;
@@ -720,14 +726,13 @@ struct Attend {
                 s[i][r] = (on >> (4 * i + r)) & 1 ? s[i][r] : -INFINITY;
                 mt = fmaxf(mt, s[i][r]);
             }
-        mt = max_over_groups(mt);
-        float gamma, sum = 0.f;
-        const float alpha = enter(mt, gamma);
+        const float alpha = enter(max_over_groups(mt));
+        float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                s[i][r] = __builtin_amdgcn_exp2f(s[i][r] - mt) * gamma;
+                s[i][r] = __builtin_amdgcn_exp2f(s[i][r] - m);
                 sum += s[i][r];
             }
         l = fmaf(l, alpha, sum);
@@ -736,6 +741,16 @@ struct Attend {
         uint32_t keep[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) keep[e] = (some >> e) & 1 ? ~0u : 0u;
+        Operand p[3][2];      // bf16: the probabilities in three pieces, rows 8 h .. 8 h + 7 of the lane's
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+                uint32_t two[3];
+                cut_bf16x2<3>(s[e >> 2][e & 3], s[e >> 2][(e & 3) + 1], two);
+#pragma unroll
+                for (int x = 0; x < 3; ++x) p[x][e >> 3].u[(e & 7) >> 1] = two[x];
+            }
+        }
         float zero = 0.f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -743,19 +758,15 @@ struct Attend {
             const T* vr = vt + (16 * j + c) * bl + per * g;
             if constexpr (sizeof(T) == 2) {
 #pragma unroll
-                for (int h = 0; h < 16; h += 8) {
-                    if (h >= per) continue;
-                    union { uint32_t u[4]; bf16x8 f; } vf, hi, lo;
+                for (int h = 0; h < 2; ++h) {
+                    if (8 * h >= per) continue;      // per is 4, 8 or 16
+                    Operand vf;
+                    const uint2 low = *(const uint2*)(vr + 8 * h), high = per > 4 ? *(const uint2*)(vr + 8 * h + 4) : uint2{0, 0};
+                    const uint32_t four[4] = {low.x, low.y, high.x, high.y};
 #pragma unroll
-                    for (int e = 0; e < 8; e += 2) {
-                        const float p0 = s[(h + e) >> 2][(h + e) & 3], p1 = s[(h + e + 1) >> 2][(h + e + 1) & 3];
-                        vf.u[e >> 1] = h + e < per ? *(const uint32_t*)(vr + h + e) : 0u;      // per is 4, 8 or 16
-                        vf.u[e >> 1] &= __builtin_amdgcn_perm(keep[h + e + 1], keep[h + e], 0x05040100);
-                        hi.u[e >> 1] = pack_bf16x2(p0, p1);
-                        lo.u[e >> 1] = pack_bf16x2(p0 - __uint_as_float(hi.u[e >> 1] << 16), p1 - __uint_as_float(hi.u[e >> 1] & 0xffff0000u));
-                    }
-                    o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.f, hi.f, o[j], 0, 0, 0);
-                    o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.f, lo.f, o[j], 0, 0, 0);
+                    for (int e = 0; e < 4; ++e) vf.u[e] = four[e] & __builtin_amdgcn_perm(keep[8 * h + 2 * e + 1], keep[8 * h + 2 * e], 0x05040100);
+#pragma unroll
+                    for (int x = 2; x >= 0; --x) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf.f, p[x][h].f, o[j], 0, 0, 0);
                 }
             } else {
 #pragma unroll
@@ -800,12 +811,10 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kv8_kernel(AttnArgs a) {
     __shared__ float merged[NW > 1 ? NW : 1][NW > 1 ? 16 : 1][D + 4];
     const int wave = NW > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
     A w(a);
-    int64_t id = blockIdx.x;
-    const int split = (int)(id % a.n_split);
-    id /= a.n_split;
-    const int rg = (int)(id % a.row_groups);
-    w.bh = id / a.row_groups;
-    const int64_t b = w.bh / a.c.kv_heads;
+    const uint32_t part = blockIdx.x / (uint32_t)a.n_split, head = part / (uint32_t)a.row_groups;
+    const int split = (int)(blockIdx.x - part * (uint32_t)a.n_split), rg = (int)(part - head * (uint32_t)a.row_groups);
+    w.bh = head;
+    const int64_t b = head / (uint32_t)a.c.kv_heads;
     const int h0 = (int)(w.bh - b * a.c.kv_heads) * a.share;
     const int pos0 = a.pos0_dev ? *a.pos0_dev : a.pos0_host;
     const int row = rg * 16 + w.c;
@@ -833,7 +842,8 @@ __global__ __launch_bounds__(NW * 64, 2) void attention_kv8_kernel(AttnArgs a) {
     int64_t at = split * per + wave;
     const int64_t stop = (split + 1) * per < all ? (split + 1) * per : all, closed_stop = stop < tiles ? stop : tiles;
     if (at < closed_stop) {
-        i32x4 k[4][A::NC], v[A::NJ];
+        typename A::KPart k[4][A::NC];
+        i32x4 v[A::NJ];
         typename A::Side side = w.load_side(at);
         w.load_k(at, k);
         w.load_v(at, v);

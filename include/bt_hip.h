@@ -306,9 +306,8 @@ int bt_kv8_read(int dtype, const bt_kv8_cache* cache, int64_t n, int64_t first, 
 
 /* Causal softmax attention over the cache: query row t of head h sees rows j <= pos0 + t (j < n_max) of head h / (heads / kv_heads) with
  * mask[b, j] != 0 (mask may be NULL);  out[(b * q_len + t) * ldo + h * head_dim + :], zeros where nothing is left to see.  The rows
- * pos0 .. pos0 + q_len - 1 have been appended; hidden rows may hold anything, blocks that are hidden as a whole any scale too.  q (two
- * 8-bit digits for bf16, three for fp32) and the probabilities (three digits) are multiplied with the codes themselves: exact int32
- * sums over 64 rows, fp32 across them.
+ * pos0 .. pos0 + q_len - 1 have been appended; hidden rows may hold anything, blocks that are hidden as a whole any scale too.  The
+ * arithmetic is that of fp32: q, codes and probabilities are multiplied with all their bits, sums are fp32 (scores have to stay within it).
  * n_split > 1 splits the rows over that many workgroups (bt_attention_kv8_split_count gives a good number for a batch; it depends on
  * its arguments alone) and needs a workspace of bt_attention_kv8_workspace_bytes(...).  mask_ld >= pos0_host + q_len, or >= n_max with
  * a device-side pos0. */
