@@ -114,7 +114,11 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
             load_piece<T>(w, c, K, wv);
             load_piece<T>(b, c, K, bv);
 #pragma unroll
-            for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, wv[e], bv[e]);      // 0 beyond K, as wv and bv are
+            for (int e = 0; e < V; ++e) v[i][e] = fmaf(v[i][e] * rstd, wv[e], bv[e]);
+            if (c + V > K) {      // (a weight of 0 does not make it 0: -mean * rstd may be infinite)
+#pragma unroll
+                for (int e = 0; e < V; ++e) v[i][e] = c + e < K ? v[i][e] : 0.f;
+            }
         }
     }
     float amax = 0.f, zero = 0.f;      // (0 * v is 0 unless v is an infinity or NaN)

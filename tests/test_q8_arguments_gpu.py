@@ -1,0 +1,27 @@
+"""Calls of the 8-bit operators that their documentation allows."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from block_transformer_amd import ops  # noqa: E402
+from block_transformer_amd.runtime import KV8Cache  # noqa: E402
+from oracle import q8_ref as ref  # noqa: E402
+
+DEV = "cuda"
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+@pytest.mark.parametrize("K", [1, 5, 13, 515, 2047])
+@pytest.mark.parametrize("M", [1, 5, 3000])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_layernorm_of_large_constant_rows(M, K, dtype):
+    """What a lane holds behind the row's end does not count: (0 - mean) * rstd may leave fp32 there.  The rows are one power of two, so that
+    sums, mean and differences are exact whatever their order: the LayerNorm of such a row is its bias, to the last bit."""
+    x = torch.full((M, K), 2.0 ** (126 - K.bit_length()), dtype=dtype)
+    g = torch.Generator().manual_seed(K)
+    w, b = torch.randn(K, generator=g).to(dtype), torch.randn(K, generator=g).to(dtype)
+    c, s = ops.quantize_rows(x.to(DEV), w.to(DEV), b.to(DEV), eps=1e-12)
+    want, scale = ref.quantize_rows(b[None])
+    assert (s.cpu().double() == scale).all()
+    assert (c.cpu()[:, :K].double() == want).all() and not c[:, K:].any()
