@@ -223,7 +223,8 @@ def _expect(t: torch.Tensor, what: str, shape, dtype) -> None:
 def quantize_rows(x: torch.Tensor, ln_w: Optional[torch.Tensor] = None, ln_b: Optional[torch.Tensor] = None, eps: float = 1e-5):
     """(codes, scales) of the rows of ``x`` [..., K] -- of LayerNorm(x; ln_w, ln_b, eps) if weights are given -- in 8-bit integers with one
     scale per row: codes int8 [..., round_up(K, 16)] (zero behind column K), scales float32 [...].  Activations and weights alike:
-    ``quantize_rows(weight)`` has one scale per output channel.  A row with an infinity or NaN in it gets scale NaN."""
+    ``quantize_rows(weight)`` has one scale per output channel.  A row with an infinity or NaN in it gets scale NaN.  ``codes.columns`` is K
+(views of the codes do not have it)."""
     M, K, ldx = _flat(x)
     if K == 0:
         raise _lib.BtError("rows are empty")
@@ -240,6 +241,7 @@ def quantize_rows(x: torch.Tensor, ln_w: Optional[torch.Tensor] = None, ln_b: Op
         scales = x.new_empty(lead, dtype=torch.float32)
         check(lib().bt_quant_rows(code, M, K, x.data_ptr(), ldx, _at(ln_w), _at(ln_b), eps, codes.data_ptr(), Kp, scales.data_ptr(),
                                   _raw_stream(index)), "bt_quant_rows")
+    codes.columns = K
     return codes, scales
 
 
@@ -248,16 +250,20 @@ def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight:
               out: Optional[torch.Tensor] = None, dtype: Optional[torch.dtype] = None, scratch: Optional[torch.Tensor] = None):
     """out = act(x @ weight.T + bias) + residual in 8-bit integers with scales per token and per output channel.  ``x``: rows in fp32 or
     bf16 (quantised here) or the (codes, scales) that ``quantize_rows`` made of them; ``weight``: ``quantize_rows`` of the nn.Linear
-    weight [N, K].  The sum over K is exact; ``dtype`` (default: that of x, bias, residual or out, whichever is a float tensor) is the
+    weight [N, K]; both have to have the same K (of codes that do not say theirs -- ``codes.columns`` -- only round_up(K, 16) is compared).
+    The sum over K is exact; ``dtype`` (default: that of x, bias, residual or out, whichever is a float tensor) is the
     type of bias, residual and result.  ``scratch`` (any dtype, >= bt_linear_q8_scratch_bytes) is allocated when it is needed and not
     given."""
     wc, ws = weight
+    columns = getattr(wc, "columns", None)
     if isinstance(x, torch.Tensor):
         dtype = dtype or x.dtype
-        if x.shape[-1] > wc.shape[-1] or (x.shape[-1] + 15) // 16 * 16 != wc.shape[-1]:
-            raise _lib.BtError(f"x has {x.shape[-1]} columns, the weight's rows of codes {wc.shape[-1]}")
+        if (x.shape[-1] + 15) // 16 * 16 != wc.shape[-1] or columns not in (None, x.shape[-1]):
+            raise _lib.BtError(f"x has {x.shape[-1]} columns, the weight {columns or wc.shape[-1]}")
         x = quantize_rows(x)
     xc, xs = x
+    if columns is not None and getattr(xc, "columns", columns) != columns:
+        raise _lib.BtError(f"x has {xc.columns} columns, the weight {columns}")
     if dtype is None:
         dtype = next((t.dtype for t in (out, residual, bias) if t is not None), None)
         if dtype is None:

@@ -5,6 +5,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from block_transformer_amd import ops  # noqa: E402
+from block_transformer_amd._lib import BtError  # noqa: E402
 from block_transformer_amd.runtime import KV8Cache  # noqa: E402
 from oracle import q8_ref as ref  # noqa: E402
 
@@ -25,3 +26,13 @@ def test_layernorm_of_large_constant_rows(M, K, dtype):
     want, scale = ref.quantize_rows(b[None])
     assert (s.cpu().double() == scale).all()
     assert (c.cpu()[:, :K].double() == want).all() and not c[:, K:].any()
+
+
+def test_quantised_rows_say_how_many_columns_they_have():
+    x, w = torch.randn(3, 515, device=DEV), torch.randn(8, 520, device=DEV)
+    cx, cw = ops.quantize_rows(x), ops.quantize_rows(w)
+    assert cx[0].columns == 515 and cw[0].columns == 520
+    for rows in (x, cx):
+        with pytest.raises(BtError, match="515 columns, the weight 520"):
+            ops.linear_q8(rows, cw, dtype=F32)
+    assert torch.equal(ops.linear_q8(x, ops.quantize_rows(w[:, :515])), ops.linear_q8(cx, ops.quantize_rows(w[:, :515]), dtype=F32))
