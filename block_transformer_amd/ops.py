@@ -220,6 +220,12 @@ def _expect(t: torch.Tensor, what: str, shape, dtype) -> None:
         raise _lib.BtError(f"{what} must be contiguous {dtype} {tuple(shape)}, got {t.dtype} {tuple(t.shape)} with strides {t.stride()}")
 
 
+def _flat_memory(t: Optional[torch.Tensor], what: str) -> None:
+    """A workspace's bytes are counted by its elements: they have to lie one behind the other."""
+    if t is not None and not t.is_contiguous():
+        raise _lib.BtError(f"{what} must be contiguous")
+
+
 def quantize_rows(x: torch.Tensor, ln_w: Optional[torch.Tensor] = None, ln_b: Optional[torch.Tensor] = None, eps: float = 1e-5):
     """(codes, scales) of the rows of ``x`` [..., K] -- of LayerNorm(x; ln_w, ln_b, eps) if weights are given -- in 8-bit integers with one
     scale per row: codes int8 [..., round_up(K, 16)] (zero behind column K), scales float32 [...].  Activations and weights alike:
@@ -289,6 +295,7 @@ def linear_q8(x: Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]], weight:
         if residual.shape != shape or residual.dtype != dtype:
             raise _lib.BtError(f"residual must be {dtype} {tuple(shape)}")
         ldr = _flat(residual)[2]
+    _flat_memory(scratch, "scratch")
     index = xc.get_device()
     with _on(index, xs, wc, ws, bias, residual, out, scratch):
         if out is None:
@@ -437,6 +444,7 @@ def attention_kv8(q: torch.Tensor, kv: Sequence[torch.Tensor], pos0, mask: Optio
         mask_ld = mask.stride(0) if B > 1 else mask.shape[1]
         if mask.shape[1] < (n_max if pos_dev else pos_host + q_len):
             raise _lib.BtError("mask row too short")
+    _flat_memory(ws, "ws")
     index = q.get_device()
     with _on(index, *kv, mask, out, ws, pos0 if pos_dev else None):
         if out is None:

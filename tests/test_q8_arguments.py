@@ -4,6 +4,7 @@ import torch
 
 from block_transformer_amd import ops
 from block_transformer_amd._lib import BtError
+from block_transformer_amd.runtime import KV8Cache
 
 
 def weight(columns, rows=8):
@@ -24,3 +25,14 @@ def test_linear_q8_of_another_number_of_columns():
         ops.linear_q8(weight(520, 3), weight(520), dtype=torch.float32)
     with pytest.raises(BtError, match="GPU memory"):      # codes that do not say
         ops.linear_q8(torch.zeros(3, 515), (torch.zeros(8, 528, dtype=torch.int8), torch.zeros(8)))
+
+
+def test_workspaces_whose_elements_share_memory():
+    """An expanded tensor has more elements than memory: a kernel that took it by its size would write behind it."""
+    thin = torch.zeros(1, dtype=torch.uint8).expand(1 << 20)
+    with pytest.raises(BtError, match="scratch must be contiguous"):
+        ops.linear_q8(weight(64, 3), weight(64), dtype=torch.float32, scratch=thin)
+    kv, q = KV8Cache(1, 3, 4, 64, 32, torch.bfloat16, "cpu")[0], torch.zeros(3, 1, 4, 32, dtype=torch.bfloat16)
+    for ws in (thin, torch.zeros(1 << 20, dtype=torch.uint8)[::2]):
+        with pytest.raises(BtError, match="ws must be contiguous"):
+            ops.attention_kv8(q, kv, 0, n_split=2, ws=ws)
