@@ -357,6 +357,15 @@ def _kv8_rows(t: torch.Tensor, what: str, batch: int, q_len: int, d: int, dtype)
     return _lib.bt_kv8_rows(t.data_ptr(), sb if batch > 1 else 0, st if q_len > 1 else 0, sh if heads > 1 else 0), heads
 
 
+def _apart(t: torch.Tensor, what: str) -> None:
+    """No two elements of rows [batch, q_len, heads, d] that are written may share a place."""
+    extent = t.shape[3]
+    for stride, n in sorted((t.stride(i), t.shape[i]) for i in range(3) if t.shape[i] > 1):
+        if stride < extent:
+            raise _lib.BtError(f"{what} overlaps itself: strides {t.stride()} of {tuple(t.shape)}")
+        extent += stride * (n - 1)
+
+
 def _pos0(pos0):
     if isinstance(pos0, torch.Tensor):
         if pos0.dtype != torch.int32 or pos0.numel() != 1:
@@ -384,6 +393,8 @@ def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.T
     cos = sin = None
     if q is not None:
         qr, heads = _kv8_rows(q, "q", B, q_len, d, dtype)
+    if q_out is not None and q_out.dim() == 4:
+        _apart(q_out, "q_out")
     pos_dev, pos_host = _pos0(pos0)
     index = k.get_device()
     with _on(index, *kv, q, v, rope, pos_table, q_out, pos0 if pos_dev else None):

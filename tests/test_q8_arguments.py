@@ -36,3 +36,17 @@ def test_workspaces_whose_elements_share_memory():
     for ws in (thin, torch.zeros(1 << 20, dtype=torch.uint8)[::2]):
         with pytest.raises(BtError, match="ws must be contiguous"):
             ops.attention_kv8(q, kv, 0, n_split=2, ws=ws)
+
+
+def test_queries_that_are_written_over_each_other():
+    kv, x = KV8Cache(1, 3, 4, 64, 32, torch.bfloat16, "cpu")[0], torch.zeros(3, 5, 4, 32, dtype=torch.bfloat16)
+    rope = ops.rope_tables(64, 16, 10000.0, "cpu")
+    wide = torch.zeros(3 * 5 * 4 * 32 + 64, dtype=torch.bfloat16)
+    for q_out in (x[:1].expand(3, 5, 4, 32), x[:, :, :1].expand(3, 5, 4, 32), wide.as_strided((3, 5, 4, 32), (640, 128, 16, 1)),
+                  wide.as_strided((3, 5, 4, 32), (512, 128, 32, 1))):
+        with pytest.raises(BtError, match="q_out overlaps itself"):
+            ops.kv8_append(kv, x, x, x, 0, rope=rope, q_out=q_out)
+    fused = torch.zeros(3, 5, 12, 32, dtype=torch.bfloat16)
+    for q_out in (x, fused[:, :, 4:8], fused.transpose(1, 2)[:, :4].transpose(1, 2), torch.zeros(5, 3, 4, 32, dtype=torch.bfloat16).transpose(0, 1)):
+        with pytest.raises(BtError, match="GPU memory"):      # (refused for the device alone)
+            ops.kv8_append(kv, x, x, x, 0, rope=rope, q_out=q_out)
