@@ -379,7 +379,7 @@ def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.T
     """Append rows ``k``, ``v`` [B, q_len, kv_heads, d] (any outer strides: views of a fused projection) at row ``pos0`` (an int, or one
     int32 on the device) of one layer of an 8-bit cache (``runtime.KV8Cache``), rotating ``k`` and ``q`` [B, q_len, heads, d] by ``rope``
     (``rope_tables``) at positions pos0 + t or ``pos_table[pos0 + t]``.  Returns the rotated q -- in ``q_out`` (which may be q), new
-    memory otherwise; q itself without ``rope``.  Blocks that fill up are quantised in the same call."""
+    memory otherwise; q itself without ``rope`` or with one of no columns.  Blocks that fill up are quantised in the same call."""
     cache, code, B, H, n_max, d, dtype = _kv8(kv)
     q_len = k.shape[1] if k.dim() == 4 else 0
     kr, k_heads = _kv8_rows(k, "k", B, q_len, d, dtype)
@@ -403,6 +403,7 @@ def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.T
             if len(table) != 3 or table[0] != 2 or rope.dtype != torch.float32 or not rope.is_contiguous():
                 raise _lib.BtError("rope must be contiguous float32 [2, max_pos, rot / 2] (rope_tables)")
             max_pos, rot = table[1], 2 * table[2]
+        if rot:
             cos = rope.data_ptr()
             sin = cos + max_pos * table[2] * 4
             if q is not None:

@@ -36,3 +36,18 @@ def test_quantised_rows_say_how_many_columns_they_have():
         with pytest.raises(BtError, match="515 columns, the weight 520"):
             ops.linear_q8(rows, cw, dtype=F32)
     assert torch.equal(ops.linear_q8(x, ops.quantize_rows(w[:, :515])), ops.linear_q8(cx, ops.quantize_rows(w[:, :515]), dtype=F32))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_append_with_a_rotary_table_of_no_columns(dtype):
+    """rope_tables(n, 0): nothing is rotated, q comes back as it is."""
+    B, H, d, n = 2, 2, 32, 20
+    x = torch.randn(B, n, 3, H, d, generator=torch.Generator().manual_seed(2)).to(dtype).to(DEV)
+    a, b = (KV8Cache(1, B, H, n, d, dtype, DEV)[0] for _ in range(2))
+    for t in a + b:
+        t.zero_()
+    q = x[:, :, 0]
+    none = ops.rope_tables(64, 0, 10000.0, DEV)
+    assert ops.kv8_append(a, q, x[:, :, 1], x[:, :, 2], 0, rope=none) is q
+    assert ops.kv8_append(b, q, x[:, :, 1], x[:, :, 2], 0) is q
+    assert all(torch.equal(s, t) for s, t in zip(a, b))
