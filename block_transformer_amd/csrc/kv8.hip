@@ -1111,7 +1111,8 @@ extern "C" int bt_attention_kv8(int dtype, const bt_kv8_cache* cache, int32_t q_
     BT_CHECK_ARG(out && aligned16(out) && ldo % V == 0 && ldo >= (int64_t)heads * cache->head_dim,
                  "bt_attention_kv8: output rows must be 16-byte granular and hold heads * head_dim");
     BT_CHECK_ARG(pos0_dev || (pos0_host >= 0 && (int64_t)pos0_host + q_len <= cache->n_max), "bt_attention_kv8: cache overflow");
-    BT_CHECK_ARG(!mask || mask_ld >= (pos0_dev ? cache->n_max : (int64_t)pos0_host + q_len), "bt_attention_kv8: mask row too short");
+    BT_CHECK_ARG(!mask || mask_ld == 0 || mask_ld >= (pos0_dev ? cache->n_max : (int64_t)pos0_host + q_len),
+                 "bt_attention_kv8: mask row too short");      // (0: one row for all sequences)
     BT_CHECK_ARG(n_split >= 1, "bt_attention_kv8: bad n_split %d", n_split);
     const int64_t need = bt_attention_kv8_workspace_bytes(cache->batch, q_len, heads, cache->head_dim, n_split);
     if (need > 0 && (!ws || ws_bytes < need || !aligned16(ws))) {

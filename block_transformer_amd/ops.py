@@ -440,7 +440,8 @@ def kv8_read(kv: Sequence[torch.Tensor], n: int, first: int = 0, count: Optional
 def attention_kv8(q: torch.Tensor, kv: Sequence[torch.Tensor], pos0, mask: Optional[torch.Tensor] = None,
                   out: Optional[torch.Tensor] = None, n_split: int = 0, ws: Optional[torch.Tensor] = None):
     """softmax(q k^T / sqrt(d)) v over a layer of an 8-bit cache: row t of ``q`` [B, q_len, heads, d] (rotated, any outer strides; heads a
-    multiple of the cache's) sees the rows j <= pos0 + t with mask[b, j] != 0 (uint8 or bool [B, >= n]); zeros where none is left.  The
+    multiple of the cache's) sees the rows j <= pos0 + t with mask[b, j] != 0 (uint8 or bool [B, >= n], one row expanded too); zeros where none
+    is left.  The
     rows pos0 .. pos0 + q_len - 1 are in the cache already.  ``n_split``: workgroups that share a head's rows (0: chosen from the sizes;
     with a device-side pos0 from the cache's size); ``ws``: >= bt_attention_kv8_workspace_bytes, allocated when needed and not given."""
     cache, code, B, H, n_max, d, dtype = _kv8(kv)

@@ -310,7 +310,7 @@ int bt_kv8_read(int dtype, const bt_kv8_cache* cache, int64_t n, int64_t first, 
  * arithmetic is that of fp32: q, codes and probabilities are multiplied with all their bits, sums are fp32 (scores have to stay within it).
  * n_split > 1 splits the rows over that many workgroups (bt_attention_kv8_split_count gives a good number for a batch; it depends on
  * its arguments alone) and needs a workspace of bt_attention_kv8_workspace_bytes(...).  mask_ld >= pos0_host + q_len, or >= n_max with
- * a device-side pos0. */
+ * a device-side pos0; 0: one mask row, as long, for all sequences. */
 int32_t bt_attention_kv8_split_count(int64_t batch, int32_t kv_heads, int32_t group, int32_t q_len, int64_t n);
 int64_t bt_attention_kv8_workspace_bytes(int64_t batch, int32_t q_len, int32_t heads, int32_t head_dim, int32_t n_split);
 int bt_attention_kv8(int dtype, const bt_kv8_cache* cache, int32_t q_len, int32_t heads, const bt_kv8_rows* q, const int32_t* pos0_dev,

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from block_transformer_amd import ops
+from block_transformer_amd import _lib, ops
 from block_transformer_amd._lib import BtError
 from block_transformer_amd.runtime import KV8Cache
 
@@ -50,3 +50,12 @@ def test_queries_that_are_written_over_each_other():
     for q_out in (x, fused[:, :, 4:8], fused.transpose(1, 2)[:, :4].transpose(1, 2), torch.zeros(5, 3, 4, 32, dtype=torch.bfloat16).transpose(0, 1)):
         with pytest.raises(BtError, match="GPU memory"):      # (refused for the device alone)
             ops.kv8_append(kv, x, x, x, 0, rope=rope, q_out=q_out)
+
+
+def test_one_mask_row_for_all_sequences():
+    """mask_ld = 0 is a row that all share; what lies between is too short.  (The last argument that is checked refuses the call.)"""
+    p = 0x1000      # a pointer that is never followed
+    cache = _lib.bt_kv8_cache(16, 2, 64, 3, 64, p, p, p, p, p, p)
+    for ld, text in ((0, b"n_split"), (10, b"mask row too short"), (11, b"n_split")):
+        rc = _lib.lib().bt_attention_kv8(1, cache, 1, 4, _lib.bt_kv8_rows(p, 1024, 128, 64), None, 10, p, ld, p, 256, 0, None, 0, None)
+        assert rc == -1 and text in _lib.lib().bt_last_error()

@@ -51,3 +51,15 @@ def test_append_with_a_rotary_table_of_no_columns(dtype):
     assert ops.kv8_append(a, q, x[:, :, 1], x[:, :, 2], 0, rope=none) is q
     assert ops.kv8_append(b, q, x[:, :, 1], x[:, :, 2], 0) is q
     assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+def test_attention_with_one_mask_for_all_sequences():
+    """mask.expand(B, n): a batch stride of 0."""
+    B, H, d, n = 3, 2, 64, 100
+    x = torch.randn(B, n, 2, H, d, generator=torch.Generator().manual_seed(1)).to(BF16).to(DEV)
+    kv = KV8Cache(1, B, H, n, d, BF16, DEV)[0]
+    ops.kv8_append(kv, None, x[:, :, 0], x[:, :, 1], 0)
+    mask = (torch.arange(n, device=DEV) % 3 != 0)[None]
+    for m in (mask, mask.to(torch.uint8)):
+        got = ops.attention_kv8(x[:, -1:, 0], kv, n - 1, mask=m.expand(B, n))
+        assert torch.equal(got, ops.attention_kv8(x[:, -1:, 0], kv, n - 1, mask=m.repeat(B, 1)))
