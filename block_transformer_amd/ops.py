@@ -179,7 +179,9 @@ def rope_tables(max_pos: int, rot: int, base: float, device) -> torch.Tensor:
 # ---- 8-bit serving ----------------------------------------------------------------------------------------------------------------
 _HERE = contextlib.nullcontext()
 # the current stream's handle and the current device without the Python objects around them: together 5 us of a call that takes 10
-_raw_stream, _device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
+# (a torch built without GPU support has neither name: nothing can be launched there, but importing this module is no launch)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 # bt_kv8_cache as bytes: a third of the time that its fields take one by one
 _cache_bytes = struct.Struct("=I3i2q6Q").pack
 _CACHE_SIZE = ctypes.sizeof(_lib.bt_kv8_cache)

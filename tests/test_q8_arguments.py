@@ -1,4 +1,6 @@
 """Calls of the 8-bit operators that are refused, and that nothing else depends on: without a GPU."""
+import importlib.util
+
 import pytest
 import torch
 
@@ -59,3 +61,14 @@ def test_one_mask_row_for_all_sequences():
     for ld, text in ((0, b"n_split"), (10, b"mask row too short"), (11, b"n_split")):
         rc = _lib.lib().bt_attention_kv8(1, cache, 1, 4, _lib.bt_kv8_rows(p, 1024, 128, 64), None, 10, p, ld, p, 256, 0, None, 0, None)
         assert rc == -1 and text in _lib.lib().bt_last_error()
+
+
+def test_the_module_is_imported_on_a_torch_without_gpu_support(monkeypatch):
+    """Such a build has no torch._C._cuda_*; calls are refused as on any machine without a GPU."""
+    for name in ("_cuda_getCurrentRawStream", "_cuda_getDevice"):
+        monkeypatch.delattr(torch._C, name, raising=False)
+    spec = importlib.util.spec_from_file_location("block_transformer_amd.ops_again", ops.__file__)
+    again = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(again)
+    with pytest.raises(BtError, match="GPU memory"):
+        again.quantize_rows(torch.zeros(3, 40))
