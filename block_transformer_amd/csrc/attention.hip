@@ -993,6 +993,8 @@ __global__ __launch_bounds__(NW * 64, NW * QF_ == 8 ? (QF_ == 1 ? 4 : 2) : 1) vo
 // K/V tile staging for the persistent kernel: wave-uniform 64-bit base in SGPRs + one 32-bit byte offset per lane (the v2
 // helper's per-lane 64-bit addresses cost the persistent kernel its last registers: 29 spills, reloaded inside the tile loop).
 // Every LDS-DMA of that kernel goes through this helper, so the compiler never has its own idea of M0 there.
+// The waits cover an M0 write right before the load (1) and a base that a v_readlane has just brought back from a spill (5, the s_mov among
+// them): neither is padded inside an asm string, and head_dim 64 does have such a reload right in front.
 template <int D, int NW = 4>
 __device__ inline void flash_stage_tile_s(const bf16* __restrict__ kbase, const bf16* __restrict__ vbase, int key0, int n_keys,
                                           char* kbuf, char* vbuf, int wave, int lane) {
@@ -1012,8 +1014,8 @@ __device__ inline void flash_stage_tile_s(const bf16* __restrict__ kbase, const 
         const uint32_t vo = (uint32_t)(kr * ROWB + ((p ^ (((row & 7) << 1) & (SLOTS - 1))) << 4));
         const uint32_t kl = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(kbuf + rbase * ROWB);
         const uint32_t vl = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)(vbuf + rbase * ROWB);
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(ko), "s"(kbase), "s"(kl) : "memory");
-        asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(vo), "s"(vbase), "s"(vl) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(ko), "s"(kbase), "s"(kl) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %0, %1" : : "v"(vo), "s"(vbase), "s"(vl) : "memory");
     }
 }
 
