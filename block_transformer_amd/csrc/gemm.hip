@@ -1481,8 +1481,9 @@ __device__ inline uint32_t lds_addr(const char* p) {
 }
 
 // 16-byte-per-lane LDS-DMA, global address = SGPR base + 32-bit VGPR offset, LDS address = lds_base (M0) + lane * 16
+// (an LDS-DMA needs one wait state behind the write of M0 that it reads; nothing pads that inside an asm string)
 __device__ inline void glds16_sbase(const char* base_uniform, uint32_t voff, uint32_t lds_base_uniform) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1"
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1"
                  :
                  : "v"(voff), "s"(base_uniform), "s"(lds_base_uniform)
                  : "memory");
@@ -1491,7 +1492,7 @@ __device__ inline void glds16_sbase(const char* base_uniform, uint32_t voff, uin
 // same with a per-lane 64-bit global address (edge tiles, bias row).  The persistent kernel issues every LDS-DMA through
 // these two helpers so the compiler never emits its own M0 writes in that kernel (it does not know the asm changes M0).
 __device__ inline void glds16_vaddr(const void* gptr, uint32_t lds_base_uniform) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(gptr), "s"(lds_base_uniform) : "memory");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" : : "v"(gptr), "s"(lds_base_uniform) : "memory");
 }
 
 // one half-tile (kind in consumption order A0, W0, W1, A1) of the K-tile at k0 into ring buffer `parity`.

@@ -1,7 +1,7 @@
 """The SGPR hazard scan over what the build compiles: its own flags, and every source that issues LDS-DMA from inline asm.
 
 A vector memory instruction that takes an SGPR pair as its base needs five wait states behind a vector instruction that wrote the pair
-(v_readlane, v_readfirstlane); hipcc does not pad that inside an asm string."""
+(v_readlane, v_readfirstlane), and an LDS-DMA one behind the write of M0 that it reads; hipcc does not pad that inside an asm string."""
 import os
 import re
 import subprocess
@@ -43,3 +43,11 @@ def test_no_valu_written_sgpr_base_within_five_wait_states(kernels):
 def test_no_packed_fp32_arithmetic(kernels):
     for name, body in kernels[1].items():
         assert not re.search(r"\bv_pk_(add|mul|fma)_f32\b", body), name
+
+
+def test_no_dma_right_behind_its_m0(kernels):
+    for name, body in kernels[1].items():
+        ins = [l.strip() for l in body.split("\n")]
+        ins = [l for l in ins if l and not l.startswith((";", ".")) and not l.endswith(":")]
+        for before, dma in zip(ins, ins[1:]):
+            assert not (" lds" in dma or "load_lds" in dma) or not re.match(r"s_\w+ m0,", before), (name, before, dma)
