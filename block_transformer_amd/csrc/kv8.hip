@@ -1039,7 +1039,9 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     // 8 x 100 9.8 and 14.9; a step of 256 sequences that fills no block 9.8 and 7.5.
     a.split = pos0_dev ? q_len > 1 : ((int64_t)pos0_host + q_len) / cache->block > pos0_host / cache->block;
     const int64_t kv_items = (cache->batch * cache->kv_heads * a.blocks) << a.split, q_rows = q ? cache->batch * q_len * heads : 0;
-    BT_CHECK_ARG(kv_items < (1ll << 30) && q_rows < (1ll << 30), "bt_kv8_append: too many rows for one call");
+    const int V = dtype == BT_BF16 ? 8 : 4;
+    BT_CHECK_ARG(kv_items < (1ll << 25) && q_rows < (1ll << 30) && ceil_div(q_rows * cache->head_dim, 256 * V * QU) < (1ll << 25),
+                 "bt_kv8_append: too many rows for one call");      // (2^32 threads)
     a.kv_items = (uint32_t)kv_items;
     a.q_rows = (uint32_t)q_rows;
     a.q_len = q_len;
@@ -1051,7 +1053,6 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.cos_tab = cos_tab;
     a.sin_tab = sin_tab;
     a.max_pos = max_pos;
-    const int V = dtype == BT_BF16 ? 8 : 4;
     a.vec_rope = (rot / 2) % V == 0 && aligned16(cos_tab) && aligned16(sin_tab);
     const int64_t waves = kv_items + ceil_div(q_rows * cache->head_dim, 256 * V * QU);
     const dim3 grid((unsigned)ceil_div(waves, 4));
@@ -1073,7 +1074,7 @@ extern "C" int bt_kv8_read(int dtype, const bt_kv8_cache* cache, int64_t n, int6
     if (cache->batch == 0 || count == 0 || (!k_out && !v_out)) return BT_OK;
     const int blocks = (int)((first + count - 1) / cache->block - first / cache->block) + 1;
     const int64_t waves = cache->batch * cache->kv_heads * blocks;
-    BT_CHECK_ARG(waves < (1ll << 31), "bt_kv8_read: grid too large");
+    BT_CHECK_ARG(waves < (1ll << 26), "bt_kv8_read: grid too large");      // (2^32 threads)
     const dim3 grid((unsigned)ceil_div(waves, 4));
     hipStream_t s = (hipStream_t)stream;
     ProfScope ps(BT_PROF_ROPE, s);
@@ -1130,7 +1131,8 @@ extern "C" int bt_attention_kv8(int dtype, const bt_kv8_cache* cache, int32_t q_
     a.n_split = n_split;
     a.part = n_split > 1 ? (float*)ws : nullptr;
     const int64_t groups = cache->batch * cache->kv_heads * a.row_groups;
-    BT_CHECK_ARG(groups * n_split < (1ll << 31) && cache->batch * cache->kv_heads * a.rows < (1ll << 31), "bt_attention_kv8: grid too large");
+    BT_CHECK_ARG(groups * n_split < (1ll << 26) && (n_split == 1 || cache->batch * cache->kv_heads * a.rows < (1ll << 24)),
+                 "bt_attention_kv8: grid too large");      // (2^32 threads)
     a.pos0_host = pos0_host;
     a.pos0_dev = pos0_dev;
     a.mask = mask;

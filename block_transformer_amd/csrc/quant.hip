@@ -196,7 +196,9 @@ static int launch_quant_rows(int64_t M, int64_t K, const void* x, int64_t ldx, c
     // one wave to a row from 2048 rows (8 waves to a CU) while it has at most 8 pieces a lane
     const bool one = wave_pieces <= 8 && M >= 2048;
     const int64_t pieces = one ? wave_pieces : group_pieces;
-    const dim3 grid((unsigned)(one ? ceil_div(M, 4) : M));
+    const int64_t groups = one ? ceil_div(M, 4) : M;
+    BT_CHECK_ARG(groups < (1ll << 24), "bt_quant_rows: %lld rows are too many for one launch", (long long)M);      // (2^32 threads)
+    const dim3 grid((unsigned)groups);
 #define BT_QR(LN_, NV_, R_)                                                                                                          \
     hipLaunchKernelGGL((quant_rows_kernel<T, LN_, NV_, R_>), grid, dim3(256), 0, s, (const T*)x, ldx, (const T*)w, (const T*)b, eps, \
                        codes, ldc, scales, M, (int)K)
@@ -890,6 +892,7 @@ static int launch_linear_q8(Q8Args& e, int64_t scratch_bytes, hipStream_t s) {
     Q8Plan p = q8_plan(e.M, e.N, e.K);
     if (p.slices > 1 && scratch_bytes < (int64_t)p.slices * e.M * e.N * (int64_t)sizeof(int)) p.slices = 1;
     if (e.lda >= (1 << 23) || e.ldw >= (1 << 23)) p.kind = Q8Plan::ROWS;      // a tile's rows would not be within 32 bits
+    BT_CHECK_ARG(p.kind != Q8Plan::ROWS || e.M < (1 << 21), "bt_linear_q8: M=%d is too many rows for codes so far apart", e.M);      // (grid.y)
     switch (p.kind) {
         case Q8Plan::ROWS:
             if (e.M <= 16) launch_rows<T, 1, 1>(e, s);

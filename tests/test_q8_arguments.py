@@ -72,3 +72,22 @@ def test_the_module_is_imported_on_a_torch_without_gpu_support(monkeypatch):
     spec.loader.exec_module(again)
     with pytest.raises(BtError, match="GPU memory"):
         again.quantize_rows(torch.zeros(3, 40))
+
+
+def test_launches_of_more_threads_than_32_bits_count():
+    """Such a grid would be cut or fail; the entry points say so.  (No pointer is followed.)"""
+    p, lib = 0x1000, _lib.lib()
+
+    def refused(rc, text):
+        assert rc == -1 and text in lib.bt_last_error(), (rc, lib.bt_last_error())
+
+    refused(lib.bt_quant_rows(1, 1 << 26, 16, p, 16, None, None, 1e-5, p, 16, p, None), b"too many")
+    refused(lib.bt_quant_rows(1, 1 << 24, 8192, p, 8192, None, None, 1e-5, p, 8192, p, None), b"too many")
+    refused(lib.bt_linear_q8(1, 1 << 21, 2, 16, p, 16, p, p, 1 << 23, p, None, None, 0, p, 2, 0, None, 0, None), b"too many")
+    rows = _lib.bt_kv8_rows(p, 32, 32, 32)
+    cache = lambda batch, n_max: _lib.bt_kv8_cache(16, 1, 32, batch, n_max, p, p, p, p, p, p)  # noqa: E731
+    refused(lib.bt_kv8_append(1, cache(1 << 25, 16), 1, 1, None, None, rows, rows, None, 0, None, 0, None, None, 0, None), b"too many")
+    refused(lib.bt_kv8_append(1, cache(1 << 22, 256), 200, 64, rows, rows, rows, rows, None, 0, None, 2, p, p, 256, None), b"too many")
+    refused(lib.bt_kv8_read(1, cache(1 << 20, 1024), 1024, 0, 1024, p, p, None), b"too large")
+    refused(lib.bt_attention_kv8(1, cache(1 << 26, 16), 1, 1, rows, None, 0, None, 0, p, 32, 1, None, 0, None), b"too large")
+    refused(lib.bt_attention_kv8(1, cache(1 << 24, 16), 1, 1, rows, None, 0, None, 0, p, 32, 2, p, 1 << 60, None), b"too large")
