@@ -119,8 +119,6 @@ struct BlockMax {
 // K and V are held in registers between the search for the scale and the codes; five waves to a SIMD where that fits.  Bound by memory
 // and the chain load -> scale -> codes: 32 sequences x 509 rows x 16 heads of 128 (333 MB) 88 us (3.8 TB/s), the same in blocks of 32
 // 166 us (four waves to a SIMD); a step that fills 4096 blocks of 16 rows 15.5 us, one that fills none 7.5 us.
-constexpr int QU = 1;
-
 template <typename T, int D, int BL>
 __global__ __launch_bounds__(256, D * BL <= 2048 ? 5 : D * BL <= 4096 ? 4 : 2) void kv8_append_kernel(AppendArgs a) {
     constexpr int V = Elem<T>::VEC, RP = D / V, LR = RP / 4;      // pieces of a row, lanes to a row
@@ -130,38 +128,27 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 5 : D * BL <= 4096 ? 4 : 2) v
     const uint32_t item = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int e_lane = lane % LR * V;      // piece k of this lane: dims e_lane + k D / 4
     if (item >= a.kv_items) {
-        // QU rows (b, t, h) of q a lane.  The last workgroup has waves too many, without q all of these are.
-        const uint32_t i0 = (item - a.kv_items) * (QU * 64 / LR);
+        // A row (b, t, h) of q to LR lanes.  The last workgroup has waves too many, without q all of these are.
+        const uint32_t i0 = (item - a.kv_items) * (64 / LR);
         if (i0 >= a.q_rows) return;
-        const T* src[QU];
-        T* dst[QU];
-        int64_t pos[QU];
-        bool there[QU];
-        float v[QU][4][V];
+        uint32_t i = i0 + lane / LR;
+        const bool there = i < a.q_rows;
+        i = there ? i : a.q_rows - 1;
+        const uint32_t bt = i / (uint32_t)a.heads, b = bt / (uint32_t)a.q_len;
+        const int h = (int)(i - bt * a.heads), t = (int)(bt - b * a.q_len);
+        const T* src = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
+        T* dst = (T*)a.q_out.p + b * a.q_out.b + t * a.q_out.t + h * a.q_out.h;
+        const int64_t pos = (int64_t)pos0 + t;
+        float v[4][V];
 #pragma unroll
-        for (int u = 0; u < QU; ++u) {
-            uint32_t i = i0 + u * (64 / LR) + lane / LR;
-            there[u] = i < a.q_rows;
-            i = there[u] ? i : a.q_rows - 1;
-            const uint32_t bt = i / (uint32_t)a.heads, b = bt / (uint32_t)a.q_len;
-            const int h = (int)(i - bt * a.heads), t = (int)(bt - b * a.q_len);
-            src[u] = (const T*)a.q.p + b * a.q.b + t * a.q.t + h * a.q.h;
-            dst[u] = (T*)a.q_out.p + b * a.q_out.b + t * a.q_out.t + h * a.q_out.h;
-            pos[u] = (int64_t)pos0 + t;
+        for (int k = 0; k < 4; ++k) load_vec<T>(src + e_lane + k * (D / 4), v[k]);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) load_vec<T>(src[u] + e_lane + k * (D / 4), v[u][k]);
-        }
-#pragma unroll
-        for (int u = 0; u < QU; ++u)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (e_lane + k * (D / 4) < a.rot) rotated_piece<T>(a, src[u], e_lane + k * (D / 4), angle_of(a, pos[u]), v[u][k]);
+        for (int k = 0; k < 4; ++k)
+            if (e_lane + k * (D / 4) < a.rot) rotated_piece<T>(a, src, e_lane + k * (D / 4), angle_of(a, pos), v[k]);
         asm volatile("" ::: "memory");      // q_out may be q: every lane of the row has read before one writes
 #pragma unroll
-        for (int u = 0; u < QU; ++u)
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                if (there[u]) store_vec<T>(dst[u] + e_lane + k * (D / 4), v[u][k]);
+        for (int k = 0; k < 4; ++k)
+            if (there) store_vec<T>(dst + e_lane + k * (D / 4), v[k]);
         return;
     }
     // neighbouring waves take neighbouring heads: of a fused projection's rows they read one piece of memory
@@ -1040,7 +1027,7 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.split = pos0_dev ? q_len > 1 : ((int64_t)pos0_host + q_len) / cache->block > pos0_host / cache->block;
     const int64_t kv_items = (cache->batch * cache->kv_heads * a.blocks) << a.split, q_rows = q ? cache->batch * q_len * heads : 0;
     const int V = dtype == BT_BF16 ? 8 : 4;
-    BT_CHECK_ARG(kv_items < (1ll << 25) && q_rows < (1ll << 30) && ceil_div(q_rows * cache->head_dim, 256 * V * QU) < (1ll << 25),
+    BT_CHECK_ARG(kv_items < (1ll << 25) && q_rows < (1ll << 30) && ceil_div(q_rows * cache->head_dim, 256 * V) < (1ll << 25),
                  "bt_kv8_append: too many rows for one call");      // (2^32 threads)
     a.kv_items = (uint32_t)kv_items;
     a.q_rows = (uint32_t)q_rows;
@@ -1054,7 +1041,7 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.sin_tab = sin_tab;
     a.max_pos = max_pos;
     a.vec_rope = (rot / 2) % V == 0 && aligned16(cos_tab) && aligned16(sin_tab);
-    const int64_t waves = kv_items + ceil_div(q_rows * cache->head_dim, 256 * V * QU);
+    const int64_t waves = kv_items + ceil_div(q_rows * cache->head_dim, 256 * V);
     const dim3 grid((unsigned)ceil_div(waves, 4));
     hipStream_t s = (hipStream_t)stream;
     ProfScope ps(BT_PROF_ROPE, s);

@@ -721,39 +721,34 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
     }
 }
 
-// Few rows: 16 MB rows by 16 NB columns per workgroup, the waves dividing K among themselves.  W is read once, straight into the operand
+// Few rows: 16 MB rows by 16 columns per workgroup, its eight waves dividing K among themselves.  W is read once, straight into the operand
 // registers of the matrix instruction (a lane holds 16 bytes of a row: nothing to rearrange, no LDS, no barrier in the loop), with
-// every load of four 128-byte units out at once: a problem of this size is a few microseconds of latency, not of bandwidth.  A comes the
-// same way, from the caches.  The partial sums meet in LDS; being integers, they do not depend on the number of waves.  One row: 6144 x 2048
-// 5.0 us (2.5 TB/s of weights), 8192 x 2048 5.2 us (3.2 TB/s), 2048 x 8192 7.7 us (128 workgroups: half the CUs).
-template <typename T, int MB, int NB, int NW>
-__global__ __launch_bounds__(NW * 64) void linear_q8_rows_kernel(Q8Args e) {
-    __shared__ i32x4 part[NW][MB * NB][64];
+// every load of four (MB = 2: two) 128-byte units out at once: a problem of this size is a few microseconds of latency, not of bandwidth.
+// A comes the same way, from the caches.  The partial sums meet in LDS; being integers, they do not depend on the number of waves.  One
+// row: 6144 x 2048 5.0 us (2.5 TB/s of weights), 8192 x 2048 5.2 us (3.2 TB/s), 2048 x 8192 7.7 us (128 workgroups: half the CUs).
+template <typename T, int MB>
+__global__ __launch_bounds__(512) void linear_q8_rows_kernel(Q8Args e) {
+    constexpr int NW = 8, U = MB == 1 ? 4 : 2;      // waves, units of a round
+    __shared__ i32x4 part[NW][MB][64];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
-    const int n0 = blockIdx.x * 16 * NB, m0 = blockIdx.y * 16 * MB;
+    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16 * MB;
     const int8_t* ap[MB];
-    const int8_t* wp[NB];
+    const int8_t* wp = e.W + (int64_t)min(n0 + c, e.N - 1) * e.ldw + 16 * g;
 #pragma unroll
     for (int i = 0; i < MB; ++i) ap[i] = e.A + (int64_t)min(m0 + 16 * i + c, e.M - 1) * e.lda + 16 * g;
+    i32x4 acc[MB];
 #pragma unroll
-    for (int j = 0; j < NB; ++j) wp[j] = e.W + (int64_t)min(n0 + 16 * j + c, e.N - 1) * e.ldw + 16 * g;
-    i32x4 acc[MB][NB];
-#pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) acc[i][j] = i32x4{0, 0, 0, 0};
-    constexpr int U = MB * NB >= 8 ? 1 : MB * NB >= 2 ? 2 : 4;      // units of a round
+    for (int i = 0; i < MB; ++i) acc[i] = i32x4{0, 0, 0, 0};
     const i32x4 zero{0, 0, 0, 0};
     for (int k = wave * 128; k < e.K; k += NW * 128 * U) {
-        i32x4 a[U][2][MB], w[U][2][NB];
+        i32x4 a[U][2][MB], w[U][2];
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int at = k + u * NW * 128 + h * 64;
                 const bool in = at + 16 * g < e.K;      // K is a whole number of 16-byte pieces
-#pragma unroll
-                for (int j = 0; j < NB; ++j) w[u][h][j] = in ? *(const i32x4*)(wp[j] + at) : zero;
+                w[u][h] = in ? *(const i32x4*)(wp + at) : zero;
 #pragma unroll
                 for (int i = 0; i < MB; ++i) a[u][h][i] = in ? *(const i32x4*)(ap[i] + at) : zero;
             }
@@ -762,23 +757,18 @@ __global__ __launch_bounds__(NW * 64) void linear_q8_rows_kernel(Q8Args e) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                for (int i = 0; i < MB; ++i)
-#pragma unroll
-                    for (int j = 0; j < NB; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][h][j], a[u][h][i], acc[i][j], 0, 0, 0);
+                for (int i = 0; i < MB; ++i) acc[i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[u][h], a[u][h][i], acc[i], 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < MB; ++i)
-#pragma unroll
-        for (int j = 0; j < NB; ++j) part[wave][i * NB + j][lane] = acc[i][j];
+    for (int i = 0; i < MB; ++i) part[wave][i][lane] = acc[i];
     __syncthreads();
     // lane (c, g) of fragment f: row c, columns 4 g .. 4 g + 3
-    for (int x = threadIdx.x; x < MB * NB * 64; x += NW * 64) {
+    for (int x = threadIdx.x; x < MB * 64; x += NW * 64) {
         const int f = x >> 6, l = x & 63;
         i32x4 sum = part[0][f][l];
 #pragma unroll
         for (int w = 1; w < NW; ++w) sum += part[w][f][l];
-        const int m = m0 + f / NB * 16 + (l & 15), n = n0 + f % NB * 16 + (l >> 4) * 4;
+        const int m = m0 + f * 16 + (l & 15), n = n0 + (l >> 4) * 4;
         if (m >= e.M || n >= e.N) continue;
         float sw[4], bias[4], y[4];
 #pragma unroll
@@ -880,10 +870,9 @@ static void launch_tile(Q8Args& e, int slices, hipStream_t s) {
         hipLaunchKernelGGL((linear_q8_join_kernel<T>), dim3((unsigned)ceil_div((int64_t)e.M * ((e.N + 3) / 4), 256)), dim3(256), 0, s, e);
 }
 
-template <typename T, int MB, int NB>
+template <typename T, int MB>
 static void launch_rows(const Q8Args& e, hipStream_t s) {
-    hipLaunchKernelGGL((linear_q8_rows_kernel<T, MB, NB, 8>), dim3((unsigned)ceil_div(e.N, 16 * NB), (unsigned)ceil_div(e.M, 16 * MB)), dim3(512),
-                       0, s, e);
+    hipLaunchKernelGGL((linear_q8_rows_kernel<T, MB>), dim3((unsigned)ceil_div(e.N, 16), (unsigned)ceil_div(e.M, 16 * MB)), dim3(512), 0, s, e);
 }
 
 template <typename T>
@@ -895,8 +884,8 @@ static int launch_linear_q8(Q8Args& e, int64_t scratch_bytes, hipStream_t s) {
     BT_CHECK_ARG(p.kind != Q8Plan::ROWS || e.M < (1 << 21), "bt_linear_q8: M=%d is too many rows for codes so far apart", e.M);      // (grid.y)
     switch (p.kind) {
         case Q8Plan::ROWS:
-            if (e.M <= 16) launch_rows<T, 1, 1>(e, s);
-            else launch_rows<T, 2, 1>(e, s);
+            if (e.M <= 16) launch_rows<T, 1>(e, s);
+            else launch_rows<T, 2>(e, s);
             break;
         case Q8Plan::TILE64: launch_tile<T, 2, 2, 8>(e, p.slices, s); break;
         case Q8Plan::TILE128: launch_tile<T, 4, 4, 4>(e, p.slices, s); break;
