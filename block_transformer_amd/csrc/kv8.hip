@@ -43,8 +43,9 @@ __device__ inline int64_t angle_of(const AppendArgs& a, int64_t pos) {
     return r < a.max_pos ? r : a.max_pos - 1;
 }
 
-// Dims e0 .. e0 + V - 1 of a row, rotated.  The two products of 24-bit numbers are exact in fp64, so the result is the exact one rounded
-// once: codes (and so what is compared bit for bit) do not depend on how a sum was fused.  Costs nothing here: memory is the bound.
+// Dims e0 .. e0 + V - 1 of a row, rotated.  The two products of 24-bit numbers are exact in fp64, so the result is their sum rounded to
+// fp64 and from there to fp32 (and, where the row is written in bf16, from fp32 to bf16, as torch converts): codes, and so what is compared
+// bit for bit, do not depend on how a sum was fused.  Costs nothing here: memory is the bound.
 template <typename T>
 __device__ inline void rotated_piece(const AppendArgs& a, const T* row, int e0, int64_t angle, float (&v)[Elem<T>::VEC]) {
     constexpr int V = Elem<T>::VEC;
@@ -116,9 +117,11 @@ struct BlockMax {
 //         the fp64 work of the others is skipped.
 //   V: a lane has columns 2 x, 2 x + 1 of 16 rows, that is two 16-byte runs of v_codes: rows are read 256 bytes a wave and instruction,
 //      and no transpose is needed.  Rows of the open block come in runs from v_tail, which is transposed already.
-// K and V are held in registers between the search for the scale and the codes; five waves to a SIMD where that fits.  Bound by memory
-// and the chain load -> scale -> codes: 32 sequences x 509 rows x 16 heads of 128 (333 MB) 88 us (3.8 TB/s), the same in blocks of 32
-// 166 us (four waves to a SIMD); a step that fills 4096 blocks of 16 rows 15.5 us, one that fills none 7.5 us.
+// K and V are held in registers between the search for the scale and the codes.  Bound by memory and the chain load -> scale -> codes:
+// 32 sequences x 509 rows x 16 heads of 128 (333 MB) in blocks of 16 88 .. 93 us by card (3.6 .. 3.8 TB/s; 79 registers, six waves to a
+// SIMD), in blocks of 32 166 .. 173 us (85, five), of 64 242 .. 256 us (162, three); fp32 (600 MB) in blocks of 16 149 us (4.0 TB/s).  The
+// straight-line code for a block is 54, 90 and 156 KB, so from 32 rows on more than an instruction cache holds.  A step that fills 4096
+// blocks of 16 rows 16 us, one that fills none 8 us.
 template <typename T, int D, int BL>
 __global__ __launch_bounds__(256, D * BL <= 2048 ? 5 : D * BL <= 4096 ? 4 : 2) void kv8_append_kernel(AppendArgs a) {
     constexpr int V = Elem<T>::VEC, RP = D / V, LR = RP / 4;      // pieces of a row, lanes to a row
@@ -342,7 +345,8 @@ __global__ __launch_bounds__(256, D * BL <= 2048 ? 5 : D * BL <= 4096 ? 4 : 2) v
 
 // ---- bt_kv8_read -----------------------------------------------------------------------------------------------------------
 // One wave per (sequence, head, block): K by pieces of 16 codes, V by pairs of columns and runs of 16 rows, as append has them.  Bound by
-// memory: 32 x 509 rows x 16 heads of 128 (200 MB) 31 us (6.4 TB/s, part of it from the caches).
+// memory: 32 x 509 rows x 16 heads of 128 (200 MB) 31 .. 37 us by card (5.4 .. 6.4 TB/s, part of it from the caches); in blocks of 32 44 us,
+// of 64 52 us.
 template <typename T, int D, int BL>
 __global__ __launch_bounds__(256) void kv8_read_kernel(bt_kv8_cache c, int64_t n, int64_t first, int64_t count, int blocks,
                                                       T* __restrict__ ko, T* __restrict__ vo) {
@@ -1022,8 +1026,9 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.v = rows_of(v);
     a.blocks = pos0_dev ? (q_len + cache->block - 2) / cache->block + 1
                         : (int)(((int64_t)pos0_host + q_len - 1) / cache->block - pos0_host / cache->block) + 1;
-    // Blocks that fill up have a wave for K and one for V, steps that fill none (or may: the device knows) one for both: 32 x 509 rows 88 us and 97,
-    // 8 x 100 9.8 and 14.9; a step of 256 sequences that fills no block 9.8 and 7.5.
+    // Blocks that fill up have a wave for K and one for V, steps that fill none (or may: the device knows) one for both: 32 x 509 rows 88 us
+    // and 97, 8 x 100 9.8 and 14.9; a step of 256 sequences that fills no block 9.8 and 7.5, and of a step whose position the device
+    // reads, one row at a time, at most one in 16 fills its blocks.
     a.split = pos0_dev ? q_len > 1 : ((int64_t)pos0_host + q_len) / cache->block > pos0_host / cache->block;
     const int64_t kv_items = (cache->batch * cache->kv_heads * a.blocks) << a.split, q_rows = q ? cache->batch * q_len * heads : 0;
     const int V = dtype == BT_BF16 ? 8 : 4;

@@ -33,8 +33,8 @@ __device__ inline void load_any(const T* p, float (&v)[Elem<T>::VEC]) {
 // A row is read once into registers -- NV 16-byte pieces a lane, all loads in flight together -- and everything else happens there:
 // LayerNorm statistics (two-pass, fp32), the largest magnitude, the codes.  R waves to a row: one where there are rows enough for
 // the card (no barrier), four where there are not or where the row does not fit one wave's registers.  Bound by memory: x in, one
-// byte a value out -- 8192 x 8192 bf16 35 us (5.7 TB/s), 4096 x 8192 21 us (4.8); with LayerNorm, 8192 x 2048 17 us (3.0 TB/s: the weights'
-// registers leave four waves to a SIMD), one row of 2048 3.1 us.
+// byte a value out -- 8192 x 8192 bf16 35 us (5.7 TB/s), 4096 x 8192 22 us (4.6); with LayerNorm, 8192 x 2048 16.5 us (3.0 TB/s, six waves to
+// a SIMD), 4000 x 1001 fp32 7.9 us; one row of 2048 3.0 us.
 template <int R>
 struct RowReduce {      // over the R waves of a row (R = 4: the workgroup)
     float* slot;
@@ -149,7 +149,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
     }
 }
 
-// Rows longer than four waves' registers: a workgroup passes over the row once for each of the steps above.
+// Rows longer than four waves' registers: a workgroup passes over the row once for each of the steps above (two, four with LayerNorm), an
+// element a thread.  1000 x 20000 bf16 60 us (1.0 TB/s).
 template <typename T, bool LN>
 __global__ __launch_bounds__(256) void quant_long_rows_kernel(const T* __restrict__ x, int64_t ldx, const T* __restrict__ w,
                                                              const T* __restrict__ b, float eps, int8_t* __restrict__ codes, int64_t ldc,
@@ -412,7 +413,7 @@ __device__ inline void q8_write(const Q8Args& e, const i32x4 (&acc)[NI][NB], cha
 //  * LDS rows are 64 bytes; the four 16-byte pieces of row r are stored in the order p ^ ((r >> 1) & 3) ^ ((r >> 3) & 1): the 16 rows that
 //    a fragment read touches at once are spread over all banks.
 //  * mfma(W, A): a lane gets four neighbouring columns of one row (q8_write).
-// 256 x 6144 x 2048 10.1 us by 64 x 64 tiles, 2048 x 2048 x 8192 44 us (1.6 POPS) by 128 x 128: bound by
+// 256 x 6144 x 2048 10 .. 12 us by 64 x 64 tiles, 2048 x 2048 x 8192 45 us (1.5 POPS) by 128 x 128: bound by
 // the way from L2 into a CU, as the largest kernel is, with more bytes to an operation.
 template <typename T, int MI, int NB, int NS>
 __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
@@ -559,9 +560,12 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
 //  * A tile ends with one more barrier for group 0 (group 1 has then read its last) and begins with one more for group 1, so the two
 //    epilogues run side by side.
 //  * A row of 128 bytes has its 16-byte pieces in the order p ^ (row & 7).
-// 8192 x 8192 x 2048 131 us (2.1 POPS), with GELU 141 us, 8192 x 8192 x 8192 398 us (2.8 POPS, matrix units busy two thirds of the time at the
-// 1.8 GHz that the card then holds).  Of the 131 us, 107 are the products, 10 the stores and 14 the rest of the epilogue.  4096 x 2048 x 8192
-// by 256 x 128 65 us (2.1 POPS; by 128 x 128 77, by 256 x 256 on half the CUs 80).
+// One launch after another in a graph, on a card that is cool: 8192 x 8192 x 2048 131 us (2.1 POPS), with GELU 141 us, 8192 x 8192 x 8192
+// 398 us (2.8 POPS, matrix units busy two thirds of the time at the 1.8 GHz that the card then holds); of the 131 us, 107 are the products,
+// 10 the stores and 14 the rest of the epilogue.  4096 x 2048 x 8192 by 256 x 128 65 us (2.1 POPS; by 128 x 128 77, by 256 x 256 on half
+// the CUs 80).  Single launches under the profiler, on several cards: 156, 425 and 77 .. 85 us.  fp32 results: 186 us with GELU, 4096 x 2048 x
+// 8192 77 us; the 256 x 256 form has six registers too few there and brings its load offsets back from scratch at a tile's start, which
+// waits for every load that is out.
 template <typename T, int NB>
 __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
     constexpr int HALVES = NB == 4 ? 4 : 3, RING = NB == 4 ? 2 : 3, COLS = 64 * NB;      // A0, W0, (W1,) A1
@@ -725,7 +729,7 @@ __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
 // registers of the matrix instruction (a lane holds 16 bytes of a row: nothing to rearrange, no LDS, no barrier in the loop), with
 // every load of four (MB = 2: two) 128-byte units out at once: a problem of this size is a few microseconds of latency, not of bandwidth.
 // A comes the same way, from the caches.  The partial sums meet in LDS; being integers, they do not depend on the number of waves.  One
-// row: 6144 x 2048 5.0 us (2.5 TB/s of weights), 8192 x 2048 5.2 us (3.2 TB/s), 2048 x 8192 7.7 us (128 workgroups: half the CUs).
+// row: 6144 x 2048 5.4 us (2.3 TB/s of weights), 8192 x 2048 5.6 us (3.0 TB/s), 2048 x 8192 7.4 us (128 workgroups: half the CUs).
 template <typename T, int MB>
 __global__ __launch_bounds__(512) void linear_q8_rows_kernel(Q8Args e) {
     constexpr int NW = 8, U = MB == 1 ? 4 : 2;      // waves, units of a round

@@ -381,7 +381,8 @@ def kv8_append(kv: Sequence[torch.Tensor], q: Optional[torch.Tensor], k: torch.T
     """Append rows ``k``, ``v`` [B, q_len, kv_heads, d] (any outer strides: views of a fused projection) at row ``pos0`` (an int, or one
     int32 on the device) of one layer of an 8-bit cache (``runtime.KV8Cache``), rotating ``k`` and ``q`` [B, q_len, heads, d] by ``rope``
     (``rope_tables``) at positions pos0 + t or ``pos_table[pos0 + t]``.  Returns the rotated q -- in ``q_out`` (which may be q), new
-    memory otherwise; q itself without ``rope`` or with one of no columns.  Blocks that fill up are quantised in the same call."""
+    memory otherwise; q itself without ``rope`` or with one of no columns.  Blocks that fill up are quantised in the same call.
+    (A device-side pos0 below 0 does nothing at all; rows at the cache's end and behind it are dropped.)"""
     cache, code, B, H, n_max, d, dtype = _kv8(kv)
     q_len = k.shape[1] if k.dim() == 4 else 0
     kr, k_heads = _kv8_rows(k, "k", B, q_len, d, dtype)

@@ -246,7 +246,7 @@ int bt_topk_sample(int dtype, int64_t M, int64_t V, const void* logits, int64_t 
 /* codes[m, :] = x[m, :] quantised with ONE scale per row, scales[m] = s; with ln_w / ln_b the row is LayerNorm(x[m, :]; ln_w, ln_b, eps),
  * held in fp32 and not rounded to `dtype` in between.  Columns K .. round_up(K, 16) - 1 are written as 0, so a row of codes is a whole
  * number of 16-byte units: pass round_up(K, 16) as K to bt_linear_q8.  ldc >= round_up(K, 16), ldc % 16 == 0, codes 16-byte aligned; x
- * may have any row stride.  A row that holds an infinity or NaN gets codes 0 and scale NaN: whatever is computed from it is NaN, as it
+ * may have any row stride of K or more.  A row that holds an infinity or NaN gets codes 0 and scale NaN: whatever is computed from it is NaN, as it
  * would be from the row itself.  Also lays out weights: W[N, K] gives one scale per output channel. */
 int bt_quant_rows(int dtype, int64_t M, int64_t K, const void* x, int64_t ldx, const void* ln_w, const void* ln_b, float eps,
                   int8_t* codes, int64_t ldc, float* scales, bt_stream stream);
@@ -292,9 +292,11 @@ typedef struct bt_kv8_rows {
 
 /* Append q_len rows of k and v at rows pos0 .. pos0 + q_len - 1 (rows [0, pos0) are there already) and rotate q:
  *   pos0 = pos0_dev ? *pos0_dev : pos0_host, angle position = pos_table ? pos_table[pos0 + t] : pos0 + t (clamped to the tables' max_pos
- *   rows), partial RoPE over the first `rot` dims of q and k as in bt_rope_kv_append, computed in 64 bits and rounded once.
+ *   rows), partial RoPE over the first `rot` dims of q and k as in bt_rope_kv_append, computed in 64 bits and rounded to fp32 and from there
+ *   to `dtype`.
  * q -> q_out (heads query heads; may be the same memory; both NULL: only k and v).  rot == 0: no rotation, q must be NULL.  Rows at
- * n_max and beyond, which only a device-side pos0 can reach, are dropped. */
+ * n_max and beyond, which only a device-side pos0 can reach, are dropped, but their queries are rotated all the same; a device-side pos0
+ * below 0 leaves everything as it is, q_out too. */
 int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len, int32_t heads, const bt_kv8_rows* q, const bt_kv8_rows* q_out,
                   const bt_kv8_rows* k, const bt_kv8_rows* v, const int32_t* pos0_dev, int32_t pos0_host, const int32_t* pos_table,
                   int32_t rot, const float* cos_tab, const float* sin_tab, int64_t max_pos, bt_stream stream);
