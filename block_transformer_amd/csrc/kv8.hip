@@ -968,7 +968,8 @@ static int check_cache(const char* who, int dtype, const bt_kv8_cache* c, int* s
                  sizeof(bt_kv8_cache));
     BT_CHECK_ARG(c->block == 16 || c->block == 32 || c->block == 64, "%s: block %d is not 16, 32 or 64", who, c->block);
     BT_CHECK_ARG(c->head_dim == 32 || c->head_dim == 64 || c->head_dim == 128, "%s: head_dim %d not instantiated", who, c->head_dim);
-    BT_CHECK_ARG(c->batch >= 0 && c->kv_heads > 0 && c->batch * c->kv_heads < (1ll << 31), "%s: bad batch or kv_heads", who);
+    BT_CHECK_ARG(c->batch >= 0 && c->kv_heads > 0 && c->batch < (1ll << 31) && c->batch * c->kv_heads < (1ll << 31),
+                 "%s: bad batch or kv_heads", who);
     BT_CHECK_ARG(c->n_max > 0 && c->n_max % c->block == 0 && c->n_max < (1ll << 30), "%s: n_max %lld is not a multiple of the block", who,
                  (long long)c->n_max);
     *shift = c->block == 16 ? 4 : c->block == 32 ? 5 : 6;
@@ -1024,15 +1025,17 @@ extern "C" int bt_kv8_append(int dtype, const bt_kv8_cache* cache, int32_t q_len
     a.q_out = rows_of(q_out);
     a.k = rows_of(k);
     a.v = rows_of(v);
-    a.blocks = pos0_dev ? (q_len + cache->block - 2) / cache->block + 1
+    a.blocks = pos0_dev ? (int)(((int64_t)q_len + cache->block - 2) / cache->block) + 1
                         : (int)(((int64_t)pos0_host + q_len - 1) / cache->block - pos0_host / cache->block) + 1;
     // Blocks that fill up have a wave for K and one for V, steps that fill none (or may: the device knows) one for both: 32 x 509 rows 88 us
     // and 97, 8 x 100 9.8 and 14.9; a step of 256 sequences that fills no block 9.8 and 7.5, and of a step whose position the device
     // reads, one row at a time, at most one in 16 fills its blocks.
     a.split = pos0_dev ? q_len > 1 : ((int64_t)pos0_host + q_len) / cache->block > pos0_host / cache->block;
-    const int64_t kv_items = (cache->batch * cache->kv_heads * a.blocks) << a.split, q_rows = q ? cache->batch * q_len * heads : 0;
+    const int64_t kv_items = (cache->batch * cache->kv_heads * a.blocks) << a.split;
+    BT_CHECK_ARG(!q || (double)cache->batch * q_len * heads < (double)(1 << 30), "bt_kv8_append: too many rows for one call");
+    const int64_t q_rows = q ? cache->batch * q_len * heads : 0;
     const int V = dtype == BT_BF16 ? 8 : 4;
-    BT_CHECK_ARG(kv_items < (1ll << 25) && q_rows < (1ll << 30) && ceil_div(q_rows * cache->head_dim, 256 * V) < (1ll << 25),
+    BT_CHECK_ARG(kv_items < (1ll << 25) && ceil_div(q_rows * cache->head_dim, 256 * V) < (1ll << 25),
                  "bt_kv8_append: too many rows for one call");      // (2^32 threads)
     a.kv_items = (uint32_t)kv_items;
     a.q_rows = (uint32_t)q_rows;
@@ -1061,7 +1064,8 @@ extern "C" int bt_kv8_read(int dtype, const bt_kv8_cache* cache, int64_t n, int6
                            bt_stream stream) {
     int shift;
     BT_TRY(check_cache("bt_kv8_read", dtype, cache, &shift));
-    BT_CHECK_ARG(n >= 0 && n <= cache->n_max && first >= 0 && count >= 0 && first + count <= n, "bt_kv8_read: rows out of range");
+    BT_CHECK_ARG(n >= 0 && n <= cache->n_max && first >= 0 && count >= 0 && first <= n && count <= n - first,
+                 "bt_kv8_read: rows out of range");
     BT_CHECK_ARG((!k_out || aligned16(k_out)) && (!v_out || aligned16(v_out)), "bt_kv8_read: outputs must be 16-byte aligned");
     if (cache->batch == 0 || count == 0 || (!k_out && !v_out)) return BT_OK;
     const int blocks = (int)((first + count - 1) / cache->block - first / cache->block) + 1;
@@ -1123,7 +1127,7 @@ extern "C" int bt_attention_kv8(int dtype, const bt_kv8_cache* cache, int32_t q_
     a.n_split = n_split;
     a.part = n_split > 1 ? (float*)ws : nullptr;
     const int64_t groups = cache->batch * cache->kv_heads * a.row_groups;
-    BT_CHECK_ARG(groups * n_split < (1ll << 26) && (n_split == 1 || cache->batch * cache->kv_heads * a.rows < (1ll << 24)),
+    BT_CHECK_ARG(groups < (1ll << 26) && groups * n_split < (1ll << 26) && (n_split == 1 || cache->batch * cache->kv_heads * a.rows < (1ll << 24)),
                  "bt_attention_kv8: grid too large");      // (2^32 threads)
     a.pos0_host = pos0_host;
     a.pos0_dev = pos0_dev;

@@ -91,3 +91,20 @@ def test_launches_of_more_threads_than_32_bits_count():
     refused(lib.bt_kv8_read(1, cache(1 << 20, 1024), 1024, 0, 1024, p, p, None), b"too large")
     refused(lib.bt_attention_kv8(1, cache(1 << 26, 16), 1, 1, rows, None, 0, None, 0, p, 32, 1, None, 0, None), b"too large")
     refused(lib.bt_attention_kv8(1, cache(1 << 24, 16), 1, 1, rows, None, 0, None, 0, p, 32, 2, p, 1 << 60, None), b"too large")
+
+
+def test_sizes_whose_products_leave_64_bits():
+    """They would pass for small ones.  (No pointer is followed.)"""
+    p, lib = 0x1000, _lib.lib()
+
+    def refused(rc, text):
+        assert rc in (-1, -3) and text in lib.bt_last_error(), (rc, lib.bt_last_error())
+
+    rows = _lib.bt_kv8_rows(p, 32, 32, 32)
+    cache = lambda batch, heads, n_max: _lib.bt_kv8_cache(16, heads, 32, batch, n_max, p, p, p, p, p, p)  # noqa: E731
+    refused(lib.bt_kv8_read(1, cache(1, 1, 64), 10, 1 << 62, 1 << 62, p, p, None), b"out of range")
+    refused(lib.bt_kv8_read(1, cache(1 << 62, 4, 64), 10, 0, 1, p, p, None), b"bad batch")
+    refused(lib.bt_kv8_append(1, cache(1, 1, 64), 1 << 30, 1 << 30, rows, rows, rows, rows, p, 0, None, 2, p, p, 64, None), b"too many")
+    refused(lib.bt_kv8_append(1, cache(1 << 20, 1, 64), 1 << 16, 1 << 28, rows, rows, rows, rows, p, 0, None, 2, p, p, 64, None), b"too many")
+    refused(lib.bt_attention_kv8(1, cache(1 << 20, 1, 1 << 20), 1 << 19, 1 << 10, rows, None, 0, None, 0, p, 1 << 15, 1 << 30, p, 1 << 62, None),
+            b"too large")
