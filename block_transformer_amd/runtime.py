@@ -69,7 +69,8 @@ class KVCache:
 class KV8Cache:
     """A KV cache in 8 bits: codes with one scale per (layer, sequence, head, block of ``block`` rows), the open block's rows in ``dtype``
     (layout: bt_kv8_cache in include/bt_hip.h).  About half the memory of a bf16 ``KVCache``; ``cache[layer]`` is what ``ops.kv8_append``,
-    ``ops.kv8_read`` and ``ops.attention_kv8`` take."""
+    ``ops.kv8_read`` and ``ops.attention_kv8`` take.  Rows can be taken back (by the next pos0) inside the open block or to the start of any
+    block: of a full block only codes are left."""
 
     def __init__(self, layers: int, batch: int, kv_heads: int, n_max: int, head_dim: int, dtype, device, block: int = 16):
         if block not in (16, 32, 64):

@@ -267,8 +267,10 @@ int bt_linear_q8(int dtype, int64_t M, int64_t N, int64_t K, const int8_t* A, in
  *   k_scale, v_scale  [batch][kv_heads][n_max / block]       k_tail   [batch][kv_heads][block][head_dim]   (dtype)
  *                                                            v_tail   [batch][kv_heads][head_dim][block]   (dtype)
  * A block is quantised when its last row arrives; until then its rows stand in the tail as they came, in `dtype`.  So what the cache
- * holds depends on the rows alone, not on how many came at a time, and no row is rounded twice.  V is kept token-innermost because the
- * product with the probabilities runs over tokens: a matrix instruction's operand is then one 16-byte load.
+ * holds depends on the rows alone, not on how many came at a time, and no row is rounded twice.  A cache of n rows is read and appended
+ * to as one of n rows: of a full block only codes are left, so rows can be taken back (by the next pos0) inside the open block or to the
+ * start of any block, nowhere else.  V is kept token-innermost because the product with the probabilities runs over tokens: a matrix
+ * instruction's operand is then one 16-byte load.
  * An infinity or NaN does not count for its block's scale; it is stored as +-127 or 0 (one row, masked or not, must not spoil the rows
  * it shares a scale with).  In the tail, and so in attention over the open block, it stands as it came. */
 typedef struct bt_kv8_cache {

@@ -63,3 +63,20 @@ def test_attention_with_one_mask_for_all_sequences():
     for m in (mask, mask.to(torch.uint8)):
         got = ops.attention_kv8(x[:, -1:, 0], kv, n - 1, mask=m.expand(B, n))
         assert torch.equal(got, ops.attention_kv8(x[:, -1:, 0], kv, n - 1, mask=m.repeat(B, 1)))
+
+
+@pytest.mark.parametrize("back_to", [70, 65, 64, 48, 16, 0])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rows_taken_back(back_to, dtype):
+    """Inside the open block (64 .. 70) or to the start of any block: the cache is that of the rows that stayed and those that came."""
+    B, H, d, n = 2, 2, 64, 71
+    x = torch.randn(B, 2 * n, 2, H, d, generator=torch.Generator().manual_seed(3)).to(dtype).to(DEV)
+    a, b = (KV8Cache(1, B, H, 2 * n, d, dtype, DEV)[0] for _ in range(2))
+    ops.kv8_append(a, None, x[:, :n, 0], x[:, :n, 1], 0)
+    ops.kv8_append(a, None, x[:, n:, 0], x[:, n:, 1], back_to)
+    rows = torch.cat([x[:, :back_to], x[:, n:]], 1)
+    ops.kv8_append(b, None, rows[:, :, 0], rows[:, :, 1], 0)
+    for s, t in zip(ops.kv8_read(a, back_to + n), ops.kv8_read(b, back_to + n)):
+        assert torch.equal(s, t)
+    q = x[:, :1, 0]
+    assert torch.equal(ops.attention_kv8(q, a, back_to + n - 1), ops.attention_kv8(q, b, back_to + n - 1))
