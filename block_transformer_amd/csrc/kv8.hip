@@ -436,11 +436,12 @@ __global__ __launch_bounds__(256) void kv8_read_kernel(bt_kv8_cache c, int64_t n
 //   O^T = V^T P^T B = P: the lane's own 16 rows are two operands: nothing moves between lanes.
 //                 A = V^T: lane m holds the same 16 consecutive rows of dim 16 j + m, one 16-byte load from v_codes.
 // Softmax: a running (max, sum, output) in fp32.  The open block is one more tile, its rows as they stand (fp32: v_mfma_f32_16x16x4_f32).
-// Bound by reading the cache where there is enough of it: 1024 sequences x 16 heads of 128 x 543 rows 407 .. 421 us (5.6 .. 5.8 TB/s; the
-// card reads 6.0), 256 sequences 113 .. 119 us (5.2), 4 sequences x 32773 rows, 8 heads to a KV head, 30 us with the join (4.5).  A tile
-// costs about 710 vector instructions (over half of them turn codes into bf16) and 64 matrix instructions for its 16 KB, under half of
-// what would bound it; with one wave to a SIMD that shows: 8 sequences x 24608 rows x 2 heads of 64, 20 query rows each, 24 us, where the
-// fixed-point form took 20.5.  One sequence of 21 rows: 6.2 us, three round trips to memory.
+// Bound by reading the cache where there is enough of it: 1024 sequences x 16 heads of 128 x 543 rows 401 .. 429 us by card (5.5 .. 5.9 TB/s;
+// the card reads 6.0), 256 sequences 111 .. 120 us (4.9 .. 5.3), 4 sequences x 32773 rows, 8 heads to a KV head, 30 us with the join (4.5),
+// fp32, 128 sequences, 61 .. 68 us (4.2 .. 4.7).  A tile costs about 710 vector instructions (over half of them turn codes into bf16) and 64
+// matrix instructions for its 16 KB, under half of what would bound it; with one wave to a SIMD that shows: 8 sequences x 24608 rows x 2 heads
+// of 64, 20 query rows each, 24 us, where a fixed point for a tile took 20.5.  One sequence of 21 rows: 6.2 us, three round trips to memory.
+// 32 prompts of 512 rows 222 us: every 16 query rows read K and V for themselves.
 typedef int i32x2 __attribute__((ext_vector_type(2)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

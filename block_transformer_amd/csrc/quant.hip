@@ -560,11 +560,11 @@ __global__ __launch_bounds__(256, 2) void linear_q8_tile_kernel(Q8Args e) {
 //  * A tile ends with one more barrier for group 0 (group 1 has then read its last) and begins with one more for group 1, so the two
 //    epilogues run side by side.
 //  * A row of 128 bytes has its 16-byte pieces in the order p ^ (row & 7).
-// One launch after another in a graph, on a card that is cool: 8192 x 8192 x 2048 131 us (2.1 POPS), with GELU 141 us, 8192 x 8192 x 8192
+// Launch after launch in a graph: 8192 x 8192 x 2048 131 us (2.1 POPS), with GELU 141 .. 152 us by card, 8192 x 8192 x 8192
 // 398 us (2.8 POPS, matrix units busy two thirds of the time at the 1.8 GHz that the card then holds); of the 131 us, 107 are the products,
-// 10 the stores and 14 the rest of the epilogue.  4096 x 2048 x 8192 by 256 x 128 65 us (2.1 POPS; by 128 x 128 77, by 256 x 256 on half
-// the CUs 80).  Single launches under the profiler, on several cards: 156, 425 and 77 .. 85 us.  fp32 results: 186 us with GELU, 4096 x 2048 x
-// 8192 77 us; the 256 x 256 form has six registers too few there and brings its load offsets back from scratch at a tile's start, which
+// 10 the stores and 14 the rest of the epilogue.  4096 x 2048 x 8192 by 256 x 128 65 .. 72 us (2.1 POPS; by 128 x 128 77, by 256 x 256 on
+// half the CUs 80).  Single launches under the profiler: 156 with GELU, 425 and 77 .. 85 us.  fp32 results: 176 us with GELU, 4096 x 2048 x
+// 8192 74 us; the 256 x 256 form has six registers too few there and brings its load offsets back from scratch at a tile's start, which
 // waits for every load that is out.
 template <typename T, int NB>
 __global__ __launch_bounds__(512, 2) void linear_q8_big_kernel(Q8Args e) {
